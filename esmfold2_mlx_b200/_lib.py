@@ -82,6 +82,39 @@ class TmuPairCondWeights(ctypes.Structure):
     _fields_ = [("ln_w", _vp), ("ln_b", _vp), ("proj", _vp), ("n_transitions", _i),
                 ("transitions", ctypes.POINTER(TmuCondTransitionWeights)), ("bias_w", _vp), ("bias_b", _vp)]
 
+
+TMU_F16, TMU_BF16, TMU_F32, TMU_E4M3 = 0, 1, 2, 3
+TMU_NORM_NONE, TMU_NORM_RMS, TMU_NORM_LAYER = 0, 1, 2
+
+
+class TmuHeads(ctypes.Structure):
+    """Mirror of ``tmu_heads``."""
+
+    _fields_ = [("data", _vp), ("stride_token", ctypes.c_longlong), ("stride_head", ctypes.c_longlong)]
+
+
+class TmuQkNorm(ctypes.Structure):
+    """Mirror of ``tmu_qk_norm``."""
+
+    _fields_ = [("kind", _i), ("eps", _f), ("q_weight", _vp), ("q_bias", _vp), ("k_weight", _vp), ("k_bias", _vp)]
+
+
+class TmuRotary(ctypes.Structure):
+    """Mirror of ``tmu_rotary``."""
+
+    _fields_ = [("positions", _vp), ("position_bytes", _i), ("turns", _vp), ("gain", _f), ("rot", _i),
+                ("interleaved", _i)]
+
+
+class TmuAttnBias(ctypes.Structure):
+    """Mirror of ``tmu_attn_bias``."""
+
+    _fields_ = [("data", _vp), ("stride_seq", ctypes.c_longlong), ("stride_head", ctypes.c_longlong),
+                ("stride_row", ctypes.c_longlong), ("n", _i)]
+
+
+_H = ctypes.POINTER(TmuHeads)
+_ll = ctypes.c_longlong
 _W = ctypes.POINTER(TmuTrimulWeights)
 _G = ctypes.POINTER(TmuPairLayout)
 _TW = ctypes.POINTER(TmuTransitionWeights)
@@ -116,6 +149,12 @@ SIGNATURES = {
                            _sz, _vp, _vp]),
     "tmu_parcae_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmu_parcae_step": (_i, [_vp, _vp, _vp, ctypes.POINTER(TmuParcaeWeights), _vp, _i, _i, _i, _vp, _sz, _vp, _vp]),
+    "tmu_qk_norm_rope": (_i, [_H, _H, _H, _H, ctypes.POINTER(TmuQkNorm), ctypes.POINTER(TmuRotary), _i, _i, _i, _i, _i,
+                              _vp]),
+    "tmu_attention": (_i, [_H, _H, _H, _H, _vp, ctypes.POINTER(TmuAttnBias), _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
+    "tmu_quantize_rows": (_i, [_vp, _i, _ll, _i, _i, _vp, _vp, _vp]),
+    "tmu_linear_fp8_workspace_bytes": (_sz, [_i, _i, _i]),
+    "tmu_linear_fp8": (_i, [_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _i, _ll, _i, _i, _i, _vp, _sz, _vp, _vp]),
     "tmu_ipc_export": (_i, [_vp, _vp, ctypes.POINTER(_ull)]),
     "tmu_ipc_import": (_i, [_vp, _ull, ctypes.POINTER(_vp)]),
     "tmu_ipc_close": (_i, [_vp]),

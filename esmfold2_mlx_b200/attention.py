@@ -1,0 +1,271 @@
+"""Attention over packed sequences, and the norm and rotation of its queries and keys (K7, K8).
+
+The sequence dimension's side of the model: the diffusion head's token transformer, whose additive
+pair biases :func:`pair_cond.pair_biases` makes (``mlx_diffusion.py:259,369``), and the language
+model in front of the trunk (``mlx_esmc.py``).  Tokens of all sequences lie behind one another,
+``[T, heads, D]``, and ``cu_seqlens`` says where each sequence begins, so nothing is padded.
+
+    q, k = qk_norm_rope(q, k, positions, rotary, norm="layer", q_weight=..., k_weight=...)
+    o = attention(q, k, v, cu_seqlens)
+
+``q``, ``k`` and ``v`` may be slices of one fused projection: the values of a head are contiguous and
+the other strides are multiples of 8 elements.  Launches go on the current stream of the tensors'
+device; nothing synchronises.  Inference only: an input that asks for gradients is refused.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .ops import _ptr, _stream_ptr
+
+_DTYPES = {torch.float16: _lib.TMU_F16, torch.bfloat16: _lib.TMU_BF16}
+_NORMS = {None: _lib.TMU_NORM_NONE, "rms": _lib.TMU_NORM_RMS, "layer": _lib.TMU_NORM_LAYER}
+
+
+def refuse_grad(where: str, *tensors) -> None:
+    """Raise if autograd would expect a gradient from an operator that has none."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{where} has no backward pass: call it under torch.no_grad() or detach its inputs")
+
+
+def spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges that two strided tensors reach over meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+
+    def span(t):
+        return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    return a.data_ptr() < b.data_ptr() + span(b) and b.data_ptr() < a.data_ptr() + span(a)
+
+
+def _check_heads(name: str, t: torch.Tensor, T: int, D: int, like: torch.Tensor) -> None:
+    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D:
+        raise ValueError(f"{name} must be [{T}, heads, {D}], got {tuple(t.shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must have q's type and device")
+    if D > 1 and t.stride(2) != 1:
+        raise ValueError(f"the values of a head of {name} must be contiguous")
+
+
+def _heads(t: torch.Tensor) -> _lib.TmuHeads:
+    # an axis of length one is never stepped along: its stride is whatever the view happened to have
+    return _lib.TmuHeads(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _check_first(name: str, q: torch.Tensor) -> int:
+    if not q.is_cuda or q.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be a CUDA fp16 or bf16 tensor")
+    if q.dim() != 3:
+        raise ValueError(f"{name} must be [T, heads, D], got {tuple(q.shape)}")
+    return _DTYPES[q.dtype]
+
+
+class Rotary:
+    """Rotary position embedding of the first ``rot`` values of a head: pair i turns by
+    ``position * base ** (-2 i / rot)`` radians.
+
+    ``layout`` pairs (i, i + rot / 2) as ``"half"`` and (2 i, 2 i + 1) as ``"interleaved"``.
+    ``scaling`` stretches it to contexts longer than the trained one:
+
+    * ``{"type": "linear", "factor": s}``: every frequency divided by s.
+    * ``{"type": "ntk", "factor": s}``: base times ``s ** (rot / (rot - 2))``, which leaves the fastest
+      pair and divides the slowest by s.
+    * ``{"type": "yarn", "factor": s, "original_length": n, "beta_fast": 32, "beta_slow": 1,
+      "gain": 0.1 ln s + 1}``: pairs that turn more than ``beta_fast`` times over n positions stay, those
+      below ``beta_slow`` are divided by s, with a linear ramp over the pair index between, and the
+      rotated values are multiplied by ``gain``.
+
+    Frequencies are kept as turns a position in 64-bit fixed point, so no position is too far: the
+    angle is exact to 2^-32 of a turn for every 64-bit position, negative ones included."""
+
+    def __init__(self, rot: int, base: float = 10000.0, layout: str = "half", scaling: dict | None = None,
+                 device="cuda"):
+        if rot < 16 or rot % 16:
+            raise ValueError("rot must be a positive multiple of 16")
+        if layout not in ("half", "interleaved"):
+            raise ValueError("layout must be 'half' or 'interleaved'")
+        self.rot, self.base, self.layout = int(rot), float(base), layout
+        self.gain = 1.0
+        self.frequencies = self._frequencies(scaling)  # radians a position
+        fixed = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequencies]
+        signed = [f - 2**64 if f >= 2**63 else f for f in fixed]
+        self.turns = torch.tensor(signed, dtype=torch.int64).to(device)
+
+    def _frequencies(self, scaling: dict | None) -> list[float]:
+        half, base = self.rot // 2, self.base
+        kind = None if scaling is None else scaling.get("type")
+        if kind not in (None, "linear", "ntk", "yarn"):
+            raise ValueError(f"unknown scaling {kind!r}")
+        s = 1.0 if kind is None else float(scaling["factor"])
+        if s <= 0.0 or base <= 1.0:
+            raise ValueError("the factor must be positive and the base above 1")
+        if kind == "ntk":
+            base *= s ** (self.rot / (self.rot - 2))
+        freq = [base ** (-i / half) for i in range(half)]
+        if kind == "linear":
+            return [f / s for f in freq]
+        if kind == "yarn":
+            n = float(scaling["original_length"])
+
+            def pair_at(turns):  # the pair index that turns `turns` times over n positions
+                return half * math.log(n / (turns * 2.0 * math.pi)) / math.log(base)
+
+            lo = max(math.floor(pair_at(float(scaling.get("beta_fast", 32.0)))), 0)
+            hi = min(math.ceil(pair_at(float(scaling.get("beta_slow", 1.0)))), self.rot - 1)
+            self.gain = float(scaling.get("gain", 0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0))
+            ramp = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(half)]
+            return [f * (1.0 - r) + f / s * r for f, r in zip(freq, ramp)]
+        return freq
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | None = None, rotary: Rotary | None = None,
+                 *, norm: str | None = None, q_weight=None, k_weight=None, q_bias=None, k_bias=None,
+                 eps: float = 1e-5, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
+    """K8: the norm of every head of ``q`` [T, Hq, D] and ``k`` [T, Hkv, D] over its D values, then the
+    rotation by ``positions`` [T] (int32 or int64), in one pass; returns ``(q_out, k_out)``.
+
+    ``norm`` is None, ``"rms"`` or ``"layer"``, with fp32 weights and biases [D] (None: 1 and 0); without
+    ``rotary`` only the norm is applied.  D is a multiple of 16, at most 256.  ``q_out`` may be ``q`` and
+    ``k_out`` may be ``k``; other overlaps are refused."""
+    dtype = _check_first("q", q)
+    T, hq, D = q.shape
+    _check_heads("k", k, T, D, q)
+    _check_heads("q", q, T, D, q)
+    if norm not in _NORMS:
+        raise ValueError("norm must be None, 'rms' or 'layer'")
+    refuse_grad("qk_norm_rope", q, k, q_weight, k_weight, q_bias, k_bias)
+    for name, p in (("q_weight", q_weight), ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias)):
+        if p is not None:
+            if norm is None:
+                raise ValueError(f"{name} needs a norm")
+            if p.dtype != torch.float32 or p.device != q.device or p.shape != (D,) or not p.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous fp32 [{D}] tensor on q's device")
+    rot = _lib.TmuRotary(None, 4, None, 1.0, 0, 0)
+    if rotary is not None:
+        if rotary.rot > D:
+            raise ValueError(f"the rotary's {rotary.rot} values exceed the head's {D}")
+        if positions is None:
+            raise ValueError("a rotary needs positions")
+        if (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (T,)
+                or positions.device != q.device or not positions.is_contiguous()):
+            raise ValueError(f"positions must be a contiguous int32 or int64 [{T}] tensor on q's device")
+        if rotary.turns.device != q.device:
+            raise ValueError("the rotary must be on q's device")
+        rot = _lib.TmuRotary(positions.data_ptr(), positions.element_size(), rotary.turns.data_ptr(), rotary.gain,
+                             rotary.rot, 1 if rotary.layout == "interleaved" else 0)
+    for name, src, dst in (("q_out", q, q_out), ("k_out", k, k_out)):
+        if dst is not None:
+            _check_heads(name, dst, T, D, q)
+            if dst.shape != src.shape:
+                raise ValueError(f"{name} must be shaped like its input")
+            if _self_overlap(dst):
+                raise ValueError(f"{name} must not overlap itself")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k_out is None else k_out
+    if _heads_overlap(q_out, k_out):
+        raise ValueError("q_out and k_out must not overlap")
+    for name, src, dst in (("q_out and q", q, q_out), ("k_out and k", k, k_out), ("q_out and k", k, q_out),
+                           ("k_out and q", q, k_out)):
+        same = src.data_ptr() == dst.data_ptr() and src.stride() == dst.stride() and src.shape == dst.shape
+        own = name in ("q_out and q", "k_out and k")
+        if _heads_overlap(src, dst) and not (same and own):
+            raise ValueError(f"{name} must not overlap")
+    nrm = _lib.TmuQkNorm(_NORMS[norm], float(eps), _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias))
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.load().tmu_qk_norm_rope(_heads(q), _heads(k), _heads(q_out), _heads(k_out), nrm, rot, T, hq,
+                                                k.shape[1], D, dtype, _stream_ptr(q.device)), "tmu_qk_norm_rope")
+    return q_out, k_out
+
+
+def _self_overlap(t: torch.Tensor) -> bool:
+    """Whether two heads of a [T, H, D] view share memory (exact for non-negative strides)."""
+    (T, H, D), (st, sh, _) = t.shape, t.stride()
+    axes = sorted((s, n) for s, n in ((st, T), (sh, H)) if n > 1)
+    span = D
+    for s, n in axes:
+        if s < span:
+            return True
+        span = s * (n - 1) + span
+    return False
+
+
+def _heads_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [T, H, D] views share memory.  Views of one projection interleave without
+    sharing: with one token stride, their heads' ranges are compared within a token."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+
+    if not spans_overlap(a, b):
+        return False
+
+    def token_span(t):
+        return (sum((t.shape[i] - 1) * t.stride(i) for i in (1, 2)) + 1) * t.element_size()
+
+    step = a.stride(0) * a.element_size()
+    wa, wb = token_span(a), token_span(b)
+    if a.shape[0] > 1 and a.stride(0) == b.stride(0) and step >= max(wa, wb):
+        off = (b.data_ptr() - a.data_ptr()) % step  # b's heads begin `off` bytes behind a's in each period
+        return off < wa or off + wb > step
+    return True
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *, causal: bool = False,
+              scale: float | None = None, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              status: torch.Tensor | None = None) -> torch.Tensor:
+    """K7: softmax attention within each packed sequence: ``q`` [T, Hq, D], ``k`` and ``v`` [T, Hkv, D]
+    (Hq a multiple of Hkv: query head h reads key head h // (Hq / Hkv)), ``cu_seqlens`` int32 [S + 1]
+    on the device, ascending; returns ``out`` [T, Hq, D].
+
+    ``scale`` defaults to 1 / sqrt(D).  ``bias`` [S or 1, Hq, n, n] of q's type is added to the scaled
+    scores of each sequence's first n positions (``pair_cond.pair_biases(...)[block]`` with a sequence a
+    fold, or with one fold's bias for all of its samples); -inf hides a key, and a row whose keys are
+    all hidden comes out as 0.  D is a multiple of 8, at most 128.  Tokens past the last sequence are
+    left as they were in ``out`` (unset in a new one).  A hidden key's value is multiplied by a weight
+    of 0, so an infinity or NaN there still reaches the rows of its own sequence; other sequences and
+    tokens of no sequence have no influence."""
+    dtype = _check_first("q", q)
+    T, hq, D = q.shape
+    _check_heads("q", q, T, D, q)
+    _check_heads("k", k, T, D, q)
+    _check_heads("v", v, T, D, q)
+    if v.shape != k.shape:
+        raise ValueError("k and v must have the same heads")
+    refuse_grad("attention", q, k, v, bias)
+    if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1
+            or cu_seqlens.device != q.device or not cu_seqlens.is_contiguous()):
+        raise ValueError("cu_seqlens must be a contiguous int32 [S + 1] tensor on q's device")
+    S = cu_seqlens.numel() - 1
+    b = None
+    if bias is not None:
+        if (bias.dim() != 4 or bias.shape[0] not in (1, S) or bias.shape[1] != hq or bias.shape[2] != bias.shape[3]
+                or bias.dtype != q.dtype or bias.device != q.device):
+            raise ValueError(f"bias must be [1 or {S}, {hq}, n, n] of q's type on its device")
+        n = bias.shape[2]
+        if n > 1 and bias.stride(3) != 1:
+            raise ValueError("the last axis of bias must be contiguous")
+        b = _lib.TmuAttnBias(bias.data_ptr(), bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1),
+                             bias.stride(2), n)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _check_heads("out", out, T, D, q)
+        if out.shape != q.shape:
+            raise ValueError("out must be shaped like q")
+        if _self_overlap(out) or any(_heads_overlap(out, t) for t in (q, k, v)):
+            raise ValueError("out must not overlap itself, q, k or v")
+        if bias is not None and spans_overlap(out, bias):
+            raise ValueError("out must not overlap bias")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.load().tmu_attention(_heads(q), _heads(k), _heads(v), _heads(out), _ptr(cu_seqlens), b, S, T, hq,
+                                             k.shape[1], D, dtype, 1 if causal else 0, scale, _ptr(status),
+                                             _stream_ptr(q.device)), "tmu_attention")
+    return out

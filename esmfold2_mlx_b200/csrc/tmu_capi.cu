@@ -21,6 +21,9 @@
 #include "k4_transition.cuh"
 #include "k5_disto.cuh"
 #include "k6_gemm.cuh"
+#include "k7_attention.cuh"
+#include "k8_qk_rope.cuh"
+#include "k9_linear8.cuh"
 #include "tmu.h"
 
 using namespace tmu;
@@ -1477,3 +1480,5 @@ int tmu_selftest_wait_timeout(void* status, unsigned long long timeout_ns, void*
 }
 
 }  // extern "C"
+
+#include "tmu_seq_host.cuh"

@@ -1,0 +1,229 @@
+// Host side of the sequence operators (tmu_attention, tmu_qk_norm_rope, tmu_quantize_rows,
+// tmu_linear_fp8): argument checks and launches.  Included by tmu_capi.cu, whose helpers it uses.
+#pragma once
+
+namespace {
+
+// A [T, H, D] view of 16-bit values that 16-byte accesses can read: aligned base and strides.
+int check_heads(const void* p, long long st, long long sh, const char* what) {
+  if (p == nullptr) return fail(TMU_ERR_INVALID_ARGUMENT, what);
+  if (!aligned16(p) || st % 8 || sh % 8) return fail(TMU_ERR_MISALIGNED, what);
+  if (st < 0 || sh < 0) return fail(TMU_ERR_INVALID_ARGUMENT, what);
+  return TMU_OK;
+}
+
+int check_packed(int T, int hq, int hkv, int D) {
+  if (T < 0 || hq < 1 || hkv < 1 || D < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "T, heads and D must be positive");
+  return TMU_OK;
+}
+
+template <typename T, int LPH, int NORM>
+void (*k8_kernel(bool inter))(k8::Params) {
+  return inter ? k8::qk_rope_kernel<T, LPH, NORM, true> : k8::qk_rope_kernel<T, LPH, NORM, false>;
+}
+
+template <typename T, int LPH>
+void (*k8_kernel(int norm, bool inter))(k8::Params) {
+  if (norm == TMU_NORM_NONE) return k8_kernel<T, LPH, k8::kNone>(inter);
+  return norm == TMU_NORM_RMS ? k8_kernel<T, LPH, k8::kRms>(inter) : k8_kernel<T, LPH, k8::kLayer>(inter);
+}
+
+template <typename T>
+void (*k8_kernel(int lph, int norm, bool inter))(k8::Params) {
+  switch (lph) {
+    case 2: return k8_kernel<T, 2>(norm, inter);
+    case 4: return k8_kernel<T, 4>(norm, inter);
+    case 8: return k8_kernel<T, 8>(norm, inter);
+    case 16: return k8_kernel<T, 16>(norm, inter);
+    default: return k8_kernel<T, 32>(norm, inter);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int tmu_qk_norm_rope(const tmu_heads* q, const tmu_heads* k, const tmu_heads* q_out, const tmu_heads* k_out,
+                     const tmu_qk_norm* norm, const tmu_rotary* rot, int T, int Hq, int Hkv, int D, int dtype,
+                     void* stream) {
+  if (!q || !k || !q_out || !k_out || !norm || !rot) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+  int st = check_packed(T, Hq, Hkv, D);
+  if (st) return st;
+  if (D % 16 || D > 256) return fail(TMU_ERR_UNSUPPORTED, "D must be a multiple of 16, at most 256");
+  if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
+  if (norm->kind < TMU_NORM_NONE || norm->kind > TMU_NORM_LAYER) return fail(TMU_ERR_INVALID_ARGUMENT, "norm kind");
+  if (rot->rot < 0 || rot->rot > D || rot->rot % 16)
+    return fail(TMU_ERR_UNSUPPORTED, "the rotated part must be a multiple of 16, at most D");
+  if (rot->rot > 0 && (!rot->positions || !rot->turns)) return fail(TMU_ERR_INVALID_ARGUMENT, "positions or turns is NULL");
+  if (rot->position_bytes != 4 && rot->position_bytes != 8) return fail(TMU_ERR_INVALID_ARGUMENT, "position_bytes must be 4 or 8");
+  if (T == 0) return TMU_OK;
+  const tmu_heads* views[4] = {q, k, q_out, k_out};
+  static const char* const names[4] = {"q", "k", "q_out", "k_out"};
+  for (int i = 0; i < 4; ++i)
+    if ((st = check_heads(views[i]->data, views[i]->stride_token, views[i]->stride_head, names[i]))) return st;
+  const float* par[4] = {norm->q_weight, norm->q_bias, norm->k_weight, norm->k_bias};
+  for (const float* x : par)
+    if (x != nullptr && !aligned16(x)) return fail(TMU_ERR_MISALIGNED, "norm parameter not 16-byte aligned");
+  Dev dev;
+  if ((st = current_device(dev, 0, nullptr, 0))) return st;
+  int lph = 2;
+  while (lph * 8 < D) lph *= 2;
+  k8::Params p;
+  memset(&p, 0, sizeof(p));
+  k8::View* dst[4] = {&p.q, &p.k, &p.qo, &p.ko};
+  for (int i = 0; i < 4; ++i) *dst[i] = k8::View{views[i]->data, views[i]->stride_token, views[i]->stride_head};
+  p.pos = rot->positions;
+  p.pos64 = rot->position_bytes == 8;
+  p.turns = rot->turns;
+  p.gain = rot->gain;
+  p.rot = rot->rot;
+  p.qw = norm->q_weight;
+  p.qb = norm->q_bias;
+  p.kw = norm->k_weight;
+  p.kb = norm->k_bias;
+  p.eps = norm->eps;
+  p.inv_d = 1.0f / static_cast<float>(D);
+  p.T = T;
+  p.hq = Hq;
+  p.heads = Hq + Hkv;
+  p.d = D;
+  // passes of 32 / lph heads; split over more warps until the card has 16 warps an SM
+  const int passes = (p.heads * lph + 31) / 32;
+  const long long want = 16ll * dev.sms;
+  const long long slices = std::min<long long>(passes, std::max<long long>(1, (want + T - 1) / T));
+  p.passes = static_cast<int>((passes + slices - 1) / slices);
+  p.slices = (passes + p.passes - 1) / p.passes;
+  const long long blocks = (static_cast<long long>(T) * p.slices + k8::kThreads / 32 - 1) / (k8::kThreads / 32);
+  if (blocks > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "too many tokens");
+  const bool inter = rot->interleaved != 0;
+  void (*kern)(k8::Params) = dtype == TMU_F16 ? k8_kernel<__half>(lph, norm->kind, inter)
+                                              : k8_kernel<__nv_bfloat16>(lph, norm->kind, inter);
+  cudaError_t e = launch_pdl(kern, static_cast<int>(blocks), k8::kThreads, 0, static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch qk_rope_kernel");
+}
+
+int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, const tmu_heads* out,
+                  const int* cu_seqlens, const tmu_attn_bias* bias, int S, int T, int Hq, int Hkv, int D, int dtype,
+                  int causal, float scale, void* status, void* stream) {
+  if (!q || !k || !v || !out) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+  int st = check_packed(T, Hq, Hkv, D);
+  if (st) return st;
+  if (S < 0) return fail(TMU_ERR_INVALID_ARGUMENT, "S must not be negative");
+  if (Hq % Hkv) return fail(TMU_ERR_INVALID_ARGUMENT, "Hq must be a multiple of Hkv");
+  if (D % 8 || D > 128) return fail(TMU_ERR_UNSUPPORTED, "D must be a multiple of 8, at most 128");
+  if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
+  if (T == 0 || S == 0) return TMU_OK;
+  if (!cu_seqlens) return fail(TMU_ERR_INVALID_ARGUMENT, "cu_seqlens is NULL");
+  const tmu_heads* views[4] = {q, k, v, out};
+  static const char* const names[4] = {"q", "k", "v", "out"};
+  for (int i = 0; i < 4; ++i)
+    if ((st = check_heads(views[i]->data, views[i]->stride_token, views[i]->stride_head, names[i]))) return st;
+  if (bias && (bias->n < 0 || (bias->n > 0 && !bias->data))) return fail(TMU_ERR_INVALID_ARGUMENT, "bias");
+  (void)status;
+  k7::Params p;
+  memset(&p, 0, sizeof(p));
+  k8::View* dst[4] = {&p.q, &p.k, &p.v, &p.o};
+  for (int i = 0; i < 4; ++i) *dst[i] = k8::View{views[i]->data, views[i]->stride_token, views[i]->stride_head};
+  p.cu = cu_seqlens;
+  if (bias && bias->n > 0) {
+    p.bias = bias->data;
+    p.bias_ss = bias->stride_seq;
+    p.bias_sh = bias->stride_head;
+    p.bias_sr = bias->stride_row;
+    p.bias_n = bias->n;
+  }
+  p.S = S;
+  p.T = T;
+  p.hq = Hq;
+  p.hkv = Hkv;
+  p.d = D;
+  p.causal = causal != 0;
+  p.scale = scale;
+  const long long blocks = (static_cast<long long>(T) * Hq + 3) / 4;
+  void (*kern)(k7::Params) = dtype == TMU_F16 ? k7::attention_rows_kernel<__half> : k7::attention_rows_kernel<__nv_bfloat16>;
+  kern<<<static_cast<unsigned>(blocks), k7::kSimpleThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_rows_kernel");
+}
+
+int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, void* stream) {
+  if (M < 0 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, K positive");
+  if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
+  if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
+  if (M == 0) return TMU_OK;
+  if (!x || !x8 || !scales) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL tensor");
+  if (ld < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows overlap: ld < K");
+  if (!aligned16(x) || !aligned16(x8) || ld % 8) return fail(TMU_ERR_MISALIGNED, "x, x8 must be 16-byte aligned, ld a multiple of 8");
+  Dev dev;
+  int st = current_device(dev, 0, nullptr, 0);
+  if (st) return st;
+  k9::QuantParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x;
+  p.ld = ld;
+  p.M = M;
+  p.K = K;
+  p.kb = (K + 127) / 128;
+  p.x8 = static_cast<uint8_t*>(x8);
+  p.xs = scales;
+  const long long items = static_cast<long long>(M) * p.kb;
+  const int grid = static_cast<int>(std::min<long long>((items + 15) / 16, 8ll * dev.sms));
+  cudaError_t e = launch_pdl(dtype == TMU_F16 ? k9::quantize_kernel<__half> : k9::quantize_kernel<__nv_bfloat16>, grid,
+                             k9::kQuantThreads, 0, static_cast<cudaStream_t>(stream), p);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch quantize_kernel");
+}
+
+size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  const size_t x8 = (static_cast<size_t>(M) * K + 255) / 256 * 256;
+  const size_t xs = (static_cast<size_t>(M) * ((K + 127) / 128) * 4 + 255) / 256 * 256;
+  return x8 + xs;
+}
+
+int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_scales, const void* w8, const float* w_scales,
+                   const float* bias, void* out, int out_dtype, long long ldo, int M, int N, int K, void* workspace,
+                   size_t workspace_bytes, void* status, void* stream) {
+  if (M < 0 || N < 1 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, N and K positive");
+  if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
+  if (x_dtype != TMU_F16 && x_dtype != TMU_BF16 && x_dtype != TMU_E4M3) return fail(TMU_ERR_UNSUPPORTED, "x must be fp16, bf16 or e4m3");
+  if (out_dtype != TMU_F16 && out_dtype != TMU_BF16 && out_dtype != TMU_F32) return fail(TMU_ERR_UNSUPPORTED, "out must be fp16, bf16 or fp32");
+  if (M == 0) return TMU_OK;
+  if (!x || !w8 || !w_scales || !out || (x_dtype == TMU_E4M3 && !x_scales)) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL tensor");
+  if (ldo < N && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of out overlap: ldo < N");
+  if (!aligned16(x) || !aligned16(w8)) return fail(TMU_ERR_MISALIGNED, "x, w8 must be 16-byte aligned");
+  if (x_dtype == TMU_E4M3 && ldx != K) return fail(TMU_ERR_UNSUPPORTED, "e4m3 x must be contiguous");
+  (void)status;
+  const uint8_t* x8 = static_cast<const uint8_t*>(x);
+  const float* xs = x_scales;
+  if (x_dtype != TMU_E4M3) {
+    if (!workspace || workspace_bytes < tmu_linear_fp8_workspace_bytes(M, N, K))
+      return fail(TMU_ERR_WORKSPACE_TOO_SMALL, "workspace too small");
+    if (!aligned16(workspace)) return fail(TMU_ERR_MISALIGNED, "workspace not 16-byte aligned");
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    float* sc = reinterpret_cast<float*>(ws + (static_cast<size_t>(M) * K + 255) / 256 * 256);
+    int st = tmu_quantize_rows(x, x_dtype, ldx, M, K, ws, sc, stream);
+    if (st) return st;
+    x8 = ws;
+    xs = sc;
+  }
+  k9::Params p;
+  memset(&p, 0, sizeof(p));
+  p.x8 = x8;
+  p.xs = xs;
+  p.w8 = static_cast<const uint8_t*>(w8);
+  p.ws = w_scales;
+  p.bias = bias;
+  p.out = out;
+  p.ldo = ldo;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.kb = (K + 127) / 128;
+  p.out_type = out_dtype;
+  const dim3 grid((N + 15) / 16, (M + 15) / 16);
+  k9::linear8_simple_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_simple_kernel");
+}
+
+}  // extern "C"

@@ -329,6 +329,90 @@ int tmu_copy_async(void* dst, const void* src, size_t bytes, void* stream);
 int tmu_copy2d_async(void* dst, size_t dst_pitch, const void* src, size_t src_pitch, size_t width, size_t height,
                      void* stream);
 
+/* ---- Sequence operators: attention over packed sequences, the norm and rotation of queries and
+ * keys, and the linear layer with 8-bit operands: the parts of a transformer layer over residues
+ * (the diffusion head's token transformer, whose pair biases tmu_pair_cond makes, and the language
+ * model in front of the trunk).  No counterpart in the reference's kernels, which leave these to
+ * MLX (mx.fast.scaled_dot_product_attention, mx.fast.rope, mx.quantized_matmul).  Inference only.
+ *
+ * A tensor of heads is [T, H, D]: values of a head contiguous, tokens and heads at element strides
+ * that are multiples of 8 (so slices of one fused projection do), the base 16-byte aligned. */
+#define TMU_F16 0
+#define TMU_BF16 1
+#define TMU_F32 2
+#define TMU_E4M3 3
+
+typedef struct tmu_heads {
+  void* data;
+  long long stride_token, stride_head; /* elements */
+} tmu_heads;
+
+#define TMU_NORM_NONE 0
+#define TMU_NORM_RMS 1
+#define TMU_NORM_LAYER 2
+
+typedef struct tmu_qk_norm {
+  int kind;
+  float eps;
+  const float* q_weight; /* fp32 [D], 16-byte aligned, each may be NULL (1 and 0) */
+  const float* q_bias;
+  const float* k_weight;
+  const float* k_bias;
+} tmu_qk_norm;
+
+typedef struct tmu_rotary {
+  const void* positions;            /* int32 or int64 [T] */
+  int position_bytes;               /* 4 or 8 */
+  const unsigned long long* turns;  /* [rot / 2]: turns a position of each pair, times 2^64 */
+  float gain;                       /* factor of the rotated values */
+  int rot;                          /* rotated values of a head: a multiple of 16, 0 for none */
+  int interleaved;                  /* pairs (2i, 2i + 1); else (i, i + rot / 2) */
+} tmu_rotary;
+
+/* K8: norm of every head of q [T, Hq, D] and k [T, Hkv, D] over its D values, then the rotation of
+ * its first `rot` values, fp32 inside and rounded once.  D a multiple of 16, at most 256; fp16 or
+ * bf16 in and out.  An output may be its own input; otherwise the four must not overlap. */
+int tmu_qk_norm_rope(const tmu_heads* q, const tmu_heads* k, const tmu_heads* q_out, const tmu_heads* k_out,
+                     const tmu_qk_norm* norm, const tmu_rotary* rot, int T, int Hq, int Hkv, int D, int dtype,
+                     void* stream);
+
+/* Additive bias of the scores, of q's type: element (i, j) of sequence s and query head h at
+ * s * stride_seq + h * stride_head + i * stride_row + j (a stride of 0 shares it).  Positions at or
+ * past n have none. */
+typedef struct tmu_attn_bias {
+  const void* data;
+  long long stride_seq, stride_head, stride_row;
+  int n;
+} tmu_attn_bias;
+
+/* K7: out = softmax(scale q k^T + bias) v within each of S packed sequences, tokens
+ * cu_seqlens[s] .. cu_seqlens[s + 1] (int32, device, ascending; values outside [0, T] are clamped),
+ * Hq a multiple of Hkv, D a multiple of 8, at most 128, fp16 or bf16.  With `causal` a token sees
+ * itself and the tokens before it.  Scores, maxima, sums and the output are fp32 inside; the
+ * weights are rounded to q's type for their product with v.  A row whose scores are all -inf is 0,
+ * and tokens of no sequence keep what `out` holds.  `out` must not overlap q, k or v.  status may be
+ * NULL. */
+int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, const tmu_heads* out,
+                  const int* cu_seqlens, const tmu_attn_bias* bias, int S, int T, int Hq, int Hkv, int D, int dtype,
+                  int causal, float scale, void* status, void* stream);
+
+/* K9, operands: x [M, K] fp16 or bf16 (rows ld elements apart, a multiple of 8) to e4m3 x8 [M, K]
+ * and fp32 scales [M, ceil(K / 128)]: scale = max(amax / 448, 2^-126) over 128 values of a row,
+ * x8 = e4m3(x / scale), both quotients rounded as fp32.  K a multiple of 16.  A block that holds an
+ * infinity or a NaN gives NaN. */
+int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, void* stream);
+
+/* K9: out [M, N] = x w^T + bias with 8-bit operands: w8 e4m3 [N, K] with fp32 w_scales
+ * [ceil(N / 128), ceil(K / 128)], x fp16 or bf16 [M, K] (quantised as by tmu_quantize_rows into the
+ * workspace; x_scales NULL) or e4m3 with its x_scales (contiguous, no workspace needed for it),
+ * bias fp32 [N] or NULL, out fp16, bf16 or fp32, rows ldo elements apart.  Sums are fp32.
+ * Workspace: tmu_linear_fp8_workspace_bytes, 16-byte aligned; it holds nothing between calls.
+ * status may be NULL. */
+size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K);
+int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_scales, const void* w8,
+                   const float* w_scales, const float* bias, void* out, int out_dtype, long long ldo, int M, int N,
+                   int K, void* workspace, size_t workspace_bytes, void* status, void* stream);
+
 /* Self-test of the bounded-wait machinery: launches one CTA that waits on an mbarrier nothing
  * ever arrives at, with a limit of `timeout_ns`; the kernel must give up, record
  * TMU_ERR_DEVICE_TIMEOUT in `status` and exit.  Returns the launch status. */

@@ -1,0 +1,173 @@
+"""CPU checks of the sequence operators: the argument checks of their C entries (nothing is launched),
+the rotary's frequencies, the layout of 8-bit weights, and the refusals of the Python side."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from esmfold2_mlx_b200 import _lib, attention as att, build, fp8
+
+OK, INVALID, MISALIGNED, WORKSPACE, UNSUPPORTED = 0, 1, 2, 3, 4
+P = 0x1000  # a pointer that no check follows
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.load()
+
+
+def heads(data=P, st=64, sh=64):
+    return _lib.TmuHeads(data, st, sh)
+
+
+def attention(lib, q=None, k=None, v=None, o=None, cu=P, bias=None, S=1, T=4, hq=2, hkv=1, d=64, dtype=0):
+    h = heads()
+    return lib.tmu_attention(q or h, k or h, v or h, o or h, cu, bias, S, T, hq, hkv, d, dtype, 0, 0.125, None, None)
+
+
+def test_attention_refusals(lib):
+    assert attention(lib, T=-1) == INVALID
+    assert attention(lib, hq=0) == INVALID
+    assert attention(lib, hq=3, hkv=2) == INVALID
+    assert attention(lib, S=-1) == INVALID
+    assert attention(lib, d=60) == UNSUPPORTED
+    assert attention(lib, d=136) == UNSUPPORTED
+    assert attention(lib, dtype=_lib.TMU_F32) == UNSUPPORTED
+    assert attention(lib, cu=None) == INVALID
+    for name in "qkvo":
+        assert attention(lib, **{name: heads(None)}) == INVALID
+        assert attention(lib, **{name: heads(P + 2)}) == MISALIGNED
+        assert attention(lib, **{name: heads(st=65)}) == MISALIGNED
+        assert attention(lib, **{name: heads(sh=4)}) == MISALIGNED
+        assert attention(lib, **{name: heads(st=-64)}) == INVALID
+    assert attention(lib, bias=_lib.TmuAttnBias(None, 0, 0, 0, 5)) == INVALID
+    assert attention(lib, bias=_lib.TmuAttnBias(P, 0, 0, 0, -1)) == INVALID
+    assert lib.tmu_attention(None, None, None, None, P, None, 1, 4, 2, 1, 64, 0, 0, 1.0, None, None) == INVALID
+
+
+def test_empty_calls_do_nothing(lib):
+    none = heads(None)
+    assert attention(lib, q=none, k=none, v=none, o=none, T=0) == OK
+    assert attention(lib, S=0) == OK
+    assert lib.tmu_quantize_rows(None, 0, 64, 0, 64, None, None, None) == OK
+    assert lib.tmu_linear_fp8(None, 0, 64, None, None, None, None, None, 0, 8, 0, 8, 64, None, 0, None, None) == OK
+    assert lib.tmu_linear_fp8_workspace_bytes(0, 8, 64) == 0
+
+
+def rope(lib, d=64, T=4, dtype=0, kind=1, rot=64, pos=P, turns=P, nbytes=4, q=None, w=None, hq=2):
+    h = heads()
+    nrm = _lib.TmuQkNorm(kind, 1e-5, w, None, None, None)
+    r = _lib.TmuRotary(pos, nbytes, turns, 1.0, rot, 0)
+    return lib.tmu_qk_norm_rope(q or h, h, h, h, nrm, r, T, hq, 1, d, dtype, None)
+
+
+def test_qk_norm_rope_refusals(lib):
+    assert rope(lib, d=40, rot=16) == UNSUPPORTED
+    assert rope(lib, d=272) == UNSUPPORTED
+    assert rope(lib, rot=80) == UNSUPPORTED
+    assert rope(lib, rot=24) == UNSUPPORTED
+    assert rope(lib, dtype=2) == UNSUPPORTED
+    assert rope(lib, kind=3) == INVALID
+    assert rope(lib, pos=None) == INVALID
+    assert rope(lib, turns=None) == INVALID
+    assert rope(lib, nbytes=2) == INVALID
+    assert rope(lib, T=-1) == INVALID
+    assert rope(lib, hq=0) == INVALID
+    assert rope(lib, q=heads(P + 8)) == MISALIGNED
+    assert rope(lib, w=P + 4) == MISALIGNED
+    assert rope(lib, T=0) == OK
+
+
+def linear(lib, x=P, xd=0, ldx=64, xs=None, w=P, ws=P, out=P, od=0, ldo=8, M=2, N=8, K=64, work=P, nb=1 << 20):
+    return lib.tmu_linear_fp8(x, xd, ldx, xs, w, ws, None, out, od, ldo, M, N, K, work, nb, None, None)
+
+
+def test_linear_refusals(lib):
+    assert linear(lib, K=24, ldx=24) == UNSUPPORTED
+    assert linear(lib, xd=_lib.TMU_F32) == UNSUPPORTED
+    assert linear(lib, od=_lib.TMU_E4M3) == UNSUPPORTED
+    assert linear(lib, M=-1) == INVALID
+    assert linear(lib, N=0) == INVALID
+    assert linear(lib, x=None) == INVALID
+    assert linear(lib, out=None) == INVALID
+    assert linear(lib, xd=_lib.TMU_E4M3) == INVALID  # no scales
+    assert linear(lib, xd=_lib.TMU_E4M3, xs=P, ldx=80) == UNSUPPORTED
+    assert linear(lib, ldo=4) == INVALID
+    assert linear(lib, ldx=32) == INVALID
+    assert linear(lib, w=P + 8) == MISALIGNED
+    assert linear(lib, nb=16) == WORKSPACE
+    assert linear(lib, work=None) == WORKSPACE
+    assert linear(lib, work=P + 8) == MISALIGNED
+    assert lib.tmu_quantize_rows(P, 0, 60, 2, 48, P, P, None) == MISALIGNED
+    assert lib.tmu_quantize_rows(P, 0, 32, 2, 48, P, P, None) == INVALID
+    assert lib.tmu_quantize_rows(P, 2, 48, 2, 48, P, P, None) == UNSUPPORTED
+
+
+def test_python_refusals():
+    x = torch.zeros(4, 2, 64, dtype=torch.float16)
+    with pytest.raises(TypeError):
+        att.attention(x, x, x, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(TypeError):
+        att.qk_norm_rope(x, x)
+    with pytest.raises(TypeError):
+        fp8.quantize_rows(x[0])
+    w = torch.zeros(4, 32, dtype=torch.float8_e4m3fn)
+    with pytest.raises(TypeError):
+        fp8.linear(x[0], fp8.BlockWeight(w, torch.ones(1, 1)))
+    for bad in (lambda: fp8.BlockWeight(w, torch.ones(1, 2)), lambda: fp8.BlockWeight(w.half(), torch.ones(1, 1)),
+                lambda: fp8.BlockWeight(w[:, :24], torch.ones(1, 1)), lambda: fp8.BlockWeight(w.t(), torch.ones(1, 1)),
+                lambda: att.Rotary(24, device="cpu"), lambda: att.Rotary(32, layout="pairs", device="cpu"),
+                lambda: att.Rotary(32, scaling={"type": "x"}, device="cpu"),
+                lambda: att.Rotary(32, scaling={"type": "linear", "factor": 0.0}, device="cpu")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_heads_overlap():
+    buf = torch.zeros(10, 6, 64)
+    q, k, v = buf[:, :2], buf[:, 2:4], buf[:, 4:]
+    assert not att._heads_overlap(q, k) and not att._heads_overlap(v, q)
+    assert att._heads_overlap(buf[:, :3], k) and att._heads_overlap(buf, v) and att._heads_overlap(q, q)
+    assert not att._heads_overlap(buf[:5], buf[5:])
+    assert att._heads_overlap(buf[:6], buf[5:])
+    assert att._heads_overlap(buf[..., :32], buf[..., 32:])  # interleaved within a token: refused as if shared
+    assert att._self_overlap(torch.zeros(1, 2, 64).expand(5, 2, 64)) and not att._self_overlap(q)
+    assert att._self_overlap(torch.as_strided(buf, (3, 2, 64), (64, 32, 1)))
+
+
+def test_rotary_frequencies():
+    r = att.Rotary(64, device="cpu")
+    turns = [t % 2**64 for t in r.turns.tolist()]
+    for i, t in enumerate(turns):
+        f = 10000.0 ** (-2 * i / 64) / (2 * math.pi)
+        assert abs(t / 2.0**64 - f) <= 2.0 ** -52
+    assert r.gain == 1.0
+    lin = att.Rotary(64, scaling={"type": "linear", "factor": 4.0}, device="cpu")
+    assert all(abs(a * 4 - b) < 1e-12 for a, b in zip(lin.frequencies, r.frequencies))
+    ntk = att.Rotary(64, scaling={"type": "ntk", "factor": 4.0}, device="cpu")
+    assert ntk.frequencies[0] == 1.0 and abs(ntk.frequencies[-1] * 4 / r.frequencies[-1] - 1) < 1e-12
+    y = att.Rotary(64, scaling={"type": "yarn", "factor": 16.0, "original_length": 4096}, device="cpu")
+    ratio = [a / b for a, b in zip(y.frequencies, r.frequencies)]
+    assert ratio[0] == 1.0 and abs(ratio[-1] * 16 - 1) < 1e-12 and all(a >= b for a, b in zip(ratio, ratio[1:]))
+    assert abs(y.gain - (0.1 * math.log(16) + 1)) < 1e-15
+    turned = [f * 4096 / (2 * math.pi) for f in r.frequencies]
+    assert all(q == 1.0 for q, t in zip(ratio, turned) if t > 50) and all(q < 0.07 for q, t in zip(ratio, turned) if t < 0.7)
+
+
+def test_weight_layout():
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(200, 272, generator=g)
+    w[130:] *= 100
+    q = fp8.quantize_weight(w, "cpu")
+    assert q.scales.shape == (2, 3) and q.shape == (200, 272)
+    d = q.dequantize()
+    s = q.scales.repeat_interleave(128, 0)[:200].repeat_interleave(128, 1)[:, :272]
+    # half a step of 3 mantissa bits, or of the least subnormal 2^-9
+    assert ((d - w).abs() <= torch.maximum(w.abs() * 2.0**-4, s * 2.0**-10) * (1 + 1e-6)).all()
+    z = fp8.quantize_weight(torch.zeros(8, 16), "cpu")
+    assert (z.dequantize() == 0).all() and (z.scales == fp8.SCALE_MIN).all()
