@@ -3,6 +3,29 @@
 // Row i of sequence s (tokens cu[s] .. cu[s + 1]) and query head h, key head h / (Hq / Hkv):
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(x_ij - max_j x_ij),   x_ij = scale q_i . k_j + bias_ij
 // over the keys j of the same sequence, j <= i if causal.  A row whose keys are all at -inf is zero.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax, in base 2 (x times
+// log2 e).  The accumulator O = sum_j 2^(x_ij - m) v_j stays in tensor memory, so moving m would
+// mean reading and writing all of it: m only moves when a tile's maximum exceeds it by more than
+// 8, so weights reach at most 2^8 (exact in fp32 sums, and a common factor of the 16-bit weights),
+// and the result, O / l, does not depend on when it moved.
+//
+// A block takes 256 rows of one head and sequence as two tiles A and B of 128 rows; a step takes
+// 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the softmax of S's rows (one thread a row), P in
+// TMEM in the inputs' type, and O += P V with P as the MMA's A operand out of TMEM.  While one
+// tile's softmax runs, the tensor cores work for the other.
+//   warps 0-3   softmax of tile A (warp w: TMEM lanes 32 w ..)     warps 4-7   softmax of tile B
+//   warp 8      TMA: Q, then K and V through rings of kStages tiles
+//   warp 9      TMEM and the MMAs (one thread)
+//   warps 10-11 idle (they complete the warpgroup that gives its registers to the softmax)
+// TMEM (512 columns): D <= 64: O 2 x 64, S 2 x 128, P 2 x 64: S has its own columns, so the next
+// S is made while the softmax works on this one.  D > 64: O 2 x 128, S 2 x 128, and P overwrites S;
+// the MMAs of a block execute in issue order, so S of step j + 1 follows the P V that reads them.
+//
+// Blocks find their sequence without a prefix sum over the lengths: sequence s owns the slots
+// from floor(cu[s] / 256) + s, at least as many as it has tile pairs, and the slots it does not
+// need return at once.  The heads are the grid's fast axis, and later rows come first when causal,
+// so the long blocks start first.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -12,76 +35,389 @@
 namespace tmu {
 namespace k7 {
 
+constexpr int kRows = 256;     // query rows of a block
+constexpr int kTile = 128;     // query rows of a tile, keys of a step
+constexpr int kThreads = 384;
+constexpr int kAtom = kTile * 128;  // 64 values of 128 rows
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 256 * 208 + 128 * 88 = 384 * 168
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMoveMax = 8.f;
+
 struct Params {
-  k8::View q, k, v, o;
+  CUtensorMap tm_q, tm_k, tm_v;  // [H, T, D]: box {64, 128, 1}, 128B swizzle, zero past the ends
+  k8::View o;
   const int* cu;
   const void* bias;  // [S or 1, Hq, n, n] or null, the last axis contiguous
   long long bias_ss, bias_sh, bias_sr;
   int bias_n;
-  int S, T, hq, hkv, d, causal;
-  float scale;
+  int S, T, hq, group, d, causal;
+  float scale_log2;  // scale * log2 e
+  DeviceStatus* status;
+  unsigned long long timeout_ns;
 };
 
-constexpr int kSimpleThreads = 128;
+template <int DP>
+struct Cfg {
+  static constexpr int kAtoms = DP / 64;
+  static constexpr int kTileBytes = kAtoms * kAtom;
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr bool kOwnP = DP == 64;  // P beside S instead of over it
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = 2 * kTileBytes;
+  static constexpr int OFF_V = OFF_K + kStages * kTileBytes;
+  static constexpr int OFF_BAR = OFF_V + kStages * kTileBytes;
+  static constexpr int SMEM_BYTES = OFF_BAR + 512;
+  // TMEM columns of tile x
+  __device__ static constexpr uint32_t o_col(int x) { return x * DP; }
+  __device__ static constexpr uint32_t s_col(int x) { return 2 * DP + x * 128; }
+  __device__ static constexpr uint32_t p_col(int x) { return kOwnP ? 2 * DP + 256 + x * 64 : s_col(x); }
+};
+static_assert(Cfg<64>::SMEM_BYTES <= 232448 && Cfg<128>::SMEM_BYTES <= 232448, "K7 shared memory exceeds the limit");
 
-// One warp a row and head; lanes take keys for the scores and head values for the output.
-template <typename T>
-__global__ void __launch_bounds__(kSimpleThreads) attention_rows_kernel(const __grid_constant__ Params p) {
-  __shared__ float qs[kSimpleThreads / 32][128];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long item = static_cast<long long>(blockIdx.x) * (kSimpleThreads / 32) + warp;
-  if (item >= static_cast<long long>(p.T) * p.hq) return;
-  const int t = static_cast<int>(item / p.hq), h = static_cast<int>(item % p.hq);
-  int beg = 0, end = 0, seq = -1;
-  for (int s = 0; s < p.S; ++s) {
-    const int b = min(max(p.cu[s], 0), p.T), e = min(max(p.cu[s + 1], b), p.T);
-    if (t >= b && t < e) {
-      beg = b;
-      end = e;
-      seq = s;
-      break;
+enum Site : unsigned int {
+  kSiteProdK = 0x701, kSiteProdV = 0x702, kSiteMmaQ = 0x703, kSiteMmaK = 0x704, kSiteMmaV = 0x705, kSiteMmaS = 0x706,
+  kSiteMmaP = 0x707, kSiteFix = 0x708, kSiteSoftS = 0x709, kSiteSoftO = 0x70a, kSiteEpi = 0x70b, kSiteLayout = 0x7ff
+};
+
+// Where the status of calls without a status block of their own goes.
+__device__ DeviceStatus g_own_status;
+
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Ties registers of an earlier tcgen05.ld to the wait in front of it.
+__device__ __forceinline__ void tie(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ int clamp_token(int t, int T) { return min(max(t, 0), T); }
+
+// The sequence that owns `slot` (a warp searches 32-ary): the last s with floor(cu[s] / kRows) + s <= slot.
+__device__ __forceinline__ int find_sequence(const int* cu, int S, int T, int slot) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = S;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const long long s = lo + static_cast<long long>(lane) * step;
+    const bool in = s < hi && (lane == 0 || clamp_token(__ldg(cu + s), T) / kRows + s <= slot);
+    const int b = 31 - __clz(__ballot_sync(0xffffffffu, in));
+    lo += b * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+template <typename T, int DP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<DP>;
+  constexpr int NS = C::kStages;
+  extern __shared__ uint8_t smem[];
+  DeviceStatus* const status = p.status != nullptr ? p.status : &g_own_status;
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) record_status(status, kStatusLayout, kSiteLayout);
+    return;
+  }
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  griddep_wait();
+
+  const int slot = blockIdx.x / p.hq, head = blockIdx.x - slot * p.hq;
+  const int seq = find_sequence(p.cu, p.S, p.T, slot);
+  const int beg = clamp_token(__ldg(p.cu + seq), p.T);
+  const int len = max(clamp_token(__ldg(p.cu + seq + 1), p.T) - beg, 0);
+  const int blocks = (len + kRows - 1) / kRows;
+  const int blk = slot - (beg / kRows + seq);
+  if (blk < 0 || blk >= blocks) return;
+  const int q0 = (p.causal ? blocks - 1 - blk : blk) * kRows;
+  // steps of tiles A and B (B may have no rows)
+  auto steps = [&](int x) {
+    const int first = q0 + x * kTile;
+    if (first >= len) return 0;
+    const int keys = p.causal ? min(len, first + kTile) : len;
+    return (keys + kTile - 1) / kTile;
+  };
+  const int n0 = steps(0), n1 = steps(1), n = max(n0, n1);
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* kfull = bars;
+  uint64_t* kempty = bars + 4;
+  uint64_t* vfull = bars + 8;
+  uint64_t* vempty = bars + 12;
+  uint64_t* qfull = bars + 16;   // [2]
+  uint64_t* sfull = bars + 18;   // [2] S of a step is in TMEM
+  uint64_t* sfree = bars + 20;   // [2] the softmax has read S (own P columns only)
+  uint64_t* pfull = bars + 22;   // [2] P of a step is in TMEM
+  uint64_t* ofull = bars + 24;   // [2] P V of a step is done
+  uint64_t& vfixed = bars[26];   // the last V tile's foreign rows are cleared
+  uint64_t& drain_bar = bars[27];
+  uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(bars + 28);
+  volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(bars + 28) + 4);
+  const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&kfull[s], 1);
+      mbar_init(&kempty[s], 1);
+      mbar_init(&vfull[s], 1);
+      mbar_init(&vempty[s], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&qfull[x], 1);
+      mbar_init(&sfull[x], 1);
+      mbar_init(&sfree[x], 4);  // the tile's four warps
+      mbar_init(&pfull[x], 4);
+      mbar_init(&ofull[x], 1);
+    }
+    mbar_init(&vfixed, 1);
+    mbar_init(&drain_bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&tmem_base_sh, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  griddep_trigger();
+  const bool fix = n * kTile > len;  // the last step's keys end inside the tile
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+      // ------------------------------ loads ------------------------------
+      if (lane == 0) {
+        const int kv = head / p.group;
+        auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int h) {
+          mbar_arrive_expect_tx(bar, C::kTileBytes);
+          for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kAtom, map, bar, a * 64, row, h);
+        };
+        int j = 0;
+        load(smem + C::OFF_Q, &p.tm_q, &qfull[0], beg + q0, head);
+        for (; j < n; ++j) {
+          const int s = j % NS, ph = (j / NS) & 1;
+          if (!mbar_wait(&kempty[s], ph ^ 1, ctx, kSiteProdK)) break;
+          load(smem + C::OFF_K + s * C::kTileBytes, &p.tm_k, &kfull[s], beg + j * kTile, kv);
+          if (j == 0 && n1 > 0) load(smem + C::OFF_Q + C::kTileBytes, &p.tm_q, &qfull[1], beg + q0 + kTile, head);
+          if (!mbar_wait(&vempty[s], ph ^ 1, ctx, kSiteProdV)) {
+            mbar_drain(&kfull[s], ph, 200000000ull);
+            break;
+          }
+          load(smem + C::OFF_V + s * C::kTileBytes, &p.tm_v, &vfull[s], beg + j * kTile, kv);
+      }
+        if (abort_sh) {
+          mbar_drain(&qfull[0], 0, 200000000ull);
+          if (n1 > 0 && j > 0) mbar_drain(&qfull[1], 0, 200000000ull);
+          for (int s = 0; s < NS; ++s) {
+            const int armed = j > s ? (j - s + NS - 1) / NS : 0;
+            if (armed) {
+              mbar_drain(&kfull[s], (armed - 1) & 1, 200000000ull);
+              mbar_drain(&vfull[s], (armed - 1) & 1, 200000000ull);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      // Clear the last V tile's rows that belong to no key of the sequence: their weights are 0, but
+      // 0 times another sequence's NaN would be a NaN.  This warp made the load, so the phase it
+      // waits for is the barrier's current one.
+      const int s = (n - 1) % NS, keep = len - (n - 1) * kTile;
+      if (fix && warp_wait(&vfull[s], ((n - 1) / NS) & 1, ctx, kSiteFix)) {
+        for (int c = keep * 8 + lane; c < kTile * 8; c += 32)
+          for (int a = 0; a < C::kAtoms; ++a)
+            *reinterpret_cast<uint4*>(smem + C::OFF_V + s * C::kTileBytes + a * kAtom + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&vfixed);
+      }
+    } else if (warp == 9 && lane == 0) {
+      // ------------------------------ MMAs ------------------------------
+      constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+      const int ksteps = (p.d + 15) / 16;
+      const uint32_t id_s = kBf16 ? idesc_bf16_f32(128, 128, false, false) : idesc_f16_f32(128, 128, false, false);
+      const uint32_t id_o = kBf16 ? idesc_bf16_f32(128, ksteps * 16, false, true) : idesc_f16_f32(128, ksteps * 16, false, true);
+      const uint64_t qd = sdesc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
+      const uint64_t kd = sdesc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
+      const uint64_t vd = sdesc_sw128(smem_u32(smem + C::OFF_V), kAtom, 1024);
+      const int nx[2] = {n0, n1};
+      auto issue_s = [&](int x, int j) {  // S_x(j) = Q_x K_j^T
+        const int s = j % NS;
+        if (j == 0 && !mbar_wait(&qfull[x], 0, ctx, kSiteMmaQ)) return false;
+        if (!mbar_wait(&kfull[s], (j / NS) & 1, ctx, kSiteMmaK)) return false;
+        tc_fence_after();
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t off = (k >> 2) * kAtom + (k & 3) * 32;
+          umma_f16(tmem + C::s_col(x), sdesc_add(qd, x * C::kTileBytes + off), sdesc_add(kd, s * C::kTileBytes + off), id_s,
+                   k > 0 ? 1u : 0u);
+        }
+        umma_commit(&sfull[x]);
+        if (x == 1 || j >= n1) umma_commit(&kempty[s]);  // the last use of K_j
+        return true;
+      };
+      bool ok = issue_s(0, 0) && (n1 == 0 || issue_s(1, 0));
+      for (int j = 0; ok && j < n; ++j) {
+        const int s = j % NS;
+        if (!(ok = mbar_wait(&vfull[s], (j / NS) & 1, ctx, kSiteMmaV))) break;
+        if (fix && j == n - 1 && !(ok = mbar_wait(&vfixed, 0, ctx, kSiteMmaV))) break;
+        for (int x = 0; ok && x < 2; ++x) {
+          if (j >= nx[x]) continue;
+          if (C::kOwnP && j + 1 < nx[x]) {
+            if (!(ok = mbar_wait(&sfree[x], j & 1, ctx, kSiteMmaS) && issue_s(x, j + 1))) break;
+          }
+          if (!(ok = mbar_wait(&pfull[x], j & 1, ctx, kSiteMmaP))) break;
+          tc_fence_after();
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_ts(tmem + C::o_col(x), tmem + C::p_col(x) + k * 8, sdesc_add(vd, s * C::kTileBytes + k * 2048), id_o,
+                    (j > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&ofull[x]);
+          if (!C::kOwnP && j + 1 < nx[x]) ok = issue_s(x, j + 1);
+        }
+        if (ok) umma_commit(&vempty[s]);
+      }
+      umma_commit(&drain_bar);
+      mbar_drain(&drain_bar, 0, 200000000ull);
+    }
+  } else {
+    // ------------------------------ softmax ------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int x = warp >> 2;
+    const int nx = x == 0 ? n0 : n1;
+    const int tile0 = q0 + x * kTile;
+    const int row = tile0 + (warp & 3) * 32 + lane;  // within the sequence
+    const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const bool flip = p.scale_log2 < 0.f;
+    // a scale of 0 would turn a hidden key's -inf into a NaN
+    const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const T* brow = nullptr;
+    if (BIAS && row < min(p.bias_n, len))
+      brow = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh + row * p.bias_sr;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nx; ++j) {
+      if (!(ok = warp_wait(&sfull[x], j & 1, ctx, kSiteSoftS))) break;
+      tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) tmem_ld32(tl + C::s_col(x) + b * 32, r[b]);
+      tmem_wait_ld(r[0]);
+      tie(r[1]);
+      tie(r[2]);
+      tie(r[3]);
+      if (C::kOwnP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sfree[x]);
+      }
+      float* v = reinterpret_cast<float*>(&r[0][0]);
+      if (flip) {
+#pragma unroll
+        for (int e = 0; e < 128; ++e) v[e] = -v[e];
+      }
+      const int k0 = j * kTile;
+      float mul = c;
+      if (BIAS) {  // x = s c + bias log2 e at once; without a bias the product is folded into the exponential
+        mul = 1.f;
+#pragma unroll
+        for (int e = 0; e < 128; ++e) {
+          const float b = brow != nullptr && k0 + e < min(p.bias_n, len) ? static_cast<float>(brow[k0 + e]) : 0.f;
+          v[e] = fmaf(v[e], c, b * kLog2e);
+        }
+      }
+      if (k0 + kTile > len || (p.causal && k0 + kTile - 1 > tile0)) {
+        const int lim = (p.causal ? min(len, row + 1) : len) - k0;
+#pragma unroll
+        for (int e = 0; e < 128; ++e) v[e] = e < lim ? v[e] : -INFINITY;
+      }
+      float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+      for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+      if (j > 0 && C::kOwnP) {  // P's columns and O belong to P V of the last step (else S's being there says so)
+        if (!(ok = warp_wait(&ofull[x], (j - 1) & 1, ctx, kSiteSoftO))) break;
+        tc_fence_after();
+      }
+      const bool move = top > m + kMoveMax || (m == -INFINITY && top > m);
+      if (j == 0) {
+        m = fmaxf(m, top);
+      } else if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? ex2_approx(m - top) : 1.f;
+        if (move) m = top;
+        l *= f;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) {
+          uint32_t o[32];
+          tmem_ld32(tl + C::o_col(x) + b * 32, o);
+          tmem_wait_ld(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st32(tl + C::o_col(x) + b * 32, o);
+        }
+      }
+      const float neg = m == -INFINITY ? 0.f : -m;
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float2 t = __ffma2_rn(make_float2(v[b * 64 + 2 * e], v[b * 64 + 2 * e + 1]), make_float2(mul, mul),
+                                      make_float2(neg, neg));
+          const float2 q = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+          sum = __fadd2_rn(sum, q);
+          w[e] = k8::pack2(q.x, q.y, T());
+        }
+        tmem_st32(tl + C::p_col(x) + b * 32, w);
+      }
+      l += sum.x + sum.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pfull[x]);
+    }
+    if (ok && nx > 0 && warp_wait(&ofull[x], (nx - 1) & 1, ctx, kSiteEpi)) {
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(p.o.p) + static_cast<long long>(beg + row) * p.o.st + head * p.o.sh;
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) {
+        uint32_t o[32];
+        tmem_ld32(tl + C::o_col(x) + b * 32, o);
+        tmem_wait_ld(o);
+        if (row >= len) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (b * 32 + g * 8 >= p.d) break;
+          uint32_t u[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            u[e] = k8::pack2(__uint_as_float(o[g * 8 + 2 * e]) * inv, __uint_as_float(o[g * 8 + 2 * e + 1]) * inv, T());
+          *reinterpret_cast<uint4*>(out + b * 32 + g * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+      }
     }
   }
-  if (seq < 0) return;
-  const int kv = h / (p.hq / p.hkv), i = t - beg;
-  const T* q = static_cast<const T*>(p.q.p) + t * p.q.st + h * p.q.sh;
-  for (int d = lane; d < 128; d += 32) qs[warp][d] = d < p.d ? static_cast<float>(q[d]) : 0.f;
-  __syncwarp();
-  const int last = p.causal ? i + 1 : end - beg;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < last; j0 += 32) {
-    const int j = j0 + lane;
-    float x = -INFINITY;
-    if (j < last) {
-      const T* k = static_cast<const T*>(p.k.p) + static_cast<long long>(beg + j) * p.k.st + kv * p.k.sh;
-      float acc = 0.f;
-      for (int d = 0; d < p.d; ++d) acc = fmaf(qs[warp][d], static_cast<float>(k[d]), acc);
-      x = acc * p.scale;
-      if (p.bias != nullptr && i < p.bias_n && j < p.bias_n)
-        x += static_cast<float>(static_cast<const T*>(p.bias)[seq * p.bias_ss + h * p.bias_sh + i * p.bias_sr + j]);
-    }
-    float mx = x;
-    for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-    const float mn = fmaxf(m, mx);
-    if (mn == -INFINITY) continue;
-    const float f = expf(m - mn);
-    const float pj = expf(x - mn);
-    float ps = pj;
-    for (int w = 16; w > 0; w >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, w);
-    l = l * f + ps;
-    m = mn;
-    for (int e = 0; e < 4; ++e) o[e] *= f;
-    for (int jj = 0; jj < 32 && j0 + jj < last; ++jj) {
-      const float w = __shfl_sync(0xffffffffu, pj, jj);
-      const T* v = static_cast<const T*>(p.v.p) + static_cast<long long>(beg + j0 + jj) * p.v.st + kv * p.v.sh;
-      for (int e = 0; e < 4; ++e)
-        if (lane + 32 * e < p.d) o[e] = fmaf(w, static_cast<float>(v[lane + 32 * e]), o[e]);
-    }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
-  T* out = static_cast<T*>(p.o.p) + t * p.o.st + h * p.o.sh;
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < p.d) out[lane + 32 * e] = static_cast<T>(o[e] * inv);
 }
 
 }  // namespace k7

@@ -4,6 +4,19 @@
 
 namespace {
 
+// The sequence kernels' shared-memory opt-in, once a device and kernel (bits of their own).
+unsigned long long g_seq_attr_done[kMaxDevices] = {0};
+
+int seq_device(Dev& d, int bit, const void* kernel, int smem) {
+  int st = current_device(d, 0, nullptr, 0);
+  if (st) return st;
+  if (g_seq_attr_done[d.id] >> bit & 1) return TMU_OK;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+  g_seq_attr_done[d.id] |= 1ull << bit;
+  return TMU_OK;
+}
+
 // A [T, H, D] view of 16-bit values that 16-byte accesses can read: aligned base and strides.
 int check_heads(const void* p, long long st, long long sh, const char* what) {
   if (p == nullptr) return fail(TMU_ERR_INVALID_ARGUMENT, what);
@@ -37,6 +50,19 @@ void (*k8_kernel(int lph, int norm, bool inter))(k8::Params) {
     case 16: return k8_kernel<T, 16>(norm, inter);
     default: return k8_kernel<T, 32>(norm, inter);
   }
+}
+
+template <int DP>
+int launch_k7(const k7::Params& p, bool bf16, bool biased, int blocks, cudaStream_t stream) {
+  void (*kern)(k7::Params) =
+      bf16 ? (biased ? k7::attention_kernel<__nv_bfloat16, DP, true> : k7::attention_kernel<__nv_bfloat16, DP, false>)
+           : (biased ? k7::attention_kernel<__half, DP, true> : k7::attention_kernel<__half, DP, false>);
+  Dev dev;
+  const int bit = (DP == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (biased ? 1 : 0);
+  int st = seq_device(dev, bit, reinterpret_cast<const void*>(kern), k7::Cfg<DP>::SMEM_BYTES);
+  if (st) return st;
+  cudaError_t e = launch_pdl(kern, blocks, k7::kThreads, k7::Cfg<DP>::SMEM_BYTES, stream, p);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_kernel");
 }
 
 }  // namespace
@@ -119,13 +145,25 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
   for (int i = 0; i < 4; ++i)
     if ((st = check_heads(views[i]->data, views[i]->stride_token, views[i]->stride_head, names[i]))) return st;
   if (bias && (bias->n < 0 || (bias->n > 0 && !bias->data))) return fail(TMU_ERR_INVALID_ARGUMENT, "bias");
-  (void)status;
+  // a tensor map cannot step by 0
+  const int heads[3] = {Hq, Hkv, Hkv};
+  for (int i = 0; i < 3; ++i)
+    if ((T > 1 && views[i]->stride_token == 0) || (heads[i] > 1 && views[i]->stride_head == 0))
+      return fail(TMU_ERR_UNSUPPORTED, "q, k and v must not be broadcast views");
+  const bool bf16 = dtype == TMU_BF16, biased = bias && bias->n > 0;
   k7::Params p;
   memset(&p, 0, sizeof(p));
-  k8::View* dst[4] = {&p.q, &p.k, &p.v, &p.o};
-  for (int i = 0; i < 4; ++i) *dst[i] = k8::View{views[i]->data, views[i]->stride_token, views[i]->stride_head};
+  CUtensorMap* maps[3] = {&p.tm_q, &p.tm_k, &p.tm_v};
+  for (int i = 0; i < 3; ++i) {
+    const uint64_t row = ((uint64_t)D * 2 + 15) / 16 * 16;
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)T, (uint64_t)heads[i]};
+    const uint64_t str[2] = {T > 1 ? 2ull * views[i]->stride_token : row, heads[i] > 1 ? 2ull * views[i]->stride_head : row};
+    const uint32_t box[3] = {64, (uint32_t)k7::kTile, 1};
+    if ((st = encode_map(maps[i], views[i]->data, 3, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B))) return st;
+  }
+  p.o = k8::View{out->data, out->stride_token, out->stride_head};
   p.cu = cu_seqlens;
-  if (bias && bias->n > 0) {
+  if (biased) {
     p.bias = bias->data;
     p.bias_ss = bias->stride_seq;
     p.bias_sh = bias->stride_head;
@@ -135,15 +173,16 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
   p.S = S;
   p.T = T;
   p.hq = Hq;
-  p.hkv = Hkv;
+  p.group = Hq / Hkv;
   p.d = D;
   p.causal = causal != 0;
-  p.scale = scale;
-  const long long blocks = (static_cast<long long>(T) * Hq + 3) / 4;
-  void (*kern)(k7::Params) = dtype == TMU_F16 ? k7::attention_rows_kernel<__half> : k7::attention_rows_kernel<__nv_bfloat16>;
-  kern<<<static_cast<unsigned>(blocks), k7::kSimpleThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_rows_kernel");
+  p.scale_log2 = scale * k7::kLog2e;
+  p.status = static_cast<DeviceStatus*>(status);
+  p.timeout_ns = g_timeout_ns;
+  const long long blocks = (static_cast<long long>(T) / k7::kRows + S) * Hq;
+  if (blocks > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "too many sequences and heads");
+  return D <= 64 ? launch_k7<64>(p, bf16, biased, static_cast<int>(blocks), static_cast<cudaStream_t>(stream))
+                 : launch_k7<128>(p, bf16, biased, static_cast<int>(blocks), static_cast<cudaStream_t>(stream));
 }
 
 int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, void* stream) {
