@@ -79,9 +79,6 @@ enum Site : unsigned int {
   kSiteMmaP = 0x707, kSiteFix = 0x708, kSiteSoftS = 0x709, kSiteSoftO = 0x70a, kSiteEpi = 0x70b, kSiteLayout = 0x7ff
 };
 
-// Where the status of calls without a status block of their own goes.
-__device__ DeviceStatus g_own_status;
-
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(

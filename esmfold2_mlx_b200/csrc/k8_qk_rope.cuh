@@ -25,6 +25,10 @@
 #include "tmu_common.cuh"
 
 namespace tmu {
+
+// Where the sequence kernels' status goes in calls without a status block of their own.
+__device__ DeviceStatus g_own_status;
+
 namespace k8 {
 
 constexpr int kThreads = 128;

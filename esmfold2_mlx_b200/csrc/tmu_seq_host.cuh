@@ -65,6 +65,120 @@ int launch_k7(const k7::Params& p, bool bf16, bool biased, int blocks, cudaStrea
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_kernel");
 }
 
+int launch_k9_rows(const void* x, int x_dtype, long long ldx, const float* xs, const void* w8, const float* ws,
+                   const float* bias, void* out, int out_dtype, long long ldo, int M, int N, int K, cudaStream_t stream) {
+  k9::RowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x;
+  p.ldx = ldx;
+  p.xs = xs;
+  p.w8 = static_cast<const uint8_t*>(w8);
+  p.ws = ws;
+  p.bias = bias;
+  p.out = out;
+  p.ldo = ldo;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.kb = (K + 127) / 128;
+  p.out_type = out_dtype;
+  void (*kern)(k9::RowsParams);
+  if (M <= 8)
+    kern = x_dtype == TMU_F16 ? k9::linear8_rows_kernel<__half, 1>
+           : x_dtype == TMU_BF16 ? k9::linear8_rows_kernel<__nv_bfloat16, 1> : k9::linear8_rows_kernel<uint8_t, 1>;
+  else
+    kern = x_dtype == TMU_F16 ? k9::linear8_rows_kernel<__half, 2>
+           : x_dtype == TMU_BF16 ? k9::linear8_rows_kernel<__nv_bfloat16, 2> : k9::linear8_rows_kernel<uint8_t, 2>;
+  cudaError_t e = launch_pdl(kern, (N + k9::kRowsN - 1) / k9::kRowsN, k9::kRowsThreads, 0, stream, p);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_rows_kernel");
+}
+
+// A [rows, K] e4m3 matrix, read as bytes in boxes of 128 x 128.
+int encode_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t K) {
+  int st = get_encoder();
+  if (st) return st;
+  const cuuint64_t dims[2] = {K, rows}, strides[1] = {K};
+  const cuuint32_t box[2] = {128, 128}, es[2] = {1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? TMU_OK : fail(TMU_ERR_DRIVER, "cuTensorMapEncodeTiled failed for an 8-bit operand");
+}
+
+int launch_k9(const void* x8, const float* xs, const void* w8, const float* ws, const float* bias, void* out, int out_dtype,
+              long long ldo, int M, int N, int K, DeviceStatus* status, cudaStream_t stream) {
+  Dev dev;
+  int st = seq_device(dev, 8, reinterpret_cast<const void*>(&k9::linear8_kernel), k9::SMEM_BYTES);
+  if (st) return st;
+  k9::Params p;
+  memset(&p, 0, sizeof(p));
+  if ((st = encode_bytes(&p.tm_x, x8, M, K)) || (st = encode_bytes(&p.tm_w, w8, N, K))) return st;
+  p.xs = xs;
+  p.ws = ws;
+  p.bias = bias;
+  p.out = out;
+  p.ldo = ldo;
+  p.M = M;
+  p.N = N;
+  p.kb = (K + 127) / 128;
+  p.out_type = out_dtype;
+  const int es = out_dtype == TMU_F32 ? 4 : 2;
+  p.vec = aligned16(out) && ldo * es % 16 == 0;
+  p.tiles_m = (M + k9::kTile - 1) / k9::kTile;
+  const long long tiles = static_cast<long long>(p.tiles_m) * ((N + k9::kTile - 1) / k9::kTile);
+  // blocks of a cluster share a tile along K while the card has room for more blocks
+  p.split = 1;
+  while (p.split < 8 && tiles * p.split * 2 <= dev.sms && p.kb >= p.split * 4) p.split *= 2;
+  if (tiles * p.split > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "M and N are too large");
+  p.status = status;
+  p.timeout_ns = g_timeout_ns;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
+  cfg.blockDim = dim3(k9::kThreads);
+  cfg.dynamicSmemBytes = k9::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, &k9::linear8_kernel, p);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_kernel");
+}
+
+int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, bool chained,
+                  cudaStream_t stream) {
+  if (M < 0 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, K positive");
+  if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
+  if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
+  if (M == 0) return TMU_OK;
+  if (!x || !x8 || !scales) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL tensor");
+  if (ld < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows overlap: ld < K");
+  if (!aligned16(x) || !aligned16(x8) || ld % 8) return fail(TMU_ERR_MISALIGNED, "x, x8 must be 16-byte aligned, ld a multiple of 8");
+  Dev dev;
+  int st = current_device(dev, 0, nullptr, 0);
+  if (st) return st;
+  k9::QuantParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x;
+  p.ld = ld;
+  p.M = M;
+  p.K = K;
+  p.kb = (K + 127) / 128;
+  p.x8 = static_cast<uint8_t*>(x8);
+  p.xs = scales;
+  p.chained = chained;
+  const long long items = static_cast<long long>(M) * p.kb;
+  const int grid = static_cast<int>(std::min<long long>((items + 15) / 16, 8ll * dev.sms));
+  cudaError_t e = launch_pdl(dtype == TMU_F16 ? k9::quantize_kernel<__half> : k9::quantize_kernel<__nv_bfloat16>, grid,
+                             k9::kQuantThreads, 0, stream, p);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch quantize_kernel");
+}
+
 }  // namespace
 
 extern "C" {
@@ -186,34 +300,11 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
 }
 
 int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, void* stream) {
-  if (M < 0 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, K positive");
-  if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
-  if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
-  if (M == 0) return TMU_OK;
-  if (!x || !x8 || !scales) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL tensor");
-  if (ld < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows overlap: ld < K");
-  if (!aligned16(x) || !aligned16(x8) || ld % 8) return fail(TMU_ERR_MISALIGNED, "x, x8 must be 16-byte aligned, ld a multiple of 8");
-  Dev dev;
-  int st = current_device(dev, 0, nullptr, 0);
-  if (st) return st;
-  k9::QuantParams p;
-  memset(&p, 0, sizeof(p));
-  p.x = x;
-  p.ld = ld;
-  p.M = M;
-  p.K = K;
-  p.kb = (K + 127) / 128;
-  p.x8 = static_cast<uint8_t*>(x8);
-  p.xs = scales;
-  const long long items = static_cast<long long>(M) * p.kb;
-  const int grid = static_cast<int>(std::min<long long>((items + 15) / 16, 8ll * dev.sms));
-  cudaError_t e = launch_pdl(dtype == TMU_F16 ? k9::quantize_kernel<__half> : k9::quantize_kernel<__nv_bfloat16>, grid,
-                             k9::kQuantThreads, 0, static_cast<cudaStream_t>(stream), p);
-  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch quantize_kernel");
+  return quantize_rows(x, dtype, ld, M, K, x8, scales, false, static_cast<cudaStream_t>(stream));
 }
 
 size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1) return 0;
+  if (M <= k9::kRowsMax || N < 1 || K < 1) return 0;
   const size_t x8 = (static_cast<size_t>(M) * K + 255) / 256 * 256;
   const size_t xs = (static_cast<size_t>(M) * ((K + 127) / 128) * 4 + 255) / 256 * 256;
   return x8 + xs;
@@ -231,7 +322,10 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
   if (ldo < N && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of out overlap: ldo < N");
   if (!aligned16(x) || !aligned16(w8)) return fail(TMU_ERR_MISALIGNED, "x, w8 must be 16-byte aligned");
   if (x_dtype == TMU_E4M3 && ldx != K) return fail(TMU_ERR_UNSUPPORTED, "e4m3 x must be contiguous");
-  (void)status;
+  if (ldx % 8) return fail(TMU_ERR_MISALIGNED, "ldx must be a multiple of 8");
+  if (ldx < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of x overlap: ldx < K");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (M <= k9::kRowsMax) return launch_k9_rows(x, x_dtype, ldx, x_scales, w8, w_scales, bias, out, out_dtype, ldo, M, N, K, s);
   const uint8_t* x8 = static_cast<const uint8_t*>(x);
   const float* xs = x_scales;
   if (x_dtype != TMU_E4M3) {
@@ -240,29 +334,12 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
     if (!aligned16(workspace)) return fail(TMU_ERR_MISALIGNED, "workspace not 16-byte aligned");
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     float* sc = reinterpret_cast<float*>(ws + (static_cast<size_t>(M) * K + 255) / 256 * 256);
-    int st = tmu_quantize_rows(x, x_dtype, ldx, M, K, ws, sc, stream);
+    int st = quantize_rows(x, x_dtype, ldx, M, K, ws, sc, true, s);
     if (st) return st;
     x8 = ws;
     xs = sc;
   }
-  k9::Params p;
-  memset(&p, 0, sizeof(p));
-  p.x8 = x8;
-  p.xs = xs;
-  p.w8 = static_cast<const uint8_t*>(w8);
-  p.ws = w_scales;
-  p.bias = bias;
-  p.out = out;
-  p.ldo = ldo;
-  p.M = M;
-  p.N = N;
-  p.K = K;
-  p.kb = (K + 127) / 128;
-  p.out_type = out_dtype;
-  const dim3 grid((N + 15) / 16, (M + 15) / 16);
-  k9::linear8_simple_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_simple_kernel");
+  return launch_k9(x8, xs, w8, w_scales, bias, out, out_dtype, ldo, M, N, K, static_cast<DeviceStatus*>(status), s);
 }
 
 }  // extern "C"
