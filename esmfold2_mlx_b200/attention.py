@@ -15,16 +15,37 @@ device; nothing synchronises.  Inference only: an input that asks for gradients 
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from . import _lib
-from .ops import _ptr, _stream_ptr
 
 _DTYPES = {torch.float16: _lib.TMU_F16, torch.bfloat16: _lib.TMU_BF16}
 _NORMS = {None: _lib.TMU_NORM_NONE, "rms": _lib.TMU_NORM_RMS, "layer": _lib.TMU_NORM_LAYER}
+
+
+# The current stream's handle by device index, without making a Stream object for it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(device: torch.device, where: str, *args) -> None:
+    """Call the C entry ``where`` with ``args`` and the current stream of ``device``, which is made the
+    current device for the call if it is not."""
+    fn = getattr(_lib.load(), where)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        code = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code:
+        _lib.check(code, where)
+
+
+def pointer(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def refuse_grad(where: str, *tensors) -> None:
@@ -47,17 +68,19 @@ def spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _check_heads(name: str, t: torch.Tensor, T: int, D: int, like: torch.Tensor) -> None:
-    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D:
-        raise ValueError(f"{name} must be [{T}, heads, {D}], got {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != T or shape[2] != D:
+        raise ValueError(f"{name} must be [{T}, heads, {D}], got {tuple(shape)}")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must have q's type and device")
-    if D > 1 and t.stride(2) != 1:
+    if t.stride(2) != 1 and D > 1:
         raise ValueError(f"the values of a head of {name} must be contiguous")
 
 
 def _heads(t: torch.Tensor) -> _lib.TmuHeads:
     # an axis of length one is never stepped along: its stride is whatever the view happened to have
-    return _lib.TmuHeads(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+    (T, H, _), (st, sh, _) = t.shape, t.stride()
+    return _lib.TmuHeads(t.data_ptr(), st if T > 1 else 0, sh if H > 1 else 0)
 
 
 def _check_first(name: str, q: torch.Tensor) -> int:
@@ -142,12 +165,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
     if norm not in _NORMS:
         raise ValueError("norm must be None, 'rms' or 'layer'")
     refuse_grad("qk_norm_rope", q, k, q_weight, k_weight, q_bias, k_bias)
-    for name, p in (("q_weight", q_weight), ("k_weight", k_weight), ("q_bias", q_bias), ("k_bias", k_bias)):
-        if p is not None:
-            if norm is None:
-                raise ValueError(f"{name} needs a norm")
-            if p.dtype != torch.float32 or p.device != q.device or p.shape != (D,) or not p.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous fp32 [{D}] tensor on q's device")
+    if norm is None:
+        if not (q_weight is k_weight is q_bias is k_bias is None):
+            raise ValueError("weights and biases need a norm")
+    else:
+        for p in (q_weight, k_weight, q_bias, k_bias):
+            if p is not None and (p.dtype != torch.float32 or p.device != q.device or p.shape != (D,)
+                                  or not p.is_contiguous()):
+                raise ValueError(f"weights and biases must be contiguous fp32 [{D}] tensors on q's device")
     rot = _lib.TmuRotary(None, 4, None, 1.0, 0, 0)
     if rotary is not None:
         if rotary.rot > D:
@@ -161,28 +186,31 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
             raise ValueError("the rotary must be on q's device")
         rot = _lib.TmuRotary(positions.data_ptr(), positions.element_size(), rotary.turns.data_ptr(), rotary.gain,
                              rotary.rot, 1 if rotary.layout == "interleaved" else 0)
-    for name, src, dst in (("q_out", q, q_out), ("k_out", k, k_out)):
-        if dst is not None:
-            _check_heads(name, dst, T, D, q)
-            if dst.shape != src.shape:
-                raise ValueError(f"{name} must be shaped like its input")
-            if _self_overlap(dst):
-                raise ValueError(f"{name} must not overlap itself")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=q.dtype, device=q.device) if k_out is None else k_out
-    if _heads_overlap(q_out, k_out):
-        raise ValueError("q_out and k_out must not overlap")
-    for name, src, dst in (("q_out and q", q, q_out), ("k_out and k", k, k_out), ("q_out and k", k, q_out),
-                           ("k_out and q", q, k_out)):
-        same = src.data_ptr() == dst.data_ptr() and src.stride() == dst.stride() and src.shape == dst.shape
-        own = name in ("q_out and q", "k_out and k")
-        if _heads_overlap(src, dst) and not (same and own):
-            raise ValueError(f"{name} must not overlap")
-    nrm = _lib.TmuQkNorm(_NORMS[norm], float(eps), _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias))
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.load().tmu_qk_norm_rope(_heads(q), _heads(k), _heads(q_out), _heads(k_out), nrm, rot, T, hq,
-                                                k.shape[1], D, dtype, _stream_ptr(q.device)), "tmu_qk_norm_rope")
+    if q_out is not None or k_out is not None:
+        _check_rope_outputs(q, k, q_out, k_out)
+    q_out = q.new_empty(q.shape) if q_out is None else q_out
+    k_out = k.new_empty(k.shape) if k_out is None else k_out
+    nrm = _lib.TmuQkNorm(_NORMS[norm], eps, pointer(q_weight), pointer(q_bias), pointer(k_weight), pointer(k_bias))
+    launch(q.device, "tmu_qk_norm_rope", _heads(q), _heads(k), _heads(q_out), _heads(k_out), nrm, rot, T, hq,
+           k.shape[1], D, dtype)
     return q_out, k_out
+
+
+def _check_rope_outputs(q, k, q_out, k_out) -> None:
+    T, _, D = q.shape
+    for name, src, dst, other in (("q_out", q, q_out, k), ("k_out", k, k_out, q)):
+        if dst is None:
+            continue
+        _check_heads(name, dst, T, D, q)
+        if dst.shape != src.shape:
+            raise ValueError(f"{name} must be shaped like its input")
+        if _self_overlap(dst):
+            raise ValueError(f"{name} must not overlap itself")
+        in_place = src.data_ptr() == dst.data_ptr() and src.stride() == dst.stride()
+        if _heads_overlap(dst, other) or (_heads_overlap(dst, src) and not in_place):
+            raise ValueError(f"{name} may be its own input, and must not overlap one otherwise")
+    if q_out is not None and k_out is not None and _heads_overlap(q_out, k_out):
+        raise ValueError("q_out and k_out must not overlap")
 
 
 def _self_overlap(t: torch.Tensor) -> bool:
@@ -254,7 +282,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
         b = _lib.TmuAttnBias(bias.data_ptr(), bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1),
                              bias.stride(2), n)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     else:
         _check_heads("out", out, T, D, q)
         if out.shape != q.shape:
@@ -264,8 +292,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
         if bias is not None and spans_overlap(out, bias):
             raise ValueError("out must not overlap bias")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.load().tmu_attention(_heads(q), _heads(k), _heads(v), _heads(out), _ptr(cu_seqlens), b, S, T, hq,
-                                             k.shape[1], D, dtype, 1 if causal else 0, scale, _ptr(status),
-                                             _stream_ptr(q.device)), "tmu_attention")
+    launch(q.device, "tmu_attention", _heads(q), _heads(k), _heads(v), _heads(out), cu_seqlens.data_ptr(), b, S, T, hq,
+           k.shape[1], D, dtype, 1 if causal else 0, scale, pointer(status))
     return out

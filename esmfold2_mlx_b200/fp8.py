@@ -20,8 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .attention import refuse_grad, spans_overlap
-from .ops import _ptr, _stream_ptr
+from .attention import launch, pointer, refuse_grad, spans_overlap
 
 BLOCK = 128
 F8_MAX = 448.0          # the largest e4m3 value
@@ -109,9 +108,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = x.shape
     x8 = torch.empty(m, k, dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty(m, _blocks(k), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().tmu_quantize_rows(_ptr(x), _IN[x.dtype], _ld(x), m, k, _ptr(x8), _ptr(scales),
-                                                 _stream_ptr(x.device)), "tmu_quantize_rows")
+    launch(x.device, "tmu_quantize_rows", x.data_ptr(), _IN[x.dtype], _ld(x), m, k, x8.data_ptr(), scales.data_ptr())
     return x8, scales
 
 
@@ -151,7 +148,7 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
         dt = out_dtype or (torch.float16 if x.dtype == torch.float8_e4m3fn else x.dtype)
         if dt not in _OUT:
             raise TypeError("out_dtype must be fp16, bf16 or fp32")
-        out = torch.empty(*lead, n, dtype=dt, device=x.device)
+        out = x.new_empty((*lead, n), dtype=dt)
     else:
         if out.shape != (*lead, n) or out.device != x.device or out.dtype not in _OUT:
             raise ValueError(f"out must be an fp16, bf16 or fp32 {[*lead, n]} tensor on x's device")
@@ -160,11 +157,9 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
         if any(t is not None and spans_overlap(out, t) for t in (x, weight.w8, weight.scales, bias, xs)):
             raise ValueError("out must not overlap an input")
     orow = _rows("out", out)
-    lib = _lib.load()
-    with torch.cuda.device(x.device):
-        need = int(lib.tmu_linear_fp8_workspace_bytes(m, n, k))
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        _lib.check(lib.tmu_linear_fp8(_ptr(rows), _IN[x.dtype], _ld(rows), _ptr(xs), _ptr(weight.w8),
-                                      _ptr(weight.scales), _ptr(bias), _ptr(orow), _OUT[out.dtype], _ld(orow), m, n, k,
-                                      _ptr(ws), need, _ptr(status), _stream_ptr(x.device)), "tmu_linear_fp8")
+    need = int(_lib.load().tmu_linear_fp8_workspace_bytes(m, n, k)) if xs is None else 0
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    launch(x.device, "tmu_linear_fp8", rows.data_ptr(), _IN[x.dtype], _ld(rows), pointer(xs), weight.w8.data_ptr(),
+           weight.scales.data_ptr(), pointer(bias), orow.data_ptr(), _OUT[out.dtype], _ld(orow), m, n, k, pointer(ws), need,
+           pointer(status))
     return out

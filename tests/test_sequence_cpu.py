@@ -83,7 +83,7 @@ def test_qk_norm_rope_refusals(lib):
     assert rope(lib, T=0) == OK
 
 
-def linear(lib, x=P, xd=0, ldx=64, xs=None, w=P, ws=P, out=P, od=0, ldo=8, M=2, N=8, K=64, work=P, nb=1 << 20):
+def linear(lib, x=P, xd=0, ldx=64, xs=None, w=P, ws=P, out=P, od=0, ldo=8, M=40, N=8, K=64, work=P, nb=1 << 20):
     return lib.tmu_linear_fp8(x, xd, ldx, xs, w, ws, None, out, od, ldo, M, N, K, work, nb, None, None)
 
 
