@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       // 0 times another sequence's NaN would be a NaN.  This warp made the load, so the phase it
       // waits for is the barrier's current one.
       const int s = (n - 1) % NS, keep = len - (n - 1) * kTile;
-      if (fix && warp_wait(&vfull[s], ((n - 1) / NS) & 1, ctx, kSiteFix)) {
+      if (fix && warp_poll(&vfull[s], ((n - 1) / NS) & 1, ctx, kSiteFix)) {
         for (int c = keep * 8 + lane; c < kTile * 8; c += 32)
           for (int a = 0; a < C::kAtoms; ++a)
             *reinterpret_cast<uint4*>(smem + C::OFF_V + s * C::kTileBytes + a * kAtom + c * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nx; ++j) {
-      if (!(ok = warp_wait(&sfull[x], j & 1, ctx, kSiteSoftS))) break;
+      if (!(ok = warp_poll(&sfull[x], j & 1, ctx, kSiteSoftS))) break;
       tc_fence_after();
       uint32_t r[4][32];
 #pragma unroll
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
       if (j > 0 && C::kOwnP) {  // P's columns and O belong to P V of the last step (else S's being there says so)
-        if (!(ok = warp_wait(&ofull[x], (j - 1) & 1, ctx, kSiteSoftO))) break;
+        if (!(ok = warp_poll(&ofull[x], (j - 1) & 1, ctx, kSiteSoftO))) break;
         tc_fence_after();
       }
       const bool move = top > m + kMoveMax || (m == -INFINITY && top > m);
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) mbar_arrive(&pfull[x]);
     }
-    if (ok && nx > 0 && warp_wait(&ofull[x], (nx - 1) & 1, ctx, kSiteEpi)) {
+    if (ok && nx > 0 && warp_poll(&ofull[x], (nx - 1) & 1, ctx, kSiteEpi)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.o.p) + static_cast<long long>(beg + row) * p.o.st + head * p.o.sh;

@@ -18,14 +18,15 @@
 namespace tmu {
 namespace k9 {
 
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 256, kQuantUnroll = 4;
 
 struct QuantParams {
   const void* x;
   long long ld;
   int M, K, kb;
   uint8_t* x8;  // [M, K]
-  float* xs;    // [M, kb]
+  float* xs;    // scale of row m and block b at m * xs_m + b * xs_b
+  long long xs_m, xs_b;
   int chained;  // the outputs are a workspace that only the next kernel of the same call reads
 };
 
@@ -42,53 +43,94 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-// 8 values a lane, 16 lanes a block of 128 (all of the warp takes part): the block's scale and the lane's e4m3.
+__device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b, __half) {  // of two pairs, keeps a NaN
+  const __half2 r = __hmax2_nan(__habs2(*reinterpret_cast<__half2*>(&a)), __habs2(*reinterpret_cast<__half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 r =
+      __hmax2_nan(__habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 8 values a lane, 16 lanes a block of 128 (all of the warp takes part): the block's scale and the
+// lane's e4m3.  A quotient a / b is rounded correctly from the correctly rounded r = 1 / b: q = a r, then
+// q + (a - q b) r with fused multiply-adds (Markstein 1990; right but for divisors whose significand
+// is all ones: 448 = 7 * 2^6 is none, nor is an 8 or 11-bit number over it, whose 24 bits repeat
+// with the period 3 of sevenths).  The remainder must not underflow, which the scale's lower limit
+// sees to for itself (a quotient below 2^-126 is replaced) and a power of two for the values.
 template <typename T>
 __device__ __forceinline__ void quantize8(const uint32_t (&u)[4], float& s, uint2& o) {
-  float y[8], amax = 0.f;
+  uint32_t m = absmax2(absmax2(u[0], u[1], T()), absmax2(u[2], u[3], T()), T());
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 f = k8::unpack2(u[e], T());
-    y[2 * e] = f.x;
-    y[2 * e + 1] = f.y;
-    amax = max_nan(amax, max_nan(fabsf(f.x), fabsf(f.y)));
-  }
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-  s = max_nan(__fdiv_rn(amax, 448.f), 0x1p-126f);
+  for (int d = 8; d > 0; d >>= 1) m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, d), T());
+  const float2 pair = k8::unpack2(m, T());
+  const float amax = max_nan(pair.x, pair.y);
+  constexpr float r448 = 1.f / 448.f;
+  const float q0 = amax * r448;
+  s = max_nan(amax < INFINITY ? fmaf(fmaf(-q0, 448.f, amax), r448, q0) : amax, 0x1p-126f);
+  const float up = s < 0x1p-60f ? 0x1p66f : 1.f;
+  const float t = s * up, r = __frcp_rn(t);
+  const float2 r2 = make_float2(r, r), nt2 = make_float2(-t, -t);
   uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w[e] = e4m3x2(__fdiv_rn(y[2 * e], s), __fdiv_rn(y[2 * e + 1], s));
+  for (int e = 0; e < 4; ++e) {
+    float2 a = k8::unpack2(u[e], T());
+    if (up != 1.f) a = make_float2(a.x * up, a.y * up);
+    const float2 q = __fmul2_rn(a, r2);
+    const float2 v = __ffma2_rn(__ffma2_rn(q, nt2, a), r2, q);
+    w[e] = e4m3x2(v.x, v.y);
+  }
   o = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-// Half a warp takes one block of 128 of one row: 8 values (16 bytes) a lane, amax by shuffles.
+// Half a warp takes U blocks of 128 of one row (8 values, 16 bytes, a lane and block), all loaded
+// before the first is worked on, and a block of threads sixteen rows, so that the scales of a
+// block of 128, transposed for the tensor-core kernels, are written 64 bytes at a time.
 // Bound: HBM (2 bytes read and 1 written a value).
-template <typename T>
+template <typename T, int U>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantParams p) {
   const int l = threadIdx.x & 15;
-  const long long items = static_cast<long long>(p.M) * p.kb;
-  const long long step = static_cast<long long>(gridDim.x) * (kQuantThreads / 16);
-  const long long first = (static_cast<long long>(blockIdx.x) * kQuantThreads + threadIdx.x) >> 4;
+  const int per = (p.kb + U - 1) / U;
+  const int rows = blockIdx.x / per;
+  const int m = rows * (kQuantThreads / 16) + (threadIdx.x >> 4), b0 = (blockIdx.x - rows * per) * U;
   griddep_wait();
-  // the two halves of a warp run the same number of turns, so the shuffles meet
-  for (long long base = first - ((threadIdx.x >> 4) & 1); base < items; base += step) {
-    const long long it = base + ((threadIdx.x >> 4) & 1);
-    const long long m = it / p.kb;
-    const int b = static_cast<int>(it - m * p.kb), k = b * 128 + l * 8;
-    const bool on = it < items && k < p.K;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (on) raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.ld + k);
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint4 raw[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int k = (b0 + i) * 128 + l * 8;
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (m < p.M && k < p.K) raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.ld + k);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    const int k = (b0 + i) * 128 + l * 8;
     uint2 o;
     float s;
     quantize8<T>(u, s, o);
-    if (on) *reinterpret_cast<uint2*>(p.x8 + m * p.K + k) = o;
-    if (it < items && l == 0) p.xs[m * p.kb + b] = s;
+    if (m < p.M && k < p.K) {
+      *reinterpret_cast<uint2*>(p.x8 + static_cast<long long>(m) * p.K + k) = o;
+      if (l == 0) p.xs[m * p.xs_m + (b0 + i) * p.xs_b] = s;
+    }
   }
   // linear8_rows_kernel reads w8 before its dependency wait, so nothing that could be a weight may
   // be announced before it is visible
   if (p.chained) griddep_trigger();
+}
+
+// Row-major scales [M, kb] to [kb, ld], for the tensor-core kernels.
+struct ScaleParams {
+  const float* xs;
+  float* xst;
+  int M, kb, ld;
+};
+__global__ void __launch_bounds__(256) transpose_scales_kernel(const __grid_constant__ ScaleParams p) {
+  griddep_wait();
+  const int m = blockIdx.x * 256 + threadIdx.x;
+  if (m < p.M)
+    for (int b = 0; b < p.kb; ++b) p.xst[static_cast<long long>(b) * p.ld + m] = p.xs[static_cast<long long>(m) * p.kb + b];
+  griddep_trigger();
 }
 
 enum Out : int { kF16 = 0, kBf16 = 1, kF32 = 2 };
@@ -141,10 +183,10 @@ __device__ __forceinline__ uint4 load_once(const uint8_t* p) {
   return v;
 }
 
-// X: __half or __nv_bfloat16 (quantised here), or uint8_t (e4m3 already).
-template <typename X, int G>
-__global__ void __launch_bounds__(kRowsThreads) linear8_rows_kernel(const __grid_constant__ RowsParams p) {
-  constexpr int kWarps = kRowsThreads / 32;
+// X: __half or __nv_bfloat16 (quantised here), or uint8_t (e4m3 already).  PAIRS: row pairs of x, M <= 2 * PAIRS.
+template <typename X, int PAIRS>
+__global__ void __launch_bounds__(kRowsThreads, PAIRS == 1 ? 4 : PAIRS == 4 ? 3 : 2) linear8_rows_kernel(const __grid_constant__ RowsParams p) {
+  constexpr int kWarps = kRowsThreads / 32, G = PAIRS > 4 ? 2 : 1;
   __shared__ __align__(16) uint8_t xq[kWarps][8 * G][kXPitch];
   __shared__ float xsc[kWarps][8 * G];
   __shared__ float part[kWarps][8 * G][kRowsN + 1];
@@ -165,35 +207,55 @@ __global__ void __launch_bounds__(kRowsThreads) linear8_rows_kernel(const __grid
         v[r][c] = w[r] != nullptr && k < p.K ? load_once(w[r] + k) : make_uint4(0u, 0u, 0u, 0u);
       }
   };
-  uint4 cur[2][2];
+  // row 2 i + lane / 16 of x, 16 lanes of 8 values a row
+  const int l = lane & 15;
+  auto load_x = [&](int b, uint4 (&v)[PAIRS], float (&s)[PAIRS]) {
+    const int k = b * 128 + l * 8;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const int m = 2 * i + (lane >> 4);
+      const bool on = m < p.M && k < p.K;
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (sizeof(X) == 1) {
+        if (on) {
+          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.x) + m * p.ldx + k);
+          v[i].x = u.x;
+          v[i].y = u.y;
+          s[i] = p.xs[static_cast<long long>(m) * p.kb + b];
+        }
+      } else {
+        if (on) v[i] = *reinterpret_cast<const uint4*>(static_cast<const X*>(p.x) + m * p.ldx + k);
+      }
+    }
+  };
+  uint4 cur[2][2], xcur[PAIRS];
+  float scur[PAIRS];
   load_w(warp, cur);  // no kernel that starts its successor early writes a weight, so this need not wait
   griddep_wait();
+  load_x(warp, xcur, scur);
   float total[G][4];
 #pragma unroll
   for (int i = 0; i < G; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) total[i][e] = 0.f;
   for (int b = warp; b < p.kb; b += kWarps) {
-    uint4 next[2][2];
+    uint4 next[2][2], xnext[PAIRS];
+    float snext[PAIRS];
     load_w(b + kWarps, next);
-    // this block of x, two rows at a time: 16 lanes of 8 values a row
-    const int l = lane & 15, k = b * 128 + l * 8;
+    load_x(b + kWarps, xnext, snext);
     __syncwarp();
-    for (int m = lane >> 4; m < 8 * G; m += 2) {
-      uint2 o = make_uint2(0u, 0u);
-      float s = 0.f;
-      const bool on = m < p.M && k < p.K;
-      if constexpr (sizeof(X) == 1) {
-        if (on) o = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.x) + m * p.ldx + k);
-        if (m < p.M) s = __ldg(p.xs + static_cast<long long>(m) * p.kb + b);
-      } else {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (on) raw = *reinterpret_cast<const uint4*>(static_cast<const X*>(p.x) + m * p.ldx + k);
-        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    // (rows past M are staged as they come: a column of products depends on its own row only)
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      if (2 * i >= p.M) break;
+      uint2 o = make_uint2(xcur[i].x, xcur[i].y);
+      float s = scur[i];
+      if constexpr (sizeof(X) != 1) {
+        const uint32_t u[4] = {xcur[i].x, xcur[i].y, xcur[i].z, xcur[i].w};
         quantize8<X>(u, s, o);
       }
-      *reinterpret_cast<uint2*>(&xq[warp][m][l * 8]) = o;
-      if (l == 0) xsc[warp][m] = s;
+      *reinterpret_cast<uint2*>(&xq[warp][2 * i + (lane >> 4)][l * 8]) = o;
+      if (l == 0) xsc[warp][2 * i + (lane >> 4)] = s;
     }
     __syncwarp();
     const float ws = __ldg(p.ws + static_cast<long long>(n0 >> 7) * p.kb + b);
@@ -216,6 +278,11 @@ __global__ void __launch_bounds__(kRowsThreads) linear8_rows_kernel(const __grid
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int c = 0; c < 2; ++c) cur[r][c] = next[r][c];
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      xcur[i] = xnext[i];
+      scur[i] = snext[i];
+    }
   }
 #pragma unroll
   for (int i = 0; i < G; ++i) {
@@ -239,40 +306,48 @@ __global__ void __launch_bounds__(kRowsThreads) linear8_rows_kernel(const __grid
 // ------------------------------------------------------------------------------------------
 // Many rows.  A block takes 128 rows of x (TMEM lanes) and 128 of w8 (TMEM columns), whose block
 // of 128 has one scale: a thread holds one row's sums of 64 columns, and a step adds
-// xs[row, b] * ws[b] times the step's products, read from one of four TMEM slots.
-//   warp 0      TMA: x8 and w8 through a ring of kStages steps
-//   warp 1      TMEM and the MMAs (four of K = 32 a step)
-//   warps 2-3   idle
-//   warps 4-11  sums: two warps a TMEM lane quadrant, each on half of the columns
+// xs[row, b] * ws[b] times the step's products, read from one of two TMEM slots.
+//   warps 0-7   sums: two warps a TMEM lane quadrant, each on half of the columns
+//   warp 8      TMA: x8 and w8 through a ring of kStages steps
+//   warp 9      TMEM and the MMAs (four of K = 32 a step)
+// Two blocks an SM, so one's start and end and its waits fall into the other's work.
+// The scales of a step's rows come with its operands, through a ring of their own: a step's are read
+// before its TMEM slot is handed back, and the MMAs are at most two steps ahead of that and the
+// loads kStages steps ahead of the MMAs, so kStages + 2 buffers are never overrun.  (Read from
+// global memory by each thread, a sector a row, they cost as much L2 traffic as half the operands: the pair
+// kernel took 690 us at 16384 x 2560 x 10240 with an L1 that holds them and 1118 without.)
 // Few tiles: a cluster of blocks shares one tile along K.  Each leaves its sums in shared memory
 // and adds its share of the columns over the cluster's blocks, in rank order.
 // ------------------------------------------------------------------------------------------
 constexpr int kTile = 128;
-constexpr int kStages = 5;
-constexpr int kSlots = 4;
-constexpr int kThreads = 384;
+constexpr int kStages = 3;
+constexpr int kSlots = 2;
+constexpr int kThreads = 320;
 constexpr int kOperand = kTile * 128;
 constexpr int OFF_A = 0;
 constexpr int OFF_B = kStages * kOperand;
-constexpr int OFF_BAR = 2 * kStages * kOperand;
+constexpr int OFF_XS = 2 * kStages * kOperand;  // kStages + 2 buffers of 128 scales
+constexpr int OFF_BAR = OFF_XS + (kStages + 2) * 512;
 constexpr int SMEM_BYTES = OFF_BAR + 256;
+constexpr int kOutPitch = 80, kOutBytes = 32 * kOutPitch;  // a warp's staged rows of the output
 constexpr int kSumPitch = kTile + 4;  // floats of a row of sums in shared memory (over the ring)
-static_assert(SMEM_BYTES <= 232448 && kTile * kSumPitch * 4 <= OFF_BAR, "K9 shared memory");
+static_assert(2 * (SMEM_BYTES + 1024) <= 233472 && kTile * kSumPitch * 4 + 8 * kOutBytes <= OFF_BAR, "K9 shared memory");
 
 struct Params {
   CUtensorMap tm_x, tm_w;  // [rows, K] bytes: box {128, 128}, 128B swizzle, zero past the ends
-  const float* xs;
+  const float* xst;  // [kb, ld_xs]: x's scales, rows of x fastest, ld_xs M rounded up to 256
   const float* ws;
   const float* bias;
   void* out;
   long long ldo;
+  int ld_xs;
   int M, N, kb, out_type, vec;  // vec: rows of out take 16-byte stores
   int tiles_m, split;           // blocks of a cluster share a tile along K
   DeviceStatus* status;
   unsigned long long timeout_ns;
 };
 
-enum Site : unsigned int { kSiteProd = 0x901, kSiteMma = 0x902, kSiteSlot = 0x903, kSiteSum = 0x904, kSiteLayout = 0x9ff };
+enum Site : unsigned int { kSiteProd = 0x901, kSiteMma = 0x902, kSiteSlot = 0x903, kSiteSum = 0x904, kSiteScale = 0x905, kSiteLayout = 0x9ff };
 
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -283,37 +358,75 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_
       : "memory");
 }
 
+// 128 scales into shared memory, counted on `bar`.
+__device__ __forceinline__ void load_scales(void* dst, const float* src, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 512);
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 512, [%2];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // Instruction descriptor of kind::f8f6f4 with e4m3 operands (format 0), K-major, fp32 sums.
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) { return idesc_f16_f32(M, N, false, false); }
 
-// 16 sums of row m from column n on, with the bias, to the output.
-__device__ __forceinline__ void store16(const Params& p, int m, int n, const float (&v)[16]) {
-  float y[16];
+// A warp's sums to the output: lane = row m0 + lane, 64 columns from n0 on, with the bias.  64 bytes of
+// each row at a time go through shared memory (rows 80 bytes apart, so eight lanes' 16-byte accesses
+// meet 8 different bank groups), from where four lanes write a row's 16-byte pieces, or, with
+// unaligned rows of out, 32 lanes its single values: written straight from the lane of the row, an unaligned
+// output took 32 us at 1283 x 1000 x 1360, most of it in its 2-byte stores.
+__device__ __forceinline__ void store_rows(const Params& p, uint8_t* buf, int m0, int n0, const float (&sum)[64]) {
+  const int lane = threadIdx.x & 31;
+  float b0 = 0.f, b1 = 0.f;  // bias of columns n0 + lane, n0 + 32 + lane
+  if (p.bias != nullptr) {
+    if (n0 + lane < p.N) b0 = __ldg(p.bias + n0 + lane);
+    if (n0 + 32 + lane < p.N) b1 = __ldg(p.bias + n0 + 32 + lane);
+  }
+  const bool wide = p.out_type == kF32;
+  const int es = wide ? 4 : 2, cols = 64 / es;  // columns of a pass
 #pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = v[e] + (p.bias != nullptr && n + e < p.N ? __ldg(p.bias + n + e) : 0.f);
-  const long long at = static_cast<long long>(m) * p.ldo + n;
-  if (p.vec && n + 16 <= p.N) {
-    if (p.out_type == kF32) {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+  for (int g = 0; g < 4; ++g) {  // 16 columns a step
+    float y[16];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dst[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+    for (int e = 0; e < 16; ++e) y[e] = sum[g * 16 + e] + __shfl_sync(0xffffffffu, g < 2 ? b0 : b1, (g & 1) * 16 + e);
+    uint4* row = reinterpret_cast<uint4*>(buf + lane * kOutPitch);
+    if (wide) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        row[e] = make_uint4(__float_as_uint(y[4 * e]), __float_as_uint(y[4 * e + 1]), __float_as_uint(y[4 * e + 2]),
+                            __float_as_uint(y[4 * e + 3]));
     } else {
       uint32_t u[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         u[e] = p.out_type == kF16 ? k8::pack2(y[2 * e], y[2 * e + 1], __half()) : k8::pack2(y[2 * e], y[2 * e + 1], __nv_bfloat16());
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
-      dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
-      dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
+      row[(g & 1) * 2] = make_uint4(u[0], u[1], u[2], u[3]);
+      row[(g & 1) * 2 + 1] = make_uint4(u[4], u[5], u[6], u[7]);
+      if (!(g & 1)) continue;
     }
-  } else {
+    const int c0 = n0 + (wide ? g * 16 : (g >> 1) * 32);
+    __syncwarp();
+    if (p.vec && c0 + cols <= p.N) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (n + e < p.N) store_out(p.out, p.out_type, at + e, y[e]);
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        if (m0 + r < p.M)
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + ((m0 + r) * p.ldo + c0) * es + (lane & 3) * 16) =
+              *reinterpret_cast<const uint4*>(buf + r * kOutPitch + (lane & 3) * 16);
+      }
+    } else {
+      for (int i = lane; i < 32 * cols; i += 32) {
+        const int r = i / cols, c = i - r * cols;
+        if (m0 + r >= p.M || c0 + c >= p.N) continue;
+        const long long at = (m0 + r) * p.ldo + c0 + c;
+        if (wide) static_cast<float*>(p.out)[at] = *reinterpret_cast<const float*>(buf + r * kOutPitch + c * 4);
+        else static_cast<uint16_t*>(p.out)[at] = *reinterpret_cast<const uint16_t*>(buf + r * kOutPitch + c * 2);
+      }
+    }
+    __syncwarp();
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 1) linear8_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem[];
   DeviceStatus* const status = p.status != nullptr ? p.status : &g_own_status;
   const bool laid = (smem_u32(smem) & 1023) == 0;  // uniform over the grid
@@ -326,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_kernel(const __grid_const
   uint64_t* empty = bars + kStages;           // [kStages]
   uint64_t* sfull = bars + 2 * kStages;       // [kSlots] a step's products are in the slot
   uint64_t* sempty = sfull + kSlots;          // [kSlots] its eight readers have them
-  uint64_t& drain_bar = sempty[kSlots];
+  uint64_t* xfull = sempty + kSlots;          // [kStages + 2] a step's scales are in shared memory
+  uint64_t& drain_bar = xfull[kStages + 2];
   uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
   volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
   const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
@@ -345,13 +459,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_kernel(const __grid_const
       mbar_init(&sfull[s], 1);
       mbar_init(&sempty[s], 8);
     }
+    for (int s = 0; s < kStages + 2; ++s) mbar_init(&xfull[s], 1);
     mbar_init(&drain_bar, 1);
     fence_mbar_init();
     tma_prefetch_desc(&p.tm_x);
     tma_prefetch_desc(&p.tm_w);
   }
-  if (warp == 1) {
-    tmem_alloc(&tmem_base_sh, 512);
+  if (warp == 9) {
+    tmem_alloc(&tmem_base_sh, kSlots * kTile);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -362,12 +477,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_kernel(const __grid_const
   griddep_wait();
 
   float sum[64];
-  if (warp == 0) {
+  if (warp == 8) {
     if (lane == 0) {
       int i = 0;
       for (int b = b0; b < b1; ++b, ++i) {
         const int s = i % kStages;
         if (!mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, ctx, kSiteProd)) break;
+        const int x = i % (kStages + 2);
+        load_scales(smem + OFF_XS + x * 512, p.xst + static_cast<long long>(b) * p.ld_xs + m0, &xfull[x]);
         mbar_arrive_expect_tx(&full[s], 2 * kOperand);
         tma_load_2d(smem + OFF_A + s * kOperand, &p.tm_x, &full[s], b * 128, m0);
         tma_load_2d(smem + OFF_B + s * kOperand, &p.tm_w, &full[s], b * 128, n0);
@@ -377,8 +494,13 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_kernel(const __grid_const
           const int armed = i > s ? (i - s + kStages - 1) / kStages : 0;
           if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
         }
+      if (abort_sh)
+        for (int x = 0; x < kStages + 2; ++x) {
+          const int armed = i > x ? (i - x + kStages + 1) / (kStages + 2) : 0;
+          if (armed) mbar_drain(&xfull[x], (armed - 1) & 1, 200000000ull);
+        }
     }
-  } else if (warp == 1) {
+  } else if (warp == 9) {
     if (lane == 0) {
       const uint32_t idesc = idesc_e4m3_f32(kTile, kTile);
       const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
@@ -397,92 +519,327 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_kernel(const __grid_const
       umma_commit(&drain_bar);
       mbar_drain(&drain_bar, 0, 200000000ull);
     }
-  } else if (warp >= 4) {
-    const int q = warp & 3, half = (warp - 4) >> 2;
-    const int m = m0 + q * 32 + lane;
+  } else {
+    const int q = warp & 3, half = warp >> 2;
     const uint32_t tl = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * 64;
-    const float* xs = p.xs + static_cast<long long>(min(m, p.M - 1)) * p.kb;
     const float* ws = p.ws + static_cast<long long>(n0 >> 7) * p.kb;
 #pragma unroll
     for (int e = 0; e < 64; ++e) sum[e] = 0.f;
-    float sc = b0 < b1 ? __ldg(xs + b0) * __ldg(ws + b0) : 0.f;
+    // the weight's scales: lane j holds that of step 32 i + j, and of the next 32 steps
+    auto load_ws = [&](int b) { return b + lane < b1 ? __ldg(ws + b + lane) : 0.f; };
+    float w0 = load_ws(b0), w1 = load_ws(b0 + 32);
     for (int b = b0; b < b1; ++b) {
       const int i = b - b0, c = i % kSlots;
-      const float next = b + 1 < b1 ? __ldg(xs + b + 1) * __ldg(ws + b + 1) : 0.f;
-      if (!warp_wait(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum)) break;
+      if (i > 0 && (i & 31) == 0) {
+        w0 = w1;
+        w1 = load_ws(b + 32);
+      }
+      const int x = i % (kStages + 2);
+      if (!warp_poll(&xfull[x], (i / (kStages + 2)) & 1, ctx, kSiteScale)) break;
+      const float sc = __shfl_sync(0xffffffffu, w0, i & 31) * reinterpret_cast<const float*>(smem + OFF_XS + x * 512)[q * 32 + lane];
+      if (!warp_poll(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum)) break;
       tc_fence_after();
-      uint32_t r[2][32];
-      tmem_ld32(tl + c * kTile, r[0]);
-      tmem_ld32(tl + c * kTile + 32, r[1]);
-      tmem_wait_ld2(r[0], r[1]);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sempty[c]);
       const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const float2 v = make_float2(__uint_as_float(r[e >> 4][(2 * e) & 31]), __uint_as_float(r[e >> 4][(2 * e + 1) & 31]));
-        const float2 a = __ffma2_rn(v, s2, make_float2(sum[2 * e], sum[2 * e + 1]));
-        sum[2 * e] = a.x;
-        sum[2 * e + 1] = a.y;
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[32];
+        tmem_ld32(tl + c * kTile + h * 32, r);
+        tmem_wait_ld(r);
+        if (h == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sempty[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
+          a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
+        }
       }
-      sc = next;
     }
-    if (p.split == 1 && m < p.M)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v[16];
-#pragma unroll
-        for (int f = 0; f < 16; ++f) v[f] = sum[e * 16 + f];
-        store16(p, m, n0 + half * 64 + e * 16, v);
-      }
   }
 
-  if (p.split > 1) {
-    // the ring's last reads are done: a block's sums replace its operands
-    __syncthreads();
+  __syncthreads();  // the ring's last reads are done: sums and staged rows take its place
+  if (p.split == 1) {
+    if (warp < 8) store_rows(p, smem + warp * kOutBytes, m0 + (warp & 3) * 32, n0 + (warp >> 2) * 64, sum);
+  } else {
     float* sums = reinterpret_cast<float*>(smem);
-    if (warp >= 4) {
-      const int row = (warp & 3) * 32 + lane, c0 = ((warp - 4) >> 2) * 64;
+    if (warp < 8) {
+      const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * 64;
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         *reinterpret_cast<float4*>(sums + row * kSumPitch + c0 + 4 * e) = make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]);
     }
     cluster_sync_all();
-    // share r of the tile: groups of 16 columns of a row, dealt over the cluster's threads
-    for (int i = rank * kThreads + threadIdx.x; i < kTile * 8; i += p.split * kThreads) {
-      const int row = i >> 3, c = (i & 7) * 16;
-      if (m0 + row >= p.M) continue;
-      float v[16];
+    // pieces of 32 rows by 64 columns, dealt over the cluster's warps
+    for (int i = rank * 8 + warp; warp < 8 && i < 8; i += p.split * 8) {
+      const int row = (i & 3) * 32 + lane, c = (i >> 2) * 64;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = 0.f;
+      for (int e = 0; e < 64; ++e) sum[e] = 0.f;
       for (int r = 0; r < p.split; ++r) {
         const uint32_t src = cluster_addr(sums + row * kSumPitch + c, r);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 16; ++e) {
           float4 f;
           asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                        : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
                        : "r"(src + e * 16)
                        : "memory");
-          v[4 * e] += f.x;
-          v[4 * e + 1] += f.y;
-          v[4 * e + 2] += f.z;
-          v[4 * e + 3] += f.w;
+          sum[4 * e] += f.x;
+          sum[4 * e + 1] += f.y;
+          sum[4 * e + 2] += f.z;
+          sum[4 * e + 3] += f.w;
         }
       }
-      store16(p, m0 + row, n0 + c, v);
+      store_rows(p, smem + kTile * kSumPitch * 4 + warp * kOutBytes, m0 + (i & 3) * 32, n0 + c, sum);
     }
     __syncwarp();
     cluster_sync_all();  // nobody leaves while its sums are being read
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, kSlots * kTile);
   }
 }
 
+
+// ------------------------------------------------------------------------------------------
+// Many rows and columns: the same sums on CTA pairs, 256 rows of x by 256 of w8 a tile, through
+// MMAs that span both SMs (M = 256): each CTA brings half of either operand, so an SM reads half
+// the bytes a product of the 128 x 128 tiles' kernel, whose reads the L2 cannot feed at the tensor
+// cores' rate.  CTA r holds the sums of rows [128 r, + 128) of the tile.  One pair a two SMs,
+// persistent over tiles; tiles go in groups of kGroup row tiles by all column tiles, so the
+// operands of the tiles that run together stay in L2.
+//
+// A step's products are needed apart from the next step's, and TMEM holds two steps (512
+// columns), so the rate hangs on how soon a slot is free again: the step is made as two halves of
+// 128 columns with a slot each (the sums of one start while the other is made), and sixteen warps
+// take the products out, 64 columns each.
+//   warp 0      TMA of this CTA's halves, counted on the even CTA's barrier (.cta_group::2)
+//   warp 1      TMEM and, in the even CTA, the MMAs (N = 128, four of K = 32 a half)
+//   warps 2-3   idle (they complete the warpgroup that gives its registers to the sums)
+//   warps 4-19  sums: half h of the columns = warps 4 + 8 h .., two warps a TMEM lane quadrant
+// ------------------------------------------------------------------------------------------
+namespace pair {
+
+constexpr int kStages = 5;
+constexpr int kThreads = 640;
+constexpr int kTileMN = 256;
+constexpr int kGroup = 8;
+constexpr int kSumRegs = 104, kOtherRegs = 64;  // 512 * 104 + 128 * 64 = 640 * 96
+constexpr int OFF_A = 0;
+constexpr int OFF_B = kStages * kOperand;
+constexpr int OFF_XS = 2 * kStages * kOperand;  // kStages + 2 buffers of 128 scales
+constexpr int OFF_OUT = OFF_XS + (kStages + 2) * 512;  // staged rows of the output, a warp each
+constexpr int OFF_BAR = OFF_OUT + 16 * kOutBytes;
+constexpr int SMEM_BYTES = OFF_BAR + 256;
+static_assert(SMEM_BYTES <= 232448, "K9 pair shared memory");
+
+enum Site : unsigned int { kSiteProd = 0x911, kSiteMma = 0x912, kSiteSlot = 0x913, kSiteSum = 0x914, kSiteScale = 0x915, kSiteLayout = 0x91f };
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// A load into this CTA's shared memory whose bytes count on `bar`, a barrier of either CTA of the
+// pair (a shared::cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
+// Arrive on the even CTA's barrier to hand a TMEM slot back.  The loads from it have completed and
+// are ordered by tcgen05.fence::before_thread_sync; no memory write is handed over, so the arrive
+// needs no cluster-scope release (with one, and with cluster-scope waits on the MMAs' commits, a step took
+// 20 % longer at 4096 x 4736 x 2560).
+__device__ __forceinline__ void arrive_slot(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// Tile t: row tiles in groups of kGroup, column tiles inside a group, row tiles fastest.
+__device__ __forceinline__ void decode(const Params& p, int t, int& m0, int& n0) {
+  const int tiles_n = (p.N + kTileMN - 1) / kTileMN;
+  const int per = kGroup * tiles_n, g = t / per, r = t - g * per;
+  const int rows = min(kGroup, p.tiles_m - g * kGroup);
+  m0 = (g * kGroup + r % rows) * kTileMN;
+  n0 = r / rows * kTileMN;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem[];
+  DeviceStatus* const status = p.status != nullptr ? p.status : &g_own_status;
+  if (smem_u32(smem) & 1023) {  // a property of the kernel: both CTAs take the same branch
+    if (threadIdx.x == 0) record_status(status, kStatusLayout, kSiteLayout);
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
+  uint64_t* full = bars;              // [kStages] even CTA: both CTAs' halves have landed
+  uint64_t* empty = bars + kStages;   // [kStages] the paired MMAs have read the stage (both CTAs)
+  uint64_t* sfull = bars + 2 * kStages;  // [2] a step's products are in the slot (both CTAs)
+  uint64_t* sempty = sfull + 2;          // [2] even CTA: the 32 reading warps of both CTAs have them
+  uint64_t* xfull = sempty + 2;          // [kStages + 2] a step's scales are in shared memory (each CTA's)
+  uint64_t& drain_bar = xfull[kStages + 2];
+  uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
+  volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
+  const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int tiles = p.tiles_m * ((p.N + kTileMN - 1) / kTileMN);
+  if (threadIdx.x == 0) {
+    abort_sh = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sfull[s], 1);
+      mbar_init(&sempty[s], 32);
+    }
+    for (int s = 0; s < kStages + 2; ++s) mbar_init(&xfull[s], 1);
+    mbar_init(&drain_bar, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&p.tm_x);
+    tma_prefetch_desc(&p.tm_w);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&tmem_base_sh, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before any arrive across
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  griddep_trigger();
+  griddep_wait();
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 0 && lane == 0) {
+      uint32_t i = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step) {
+        int m0, n0;
+        decode(p, t, m0, n0);
+        for (int b = 0; b < p.kb; ++b, ++i) {
+          const uint32_t s = i % kStages;
+          if (!(ok = mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, ctx, kSiteProd))) break;
+          const uint32_t x = i % (kStages + 2);
+          load_scales(smem + OFF_XS + x * 512, p.xst + static_cast<long long>(b) * p.ld_xs + m0 + rank * kTile, &xfull[x]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
+          const uint32_t bar = cluster_addr(&full[s], 0);
+          tma_load_2d_pair(smem + OFF_A + s * kOperand, &p.tm_x, bar, b * 128, m0 + static_cast<int>(rank) * kTile);
+          tma_load_2d_pair(smem + OFF_B + s * kOperand, &p.tm_w, bar, b * 128, n0 + static_cast<int>(rank) * kTile);
+        }
+      }
+      if (abort_sh && rank == 0)
+        for (uint32_t s = 0; s < kStages; ++s) {
+          const uint32_t armed = i > s ? (i - s + kStages - 1) / kStages : 0;
+          if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
+        }
+      if (abort_sh)
+        for (uint32_t x = 0; x < kStages + 2; ++x) {
+          const uint32_t armed = i > x ? (i - x + kStages + 1) / (kStages + 2) : 0;
+          if (armed) mbar_drain(&xfull[x], (armed - 1) & 1, 200000000ull);
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_e4m3_f32(kTileMN, kTileMN);
+      const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
+      uint32_t i = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += step)
+        for (int b = 0; ok && b < p.kb; ++b, ++i) {
+          const uint32_t s = i % kStages, c = i & 1;
+          if (!(ok = mbar_wait(&full[s], (i / kStages) & 1, ctx, kSiteMma))) break;
+          if (!(ok = mbar_wait(&sempty[c], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f8_pair(tmem + c * 256, sdesc_add(ad, s * kOperand + k * 32), sdesc_add(bd, s * kOperand + k * 32), idesc,
+                         k > 0 ? 1u : 0u);
+          umma_commit_pair(&sfull[c], 0x3);
+          umma_commit_pair(&empty[s], 0x3);
+        }
+      umma_commit_pair(&drain_bar, 0x1);
+      mbar_drain(&drain_bar, 0, 200000000ull);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+    const int q = warp & 3, half = (warp - 4) >> 3, col = half * kTile + ((warp >> 2) & 1 ? 0 : 64);
+    const uint32_t tl = tmem + (static_cast<uint32_t>(q * 32) << 16) + col;
+    const uint32_t slots = cluster_addr(&sempty[0], 0);
+    const int nb_last = (p.N + 127) / 128 - 1;
+    uint32_t i = 0;
+    bool ok = true;
+    for (int t = first; ok && t < tiles; t += step) {
+      int m0, n0;
+      decode(p, t, m0, n0);
+      const float* ws = p.ws + static_cast<long long>(min((n0 >> 7) + half, nb_last)) * p.kb;
+      float sum[64];
+#pragma unroll
+      for (int e = 0; e < 64; ++e) sum[e] = 0.f;
+      // the weight's scales: lane j holds that of step 32 i + j, and of the next 32 steps
+      auto load_ws = [&](int b) { return b + lane < p.kb ? __ldg(ws + b + lane) : 0.f; };
+      float w0 = load_ws(0), w1 = load_ws(32);
+      for (int b = 0; b < p.kb; ++b, ++i) {
+        const uint32_t c = i & 1;
+        if (b > 0 && (b & 31) == 0) {
+          w0 = w1;
+          w1 = load_ws(b + 32);
+        }
+        const uint32_t x = i % (kStages + 2);
+        if (!(ok = warp_poll(&xfull[x], (i / (kStages + 2)) & 1, ctx, kSiteScale))) break;
+        const float sc = __shfl_sync(0xffffffffu, w0, b & 31) * reinterpret_cast<const float*>(smem + OFF_XS + x * 512)[q * 32 + lane];
+        if (!(ok = warp_poll(&sfull[c], (i >> 1) & 1, ctx, kSiteSum))) break;
+        tc_fence_after();
+        const float2 s2 = make_float2(sc, sc);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          tmem_ld32(tl + c * 256 + h * 32, r);
+          tmem_wait_ld(r);
+          if (h == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (rank == 0) mbar_arrive(&sempty[c]);
+              else arrive_slot(slots + c * sizeof(uint64_t));
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
+            a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
+          }
+        }
+      }
+      if (ok) store_rows(p, smem + OFF_OUT + (warp - 4) * kOutBytes, m0 + static_cast<int>(rank) * kTile + q * 32, n0 + col, sum);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // neither CTA leaves (or frees the pair's TMEM) while the other can still arrive on its barriers
+  // or run a paired MMA over its shared memory
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+}  // namespace pair
 }  // namespace k9
 }  // namespace tmu

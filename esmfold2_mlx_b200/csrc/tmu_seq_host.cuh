@@ -12,6 +12,9 @@ int seq_device(Dev& d, int bit, const void* kernel, int smem) {
   if (st) return st;
   if (g_seq_attr_done[d.id] >> bit & 1) return TMU_OK;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // all of the SM's memory for blocks: some kernels run two an SM
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
   g_seq_attr_done[d.id] |= 1ull << bit;
   return TMU_OK;
@@ -65,6 +68,11 @@ int launch_k7(const k7::Params& p, bool bf16, bool biased, int blocks, cudaStrea
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_kernel");
 }
 
+template <typename X>
+void (*k9_rows_kernel(int M))(k9::RowsParams) {
+  return M <= 2 ? k9::linear8_rows_kernel<X, 1> : M <= 8 ? k9::linear8_rows_kernel<X, 4> : k9::linear8_rows_kernel<X, 8>;
+}
+
 int launch_k9_rows(const void* x, int x_dtype, long long ldx, const float* xs, const void* w8, const float* ws,
                    const float* bias, void* out, int out_dtype, long long ldo, int M, int N, int K, cudaStream_t stream) {
   k9::RowsParams p;
@@ -82,13 +90,8 @@ int launch_k9_rows(const void* x, int x_dtype, long long ldx, const float* xs, c
   p.K = K;
   p.kb = (K + 127) / 128;
   p.out_type = out_dtype;
-  void (*kern)(k9::RowsParams);
-  if (M <= 8)
-    kern = x_dtype == TMU_F16 ? k9::linear8_rows_kernel<__half, 1>
-           : x_dtype == TMU_BF16 ? k9::linear8_rows_kernel<__nv_bfloat16, 1> : k9::linear8_rows_kernel<uint8_t, 1>;
-  else
-    kern = x_dtype == TMU_F16 ? k9::linear8_rows_kernel<__half, 2>
-           : x_dtype == TMU_BF16 ? k9::linear8_rows_kernel<__nv_bfloat16, 2> : k9::linear8_rows_kernel<uint8_t, 2>;
+  void (*kern)(k9::RowsParams) = x_dtype == TMU_F16    ? k9_rows_kernel<__half>(M)
+                                 : x_dtype == TMU_BF16 ? k9_rows_kernel<__nv_bfloat16>(M) : k9_rows_kernel<uint8_t>(M);
   cudaError_t e = launch_pdl(kern, (N + k9::kRowsN - 1) / k9::kRowsN, k9::kRowsThreads, 0, stream, p);
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_rows_kernel");
 }
@@ -98,22 +101,32 @@ int encode_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t K) {
   int st = get_encoder();
   if (st) return st;
   const cuuint64_t dims[2] = {K, rows}, strides[1] = {K};
-  const cuuint32_t box[2] = {128, 128}, es[2] = {1, 1};
+  const cuuint32_t box[2] = {128, k9::kTile}, es[2] = {1, 1};
   CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? TMU_OK : fail(TMU_ERR_DRIVER, "cuTensorMapEncodeTiled failed for an 8-bit operand");
 }
 
-int launch_k9(const void* x8, const float* xs, const void* w8, const float* ws, const float* bias, void* out, int out_dtype,
+// The workspace: x's scales [kb, M rounded up to 256], then x8 [M, K].
+size_t k9_scale_bytes(int M, int K) {
+  return static_cast<size_t>((M + 255) / 256) * 256 * ((K + 127) / 128) * 4;
+}
+
+int launch_k9(const void* x8, const float* xst, int ld_xs, const void* w8, const float* ws, const float* bias, void* out, int out_dtype,
               long long ldo, int M, int N, int K, DeviceStatus* status, cudaStream_t stream) {
   Dev dev;
   int st = seq_device(dev, 8, reinterpret_cast<const void*>(&k9::linear8_kernel), k9::SMEM_BYTES);
+  if (!st) st = seq_device(dev, 9, reinterpret_cast<const void*>(&k9::pair::linear8_pair_kernel), k9::pair::SMEM_BYTES);
   if (st) return st;
   k9::Params p;
   memset(&p, 0, sizeof(p));
-  if ((st = encode_bytes(&p.tm_x, x8, M, K)) || (st = encode_bytes(&p.tm_w, w8, N, K))) return st;
-  p.xs = xs;
+  const long long pair_m = (M + 255) / 256, pair_tiles = pair_m * ((N + 255) / 256);
+  const bool pairs_of_ctas = pair_tiles >= dev.sms && pair_tiles <= 0x7fffffffll;
+  if ((st = encode_bytes(&p.tm_x, x8, M, K)) || (st = encode_bytes(&p.tm_w, w8, N, K)))
+    return st;
+  p.xst = xst;
+  p.ld_xs = ld_xs;
   p.ws = ws;
   p.bias = bias;
   p.out = out;
@@ -124,14 +137,26 @@ int launch_k9(const void* x8, const float* xs, const void* w8, const float* ws, 
   p.out_type = out_dtype;
   const int es = out_dtype == TMU_F32 ? 4 : 2;
   p.vec = aligned16(out) && ldo * es % 16 == 0;
+  p.status = status;
+  p.timeout_ns = g_timeout_ns;
+  if (pairs_of_ctas) {
+    static int max_pairs[kMaxDevices] = {0};
+    if (max_pairs[dev.id] == 0) {
+      const int r = max_resident_pairs(&k9::pair::linear8_pair_kernel, k9::pair::kThreads, k9::pair::SMEM_BYTES);
+      max_pairs[dev.id] = r > 0 ? r : std::max(1, dev.sms / 2);
+    }
+    p.tiles_m = static_cast<int>(pair_m);
+    const int pairs = static_cast<int>(std::min<long long>(pair_tiles, max_pairs[dev.id]));
+    cudaError_t e = launch_pdl_pair(&k9::pair::linear8_pair_kernel, 2 * pairs, k9::pair::kThreads, k9::pair::SMEM_BYTES,
+                                    stream, p);
+    return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_pair_kernel");
+  }
   p.tiles_m = (M + k9::kTile - 1) / k9::kTile;
   const long long tiles = static_cast<long long>(p.tiles_m) * ((N + k9::kTile - 1) / k9::kTile);
   // blocks of a cluster share a tile along K while the card has room for more blocks
   p.split = 1;
   while (p.split < 8 && tiles * p.split * 2 <= dev.sms && p.kb >= p.split * 4) p.split *= 2;
   if (tiles * p.split > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "M and N are too large");
-  p.status = status;
-  p.timeout_ns = g_timeout_ns;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
   cfg.blockDim = dim3(k9::kThreads);
@@ -150,8 +175,8 @@ int launch_k9(const void* x8, const float* xs, const void* w8, const float* ws, 
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_kernel");
 }
 
-int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, bool chained,
-                  cudaStream_t stream) {
+int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, long long xs_m,
+                  long long xs_b, bool chained, cudaStream_t stream) {
   if (M < 0 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, K positive");
   if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
   if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
@@ -171,11 +196,18 @@ int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8
   p.kb = (K + 127) / 128;
   p.x8 = static_cast<uint8_t*>(x8);
   p.xs = scales;
+  p.xs_m = xs_m;
+  p.xs_b = xs_b;
   p.chained = chained;
-  const long long items = static_cast<long long>(M) * p.kb;
-  const int grid = static_cast<int>(std::min<long long>((items + 15) / 16, 8ll * dev.sms));
-  cudaError_t e = launch_pdl(dtype == TMU_F16 ? k9::quantize_kernel<__half> : k9::quantize_kernel<__nv_bfloat16>, grid,
-                             k9::kQuantThreads, 0, stream, p);
+  // four blocks of 128 a half-warp once that still gives every SM eight blocks of threads
+  const long long groups = (M + 15) / 16;
+  const bool four = groups * ((p.kb + 3) / 4) >= 8ll * dev.sms;
+  const long long grid = groups * (four ? (p.kb + 3) / 4 : p.kb);
+  if (grid > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "M and K are too large");
+  void (*kern)(k9::QuantParams) =
+      dtype == TMU_F16 ? (four ? k9::quantize_kernel<__half, 4> : k9::quantize_kernel<__half, 1>)
+                       : (four ? k9::quantize_kernel<__nv_bfloat16, 4> : k9::quantize_kernel<__nv_bfloat16, 1>);
+  cudaError_t e = launch_pdl(kern, static_cast<int>(grid), k9::kQuantThreads, 0, stream, p);
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch quantize_kernel");
 }
 
@@ -300,14 +332,12 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
 }
 
 int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, void* stream) {
-  return quantize_rows(x, dtype, ld, M, K, x8, scales, false, static_cast<cudaStream_t>(stream));
+  return quantize_rows(x, dtype, ld, M, K, x8, scales, (K + 127) / 128, 1, false, static_cast<cudaStream_t>(stream));
 }
 
 size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
   if (M <= k9::kRowsMax || N < 1 || K < 1) return 0;
-  const size_t x8 = (static_cast<size_t>(M) * K + 255) / 256 * 256;
-  const size_t xs = (static_cast<size_t>(M) * ((K + 127) / 128) * 4 + 255) / 256 * 256;
-  return x8 + xs;
+  return k9_scale_bytes(M, K) + static_cast<size_t>(M) * K;
 }
 
 int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_scales, const void* w8, const float* w_scales,
@@ -326,20 +356,23 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
   if (ldx < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of x overlap: ldx < K");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M <= k9::kRowsMax) return launch_k9_rows(x, x_dtype, ldx, x_scales, w8, w_scales, bias, out, out_dtype, ldo, M, N, K, s);
+  if (!workspace || workspace_bytes < tmu_linear_fp8_workspace_bytes(M, N, K))
+    return fail(TMU_ERR_WORKSPACE_TOO_SMALL, "workspace too small");
+  if (!aligned16(workspace)) return fail(TMU_ERR_MISALIGNED, "workspace not 16-byte aligned");
+  float* xst = static_cast<float*>(workspace);
+  const int ld_xs = (M + 255) / 256 * 256;
   const uint8_t* x8 = static_cast<const uint8_t*>(x);
-  const float* xs = x_scales;
   if (x_dtype != TMU_E4M3) {
-    if (!workspace || workspace_bytes < tmu_linear_fp8_workspace_bytes(M, N, K))
-      return fail(TMU_ERR_WORKSPACE_TOO_SMALL, "workspace too small");
-    if (!aligned16(workspace)) return fail(TMU_ERR_MISALIGNED, "workspace not 16-byte aligned");
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
-    float* sc = reinterpret_cast<float*>(ws + (static_cast<size_t>(M) * K + 255) / 256 * 256);
-    int st = quantize_rows(x, x_dtype, ldx, M, K, ws, sc, true, s);
+    uint8_t* ws = static_cast<uint8_t*>(workspace) + k9_scale_bytes(M, K);
+    int st = quantize_rows(x, x_dtype, ldx, M, K, ws, xst, 1, ld_xs, true, s);
     if (st) return st;
     x8 = ws;
-    xs = sc;
+  } else {
+    k9::ScaleParams sp{x_scales, xst, M, (K + 127) / 128, ld_xs};
+    cudaError_t e = launch_pdl(&k9::transpose_scales_kernel, (M + 255) / 256, 256, 0, s, sp);
+    if (e != cudaSuccess) return cuda_fail(e, "launch transpose_scales_kernel");
   }
-  return launch_k9(x8, xs, w8, w_scales, bias, out, out_dtype, ldo, M, N, K, static_cast<DeviceStatus*>(status), s);
+  return launch_k9(x8, xst, ld_xs, w8, w_scales, bias, out, out_dtype, ldo, M, N, K, static_cast<DeviceStatus*>(status), s);
 }
 
 }  // extern "C"

@@ -157,7 +157,7 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
         if any(t is not None and spans_overlap(out, t) for t in (x, weight.w8, weight.scales, bias, xs)):
             raise ValueError("out must not overlap an input")
     orow = _rows("out", out)
-    need = int(_lib.load().tmu_linear_fp8_workspace_bytes(m, n, k)) if xs is None else 0
+    need = int(_lib.load().tmu_linear_fp8_workspace_bytes(m, n, k))
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
     launch(x.device, "tmu_linear_fp8", rows.data_ptr(), _IN[x.dtype], _ld(rows), pointer(xs), weight.w8.data_ptr(),
            weight.scales.data_ptr(), pointer(bias), orow.data_ptr(), _OUT[out.dtype], _ld(orow), m, n, k, pointer(ws), need,

@@ -404,7 +404,7 @@ int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void
 
 /* K9: out [M, N] = x w^T + bias with 8-bit operands: w8 e4m3 [N, K] with fp32 w_scales
  * [ceil(N / 128), ceil(K / 128)], x fp16 or bf16 [M, K] (quantised as by tmu_quantize_rows into the
- * workspace; x_scales NULL) or e4m3 with its x_scales (contiguous, no workspace needed for it),
+ * workspace; x_scales NULL) or e4m3 with its x_scales (both contiguous),
  * bias fp32 [N] or NULL, out fp16, bf16 or fp32, rows ldo elements apart.  Sums are fp32.
  * Workspace: tmu_linear_fp8_workspace_bytes, 16-byte aligned; it holds nothing between calls.
  * status may be NULL. */

@@ -400,7 +400,8 @@ def linear_ref(x8, xs, w, bias, dtype):
 LINEAR_SIZES = [(1, 8, 16), (1, 128, 128), (1, 1000, 1360), (2, 77, 256), (3, 384, 2560), (7, 130, 400), (8, 256, 1024),
                 (9, 100, 512), (16, 500, 640), (17, 129, 144), (33, 1, 256), (64, 512, 2048), (100, 1000, 1008),
                 (127, 255, 384), (128, 256, 128), (129, 257, 1280), (238, 640, 5120), (300, 333, 208),
-                (513, 1025, 896), (1000, 72, 80), (700, 2560, 640)]
+                (513, 1025, 896), (1000, 72, 80), (700, 2560, 640),
+                (2500, 4100, 272), (257, 19000, 144), (38000, 130, 400), (3300, 3000, 4240)]
 
 
 @pytest.mark.parametrize("dtype", [FP16, BF16])
