@@ -311,11 +311,9 @@ __global__ void __launch_bounds__(kRowsThreads, PAIRS == 1 ? 4 : PAIRS == 4 ? 3 
 //   warp 8      TMA: x8 and w8 through a ring of kStages steps
 //   warp 9      TMEM and the MMAs (four of K = 32 a step)
 // Two blocks an SM, so one's start and end and its waits fall into the other's work.
-// The scales of a step's rows come with its operands, through a ring of their own: a step's are read
-// before its TMEM slot is handed back, and the MMAs are at most two steps ahead of that and the
-// loads kStages steps ahead of the MMAs, so kStages + 2 buffers are never overrun.  (Read from
-// global memory by each thread, a sector a row, they cost as much L2 traffic as half the operands: the pair
-// kernel took 690 us at 16384 x 2560 x 10240 with an L1 that holds them and 1118 without.)
+// The scales of a step's rows are read transposed, 32 rows in one access of a warp, two steps
+// ahead.  (Read as they lie, a sector a row, they cost as much L2 traffic as half the operands:
+// the pair kernel took 690 us at 16384 x 2560 x 10240 with an L1 that holds them and 1118 without.)
 // Few tiles: a cluster of blocks shares one tile along K.  Each leaves its sums in shared memory
 // and adds its share of the columns over the cluster's blocks, in rank order.
 // ------------------------------------------------------------------------------------------
@@ -326,8 +324,7 @@ constexpr int kThreads = 320;
 constexpr int kOperand = kTile * 128;
 constexpr int OFF_A = 0;
 constexpr int OFF_B = kStages * kOperand;
-constexpr int OFF_XS = 2 * kStages * kOperand;  // kStages + 2 buffers of 128 scales
-constexpr int OFF_BAR = OFF_XS + (kStages + 2) * 512;
+constexpr int OFF_BAR = 2 * kStages * kOperand;
 constexpr int SMEM_BYTES = OFF_BAR + 256;
 constexpr int kOutPitch = 80, kOutBytes = 32 * kOutPitch;  // a warp's staged rows of the output
 constexpr int kSumPitch = kTile + 4;  // floats of a row of sums in shared memory (over the ring)
@@ -347,7 +344,7 @@ struct Params {
   unsigned long long timeout_ns;
 };
 
-enum Site : unsigned int { kSiteProd = 0x901, kSiteMma = 0x902, kSiteSlot = 0x903, kSiteSum = 0x904, kSiteScale = 0x905, kSiteLayout = 0x9ff };
+enum Site : unsigned int { kSiteProd = 0x901, kSiteMma = 0x902, kSiteSlot = 0x903, kSiteSum = 0x904, kSiteLayout = 0x9ff };
 
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -356,14 +353,6 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-// 128 scales into shared memory, counted on `bar`.
-__device__ __forceinline__ void load_scales(void* dst, const float* src, uint64_t* bar) {
-  mbar_arrive_expect_tx(bar, 512);
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 512, [%2];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(smem_u32(bar))
-               : "memory");
 }
 
 // Instruction descriptor of kind::f8f6f4 with e4m3 operands (format 0), K-major, fp32 sums.
@@ -439,8 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
   uint64_t* empty = bars + kStages;           // [kStages]
   uint64_t* sfull = bars + 2 * kStages;       // [kSlots] a step's products are in the slot
   uint64_t* sempty = sfull + kSlots;          // [kSlots] its eight readers have them
-  uint64_t* xfull = sempty + kSlots;          // [kStages + 2] a step's scales are in shared memory
-  uint64_t& drain_bar = xfull[kStages + 2];
+  uint64_t& drain_bar = sempty[kSlots];
   uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
   volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
   const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
@@ -459,7 +447,6 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
       mbar_init(&sfull[s], 1);
       mbar_init(&sempty[s], 8);
     }
-    for (int s = 0; s < kStages + 2; ++s) mbar_init(&xfull[s], 1);
     mbar_init(&drain_bar, 1);
     fence_mbar_init();
     tma_prefetch_desc(&p.tm_x);
@@ -483,8 +470,6 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
       for (int b = b0; b < b1; ++b, ++i) {
         const int s = i % kStages;
         if (!mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, ctx, kSiteProd)) break;
-        const int x = i % (kStages + 2);
-        load_scales(smem + OFF_XS + x * 512, p.xst + static_cast<long long>(b) * p.ld_xs + m0, &xfull[x]);
         mbar_arrive_expect_tx(&full[s], 2 * kOperand);
         tma_load_2d(smem + OFF_A + s * kOperand, &p.tm_x, &full[s], b * 128, m0);
         tma_load_2d(smem + OFF_B + s * kOperand, &p.tm_w, &full[s], b * 128, n0);
@@ -493,11 +478,6 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
         for (int s = 0; s < kStages; ++s) {
           const int armed = i > s ? (i - s + kStages - 1) / kStages : 0;
           if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
-        }
-      if (abort_sh)
-        for (int x = 0; x < kStages + 2; ++x) {
-          const int armed = i > x ? (i - x + kStages + 1) / (kStages + 2) : 0;
-          if (armed) mbar_drain(&xfull[x], (armed - 1) & 1, 200000000ull);
         }
     }
   } else if (warp == 9) {
@@ -523,21 +503,26 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
     const int q = warp & 3, half = warp >> 2;
     const uint32_t tl = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * 64;
     const float* ws = p.ws + static_cast<long long>(n0 >> 7) * p.kb;
+    const float* xs = p.xst + m0 + q * 32 + lane;
 #pragma unroll
     for (int e = 0; e < 64; ++e) sum[e] = 0.f;
     // the weight's scales: lane j holds that of step 32 i + j, and of the next 32 steps
     auto load_ws = [&](int b) { return b + lane < b1 ? __ldg(ws + b + lane) : 0.f; };
     float w0 = load_ws(b0), w1 = load_ws(b0 + 32);
+    auto load_xs = [&](int b) { return b < b1 ? __ldg(xs + static_cast<long long>(b) * p.ld_xs) : 0.f; };
+    float x0 = load_xs(b0), x1 = load_xs(b0 + 1);
     for (int b = b0; b < b1; ++b) {
       const int i = b - b0, c = i % kSlots;
       if (i > 0 && (i & 31) == 0) {
         w0 = w1;
         w1 = load_ws(b + 32);
       }
-      const int x = i % (kStages + 2);
-      if (!warp_poll(&xfull[x], (i / (kStages + 2)) & 1, ctx, kSiteScale)) break;
-      const float sc = __shfl_sync(0xffffffffu, w0, i & 31) * reinterpret_cast<const float*>(smem + OFF_XS + x * 512)[q * 32 + lane];
-      if (!warp_poll(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum)) break;
+      const float x2 = load_xs(b + 2);
+      const float sc = __shfl_sync(0xffffffffu, w0, i & 31) * x0;
+      // one thread polls, the other warps park at the barrier: a warp's polls wait behind the MMAs'
+      // reads of shared memory.  After an abort every wait fails at once and the loop runs out.
+      if (threadIdx.x == 0) mbar_wait(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum);
+      named_bar_sync(1, 256);
       tc_fence_after();
       const float2 s2 = make_float2(sc, sc);
 #pragma unroll
@@ -556,6 +541,8 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
           a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
         }
       }
+      x0 = x1;
+      x1 = x2;
     }
   }
 
@@ -614,12 +601,13 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
 // operands of the tiles that run together stay in L2.
 //
 // A step's products are needed apart from the next step's, and TMEM holds two steps (512
-// columns), so the rate hangs on how soon a slot is free again: the step is made as two halves of
-// 128 columns with a slot each (the sums of one start while the other is made), and sixteen warps
-// take the products out, 64 columns each.
+// columns), so the rate hangs on how soon a slot is free again.  Sixteen warps take the products
+// out, 64 columns each, and touch no mbarrier on the way: an mbarrier operation waits behind the
+// MMAs' reads of shared memory (100 to 270 cycles each were seen), so one warp polls for the MMAs'
+// commits and one hands the slots back, and both meet the sixteen at named barriers.
 //   warp 0      TMA of this CTA's halves, counted on the even CTA's barrier (.cta_group::2)
-//   warp 1      TMEM and, in the even CTA, the MMAs (N = 128, four of K = 32 a half)
-//   warps 2-3   idle (they complete the warpgroup that gives its registers to the sums)
+//   warp 1      TMEM and, in the even CTA, the MMAs (M = N = 256, four of K = 32 a step)
+//   warp 2      waits for a step's products       warp 3   hands its slot back to the even CTA
 //   warps 4-19  sums: half h of the columns = warps 4 + 8 h .., two warps a TMEM lane quadrant
 // ------------------------------------------------------------------------------------------
 namespace pair {
@@ -628,16 +616,21 @@ constexpr int kStages = 5;
 constexpr int kThreads = 640;
 constexpr int kTileMN = 256;
 constexpr int kGroup = 8;
+constexpr int kSumThreads = 512;
+constexpr int kBarFull = 1, kBarRead = 3;  // named barriers of the two slots: products there, products read
 constexpr int kSumRegs = 104, kOtherRegs = 64;  // 512 * 104 + 128 * 64 = 640 * 96
 constexpr int OFF_A = 0;
 constexpr int OFF_B = kStages * kOperand;
-constexpr int OFF_XS = 2 * kStages * kOperand;  // kStages + 2 buffers of 128 scales
-constexpr int OFF_OUT = OFF_XS + (kStages + 2) * 512;  // staged rows of the output, a warp each
+constexpr int OFF_OUT = 2 * kStages * kOperand;  // staged rows of the output, a warp each
 constexpr int OFF_BAR = OFF_OUT + 16 * kOutBytes;
 constexpr int SMEM_BYTES = OFF_BAR + 256;
 static_assert(SMEM_BYTES <= 232448, "K9 pair shared memory");
 
-enum Site : unsigned int { kSiteProd = 0x911, kSiteMma = 0x912, kSiteSlot = 0x913, kSiteSum = 0x914, kSiteScale = 0x915, kSiteLayout = 0x91f };
+enum Site : unsigned int { kSiteProd = 0x911, kSiteMma = 0x912, kSiteSlot = 0x913, kSiteSum = 0x914, kSiteLayout = 0x91f };
+
+__device__ __forceinline__ void named_bar_arrive(uint32_t id, uint32_t nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
 
 __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                              uint32_t accumulate) {
@@ -687,9 +680,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
   uint64_t* full = bars;              // [kStages] even CTA: both CTAs' halves have landed
   uint64_t* empty = bars + kStages;   // [kStages] the paired MMAs have read the stage (both CTAs)
   uint64_t* sfull = bars + 2 * kStages;  // [2] a step's products are in the slot (both CTAs)
-  uint64_t* sempty = sfull + 2;          // [2] even CTA: the 32 reading warps of both CTAs have them
-  uint64_t* xfull = sempty + 2;          // [kStages + 2] a step's scales are in shared memory (each CTA's)
-  uint64_t& drain_bar = xfull[kStages + 2];
+  uint64_t* sempty = sfull + 2;          // [2] even CTA: both CTAs' readers have them
+  uint64_t& drain_bar = sempty[2];
   uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
   volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
   const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
@@ -705,9 +697,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sfull[s], 1);
-      mbar_init(&sempty[s], 32);
+      mbar_init(&sempty[s], 2);
     }
-    for (int s = 0; s < kStages + 2; ++s) mbar_init(&xfull[s], 1);
     mbar_init(&drain_bar, 1);
     fence_mbar_init();
     tma_prefetch_desc(&p.tm_x);
@@ -736,8 +727,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         for (int b = 0; b < p.kb; ++b, ++i) {
           const uint32_t s = i % kStages;
           if (!(ok = mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, ctx, kSiteProd))) break;
-          const uint32_t x = i % (kStages + 2);
-          load_scales(smem + OFF_XS + x * 512, p.xst + static_cast<long long>(b) * p.ld_xs + m0 + rank * kTile, &xfull[x]);
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
           const uint32_t bar = cluster_addr(&full[s], 0);
           tma_load_2d_pair(smem + OFF_A + s * kOperand, &p.tm_x, bar, b * 128, m0 + static_cast<int>(rank) * kTile);
@@ -748,11 +737,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         for (uint32_t s = 0; s < kStages; ++s) {
           const uint32_t armed = i > s ? (i - s + kStages - 1) / kStages : 0;
           if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
-        }
-      if (abort_sh)
-        for (uint32_t x = 0; x < kStages + 2; ++x) {
-          const uint32_t armed = i > x ? (i - x + kStages + 1) / (kStages + 2) : 0;
-          if (armed) mbar_drain(&xfull[x], (armed - 1) & 1, 200000000ull);
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
       const uint32_t idesc = idesc_e4m3_f32(kTileMN, kTileMN);
@@ -774,16 +758,32 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         }
       umma_commit_pair(&drain_bar, 0x1);
       mbar_drain(&drain_bar, 0, 200000000ull);
+    } else if (warp == 2) {
+      uint32_t i = 0;
+      for (int t = first; t < tiles; t += step)
+        for (int b = 0; b < p.kb; ++b, ++i) {
+          if (lane == 0) mbar_wait(&sfull[i & 1], (i >> 1) & 1, ctx, kSiteSum);
+          __syncwarp();
+          named_bar_arrive(kBarFull + (i & 1), kSumThreads + 32);
+        }
+    } else if (warp == 3) {
+      const uint32_t slots = cluster_addr(&sempty[0], 0);
+      uint32_t i = 0;
+      for (int t = first; t < tiles; t += step)
+        for (int b = 0; b < p.kb; ++b, ++i) {
+          named_bar_sync(kBarRead + (i & 1), kSumThreads + 32);
+          tc_fence_after();
+          tc_fence_before();
+          if (lane == 0) arrive_slot(slots + (i & 1) * sizeof(uint64_t));
+        }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
     const int q = warp & 3, half = (warp - 4) >> 3, col = half * kTile + ((warp >> 2) & 1 ? 0 : 64);
     const uint32_t tl = tmem + (static_cast<uint32_t>(q * 32) << 16) + col;
-    const uint32_t slots = cluster_addr(&sempty[0], 0);
     const int nb_last = (p.N + 127) / 128 - 1;
     uint32_t i = 0;
-    bool ok = true;
-    for (int t = first; ok && t < tiles; t += step) {
+    for (int t = first; t < tiles; t += step) {
       int m0, n0;
       decode(p, t, m0, n0);
       const float* ws = p.ws + static_cast<long long>(min((n0 >> 7) + half, nb_last)) * p.kb;
@@ -793,16 +793,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       // the weight's scales: lane j holds that of step 32 i + j, and of the next 32 steps
       auto load_ws = [&](int b) { return b + lane < p.kb ? __ldg(ws + b + lane) : 0.f; };
       float w0 = load_ws(0), w1 = load_ws(32);
+      const float* xs = p.xst + m0 + static_cast<int>(rank) * kTile + q * 32 + lane;
+      auto load_xs = [&](int b) { return b < p.kb ? __ldg(xs + static_cast<long long>(b) * p.ld_xs) : 0.f; };
+      float x0 = load_xs(0), x1 = load_xs(1);
       for (int b = 0; b < p.kb; ++b, ++i) {
         const uint32_t c = i & 1;
         if (b > 0 && (b & 31) == 0) {
           w0 = w1;
           w1 = load_ws(b + 32);
         }
-        const uint32_t x = i % (kStages + 2);
-        if (!(ok = warp_poll(&xfull[x], (i / (kStages + 2)) & 1, ctx, kSiteScale))) break;
-        const float sc = __shfl_sync(0xffffffffu, w0, b & 31) * reinterpret_cast<const float*>(smem + OFF_XS + x * 512)[q * 32 + lane];
-        if (!(ok = warp_poll(&sfull[c], (i >> 1) & 1, ctx, kSiteSum))) break;
+        const float x2 = load_xs(b + 2);
+        const float sc = __shfl_sync(0xffffffffu, w0, b & 31) * x0;
+        named_bar_sync(kBarFull + c, kSumThreads + 32);
         tc_fence_after();
         const float2 s2 = make_float2(sc, sc);
 #pragma unroll
@@ -812,11 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
           tmem_wait_ld(r);
           if (h == 1) {
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if (rank == 0) mbar_arrive(&sempty[c]);
-              else arrive_slot(slots + c * sizeof(uint64_t));
-            }
+            named_bar_arrive(kBarRead + c, kSumThreads + 32);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -824,8 +822,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
             a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
           }
         }
+        x0 = x1;
+        x1 = x2;
       }
-      if (ok) store_rows(p, smem + OFF_OUT + (warp - 4) * kOutBytes, m0 + static_cast<int>(rank) * kTile + q * 32, n0 + col, sum);
+      store_rows(p, smem + OFF_OUT + (warp - 4) * kOutBytes, m0 + static_cast<int>(rank) * kTile + q * 32, n0 + col, sum);
     }
   }
 
