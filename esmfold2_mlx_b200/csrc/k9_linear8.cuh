@@ -311,9 +311,10 @@ __global__ void __launch_bounds__(kRowsThreads, PAIRS == 1 ? 4 : PAIRS == 4 ? 3 
 //   warp 8      TMA: x8 and w8 through a ring of kStages steps
 //   warp 9      TMEM and the MMAs (four of K = 32 a step)
 // Two blocks an SM, so one's start and end and its waits fall into the other's work.
-// The scales of a step's rows are read transposed, 32 rows in one access of a warp, two steps
-// ahead.  (Read as they lie, a sector a row, they cost as much L2 traffic as half the operands:
-// the pair kernel took 690 us at 16384 x 2560 x 10240 with an L1 that holds them and 1118 without.)
+// The scales of a step's rows are read transposed, 32 rows in one access of a warp, and by
+// cp.async, four steps ahead: a lane later reads the value that it copied itself.  (Read as they lie,
+// a sector a row, they cost as much L2 traffic as half the operands; handed on from register to
+// register each step, the move waited for the load: 800 of a step's 1550 cycles.)
 // Few tiles: a cluster of blocks shares one tile along K.  Each leaves its sums in shared memory
 // and adds its share of the columns over the cluster's blocks, in rank order.
 // ------------------------------------------------------------------------------------------
@@ -324,7 +325,8 @@ constexpr int kThreads = 320;
 constexpr int kOperand = kTile * 128;
 constexpr int OFF_A = 0;
 constexpr int OFF_B = kStages * kOperand;
-constexpr int OFF_BAR = 2 * kStages * kOperand;
+constexpr int OFF_XS = 2 * kStages * kOperand;  // the warps' rings of scales
+constexpr int OFF_BAR = OFF_XS + 8 * 4 * 128;
 constexpr int SMEM_BYTES = OFF_BAR + 256;
 constexpr int kOutPitch = 80, kOutBytes = 32 * kOutPitch;  // a warp's staged rows of the output
 constexpr int kSumPitch = kTile + 4;  // floats of a row of sums in shared memory (over the ring)
@@ -354,6 +356,29 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+
+// The scales of a warp's 32 rows on their way to shared memory, kScaleAhead steps ahead.
+constexpr int kScaleAhead = 4;
+
+struct ScaleRing {
+  const float* xs;  // this lane's row, block 0
+  long long ld;
+  uint32_t slot;    // this lane's word of the warp's kScaleAhead x 32
+  int end;
+  __device__ __forceinline__ void fetch(int b, int i) const {  // the scale of block b, for step i
+    if (b < end)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(slot + (i % kScaleAhead) * 128),
+                   "l"(xs + static_cast<long long>(b) * ld)
+                   : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ float get(int i) const {  // of step i, fetched kScaleAhead steps ago
+    asm volatile("cp.async.wait_group %0;" ::"n"(kScaleAhead - 1) : "memory");
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(slot + (i % kScaleAhead) * 128) : "memory");
+    return v;
+  }
+};
 
 // Instruction descriptor of kind::f8f6f4 with e4m3 operands (format 0), K-major, fp32 sums.
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int M, int N) { return idesc_f16_f32(M, N, false, false); }
@@ -509,16 +534,16 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
     // the weight's scales: lane j holds that of step 32 i + j, and of the next 32 steps
     auto load_ws = [&](int b) { return b + lane < b1 ? __ldg(ws + b + lane) : 0.f; };
     float w0 = load_ws(b0), w1 = load_ws(b0 + 32);
-    auto load_xs = [&](int b) { return b < b1 ? __ldg(xs + static_cast<long long>(b) * p.ld_xs) : 0.f; };
-    float x0 = load_xs(b0), x1 = load_xs(b0 + 1);
+    const ScaleRing ring{xs, p.ld_xs, smem_u32(smem + OFF_XS + warp * (kScaleAhead * 128)) + lane * 4, b1};
+    for (int u = 0; u < kScaleAhead; ++u) ring.fetch(b0 + u, u);
     for (int b = b0; b < b1; ++b) {
       const int i = b - b0, c = i % kSlots;
       if (i > 0 && (i & 31) == 0) {
         w0 = w1;
         w1 = load_ws(b + 32);
       }
-      const float x2 = load_xs(b + 2);
-      const float sc = __shfl_sync(0xffffffffu, w0, i & 31) * x0;
+      const float sc = __shfl_sync(0xffffffffu, w0, i & 31) * ring.get(i);
+      ring.fetch(b + kScaleAhead, i);
       // one thread polls, the other warps park at the barrier: a warp's polls wait behind the MMAs'
       // reads of shared memory.  After an abort every wait fails at once and the loop runs out.
       if (threadIdx.x == 0) mbar_wait(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum);
@@ -526,23 +551,21 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
       tc_fence_after();
       const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
-        tmem_ld32(tl + c * kTile + h * 32, r);
-        tmem_wait_ld(r);
-        if (h == 1) {
+      for (int h = 0; h < 4; ++h) {
+        uint32_t r[16];
+        tmem_ld16(tl + c * kTile + h * 16, r);
+        tmem_wait_ld16(r);
+        if (h == 3) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sempty[c]);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
+        for (int e = 0; e < 8; ++e) {
+          float2& a = reinterpret_cast<float2*>(sum)[h * 8 + e];
           a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
         }
       }
-      x0 = x1;
-      x1 = x2;
     }
   }
 
@@ -622,11 +645,18 @@ constexpr int kSumRegs = 104, kOtherRegs = 64;  // 512 * 104 + 128 * 64 = 640 * 
 constexpr int OFF_A = 0;
 constexpr int OFF_B = kStages * kOperand;
 constexpr int OFF_OUT = 2 * kStages * kOperand;  // staged rows of the output, a warp each
-constexpr int OFF_BAR = OFF_OUT + 16 * kOutBytes;
+constexpr int OFF_XS = OFF_OUT + 16 * kOutBytes;  // the warps' rings of scales
+constexpr int OFF_BAR = OFF_XS + 16 * kScaleAhead * 128;
 constexpr int SMEM_BYTES = OFF_BAR + 256;
 static_assert(SMEM_BYTES <= 232448, "K9 pair shared memory");
 
 enum Site : unsigned int { kSiteProd = 0x911, kSiteMma = 0x912, kSiteSlot = 0x913, kSiteSum = 0x914, kSiteLayout = 0x91f };
+
+__device__ __forceinline__ bool elect_one() {  // one lane of the warp
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(on));
+  return on != 0;
+}
 
 __device__ __forceinline__ void named_bar_arrive(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
@@ -685,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
   uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
   volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
   const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
   const int tiles = p.tiles_m * ((p.N + kTileMN - 1) / kTileMN);
@@ -738,26 +768,41 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
           const uint32_t armed = i > s ? (i - s + kStages - 1) / kStages : 0;
           if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
+      // The whole warp walks the steps and one lane issues: what the MMAs take from uniform registers
+      // (descriptors, addresses) is then computed there, and not moved there value by value.
       const uint32_t idesc = idesc_e4m3_f32(kTileMN, kTileMN);
       const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
-      uint32_t i = 0;
+      const bool leader = elect_one();
+      uint32_t s = 0, ph = 0, i = 0;
       bool ok = true;
       for (int t = first; ok && t < tiles; t += step)
-        for (int b = 0; ok && b < p.kb; ++b, ++i) {
-          const uint32_t s = i % kStages, c = i & 1;
-          if (!(ok = mbar_wait(&full[s], (i / kStages) & 1, ctx, kSiteMma))) break;
-          if (!(ok = mbar_wait(&sempty[c], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot))) break;
+        for (int b = 0; b < p.kb; ++b, ++i) {
+          const uint32_t c = i & 1;
+          if (!(ok = warp_poll(&sempty[c], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot))) break;
+          if (!(ok = warp_poll(&full[s], ph, ctx, kSiteMma))) break;
           tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8_pair(tmem + c * 256, sdesc_add(ad, s * kOperand + k * 32), sdesc_add(bd, s * kOperand + k * 32), idesc,
-                         k > 0 ? 1u : 0u);
-          umma_commit_pair(&sfull[c], 0x3);
-          umma_commit_pair(&empty[s], 0x3);
+          const uint64_t as = sdesc_add(ad, s * kOperand), bs = sdesc_add(bd, s * kOperand);
+          const uint32_t d = tmem + c * 256;
+          if (leader) {
+            umma_f8_pair(d, as, bs, idesc, 0u);
+            umma_f8_pair(d, sdesc_add(as, 32), sdesc_add(bs, 32), idesc, 1u);
+            umma_f8_pair(d, sdesc_add(as, 64), sdesc_add(bs, 64), idesc, 1u);
+            umma_f8_pair(d, sdesc_add(as, 96), sdesc_add(bs, 96), idesc, 1u);
+            umma_commit_pair(&sfull[c], 0x3);
+            umma_commit_pair(&empty[s], 0x3);
+          }
+          __syncwarp();
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
         }
-      umma_commit_pair(&drain_bar, 0x1);
-      mbar_drain(&drain_bar, 0, 200000000ull);
+      if (leader) {
+        umma_commit_pair(&drain_bar, 0x1);
+        mbar_drain(&drain_bar, 0, 200000000ull);
+      }
+      __syncwarp();
     } else if (warp == 2) {
       uint32_t i = 0;
       for (int t = first; t < tiles; t += step)
@@ -794,36 +839,34 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       auto load_ws = [&](int b) { return b + lane < p.kb ? __ldg(ws + b + lane) : 0.f; };
       float w0 = load_ws(0), w1 = load_ws(32);
       const float* xs = p.xst + m0 + static_cast<int>(rank) * kTile + q * 32 + lane;
-      auto load_xs = [&](int b) { return b < p.kb ? __ldg(xs + static_cast<long long>(b) * p.ld_xs) : 0.f; };
-      float x0 = load_xs(0), x1 = load_xs(1);
+      const ScaleRing ring{xs, p.ld_xs, smem_u32(smem + OFF_XS + (warp - 4) * (kScaleAhead * 128)) + lane * 4, p.kb};
+      for (int u = 0; u < kScaleAhead; ++u) ring.fetch(u, u);
       for (int b = 0; b < p.kb; ++b, ++i) {
         const uint32_t c = i & 1;
         if (b > 0 && (b & 31) == 0) {
           w0 = w1;
           w1 = load_ws(b + 32);
         }
-        const float x2 = load_xs(b + 2);
-        const float sc = __shfl_sync(0xffffffffu, w0, b & 31) * x0;
+        const float sc = __shfl_sync(0xffffffffu, w0, b & 31) * ring.get(b);
+        ring.fetch(b + kScaleAhead, b);
         named_bar_sync(kBarFull + c, kSumThreads + 32);
         tc_fence_after();
         const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
-          tmem_ld32(tl + c * 256 + h * 32, r);
-          tmem_wait_ld(r);
-          if (h == 1) {
+        for (int h = 0; h < 4; ++h) {
+          uint32_t r[16];
+          tmem_ld16(tl + c * 256 + h * 16, r);
+          tmem_wait_ld16(r);
+          if (h == 3) {
             tc_fence_before();
             named_bar_arrive(kBarRead + c, kSumThreads + 32);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
+          for (int e = 0; e < 8; ++e) {
+            float2& a = reinterpret_cast<float2*>(sum)[h * 8 + e];
             a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
           }
         }
-        x0 = x1;
-        x1 = x2;
       }
       store_rows(p, smem + OFF_OUT + (warp - 4) * kOutBytes, m0 + static_cast<int>(rank) * kTile + q * 32, n0 + col, sum);
     }
