@@ -748,26 +748,36 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 0 && lane == 0) {
-      uint32_t i = 0;
+    if (warp == 0) {
+      const bool leader = elect_one();
+      const uint32_t bar0 = cluster_addr(&full[0], 0);
+      uint32_t s = 0, ph = 0, i = 0;
       bool ok = true;
       for (int t = first; ok && t < tiles; t += step) {
         int m0, n0;
         decode(p, t, m0, n0);
+        m0 += static_cast<int>(rank) * kTile;
+        n0 += static_cast<int>(rank) * kTile;
         for (int b = 0; b < p.kb; ++b, ++i) {
-          const uint32_t s = i % kStages;
-          if (!(ok = mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, ctx, kSiteProd))) break;
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
-          const uint32_t bar = cluster_addr(&full[s], 0);
-          tma_load_2d_pair(smem + OFF_A + s * kOperand, &p.tm_x, bar, b * 128, m0 + static_cast<int>(rank) * kTile);
-          tma_load_2d_pair(smem + OFF_B + s * kOperand, &p.tm_w, bar, b * 128, n0 + static_cast<int>(rank) * kTile);
+          if (!(ok = warp_poll(&empty[s], ph ^ 1, ctx, kSiteProd))) break;
+          if (leader) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
+            tma_load_2d_pair(smem + OFF_A + s * kOperand, &p.tm_x, bar0 + s * sizeof(uint64_t), b * 128, m0);
+            tma_load_2d_pair(smem + OFF_B + s * kOperand, &p.tm_w, bar0 + s * sizeof(uint64_t), b * 128, n0);
+          }
+          __syncwarp();
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
         }
       }
-      if (abort_sh && rank == 0)
-        for (uint32_t s = 0; s < kStages; ++s) {
-          const uint32_t armed = i > s ? (i - s + kStages - 1) / kStages : 0;
-          if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
+      if (!ok && rank == 0 && leader)
+        for (uint32_t r = 0; r < kStages; ++r) {
+          const uint32_t armed = i > r ? (i - r + kStages - 1) / kStages : 0;
+          if (armed) mbar_drain(&full[r], (armed - 1) & 1, 200000000ull);
         }
+      __syncwarp();
     } else if (warp == 1 && rank == 0) {
       // The whole warp walks the steps and one lane issues: what the MMAs take from uniform registers
       // (descriptors, addresses) is then computed there, and not moved there value by value.
@@ -775,12 +785,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
       const bool leader = elect_one();
       uint32_t s = 0, ph = 0, i = 0;
-      bool ok = true;
-      for (int t = first; ok && t < tiles; t += step)
+      // (after an abort every wait fails at once, and the loop runs out on whatever is there)
+      for (int t = first; t < tiles; t += step)
         for (int b = 0; b < p.kb; ++b, ++i) {
           const uint32_t c = i & 1;
-          if (!(ok = warp_poll(&sempty[c], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot))) break;
-          if (!(ok = warp_poll(&full[s], ph, ctx, kSiteMma))) break;
+          warp_poll(&full[s], ph, ctx, kSiteMma);
+          warp_poll(&sempty[c], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot);
           tc_fence_after();
           const uint64_t as = sdesc_add(ad, s * kOperand), bs = sdesc_add(bd, s * kOperand);
           const uint32_t d = tmem + c * 256;
@@ -807,8 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       uint32_t i = 0;
       for (int t = first; t < tiles; t += step)
         for (int b = 0; b < p.kb; ++b, ++i) {
-          if (lane == 0) mbar_wait(&sfull[i & 1], (i >> 1) & 1, ctx, kSiteSum);
-          __syncwarp();
+          warp_poll(&sfull[i & 1], (i >> 1) & 1, ctx, kSiteSum);
           named_bar_arrive(kBarFull + (i & 1), kSumThreads + 32);
         }
     } else if (warp == 3) {
@@ -819,7 +828,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
           named_bar_sync(kBarRead + (i & 1), kSumThreads + 32);
           tc_fence_after();
           tc_fence_before();
-          if (lane == 0) arrive_slot(slots + (i & 1) * sizeof(uint64_t));
+          if (lane == 0) {
+            if (rank == 0) mbar_arrive(&sempty[i & 1]);
+            else arrive_slot(slots + (i & 1) * sizeof(uint64_t));
+          }
         }
     }
   } else {
@@ -853,18 +865,21 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         tc_fence_after();
         const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          uint32_t r[16];
-          tmem_ld16(tl + c * 256 + h * 16, r);
-          tmem_wait_ld16(r);
-          if (h == 3) {
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[16], r1[16];
+          tmem_ld16(tl + c * 256 + h * 32, r);
+          tmem_ld16(tl + c * 256 + h * 32 + 16, r1);
+          tmem_wait_ld16x2(r, r1);
+          if (h == 1) {
             tc_fence_before();
             named_bar_arrive(kBarRead + c, kSumThreads + 32);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            float2& a = reinterpret_cast<float2*>(sum)[h * 8 + e];
+            float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
             a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
+            float2& a1 = reinterpret_cast<float2*>(sum)[h * 16 + 8 + e];
+            a1 = __ffma2_rn(make_float2(__uint_as_float(r1[2 * e]), __uint_as_float(r1[2 * e + 1])), s2, a1);
           }
         }
       }
