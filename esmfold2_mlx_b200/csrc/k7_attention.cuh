@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     if (threadIdx.x == 0) record_status(status, kStatusLayout, kSiteLayout);
     return;
   }
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   griddep_wait();
 
@@ -198,34 +198,38 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ------------------------------ loads ------------------------------
-      if (lane == 0) {
-        const int kv = head / p.group;
-        auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int h) {
+      const bool leader = elect_one();
+      const int kv = head / p.group;
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int h) {
+        if (leader) {
           mbar_arrive_expect_tx(bar, C::kTileBytes);
+#pragma unroll
           for (int a = 0; a < C::kAtoms; ++a) tma_load_3d(dst + a * kAtom, map, bar, a * 64, row, h);
-        };
-        int j = 0;
-        load(smem + C::OFF_Q, &p.tm_q, &qfull[0], beg + q0, head);
-        for (; j < n; ++j) {
-          const int s = j % NS, ph = (j / NS) & 1;
-          if (!mbar_wait(&kempty[s], ph ^ 1, ctx, kSiteProdK)) break;
-          load(smem + C::OFF_K + s * C::kTileBytes, &p.tm_k, &kfull[s], beg + j * kTile, kv);
-          if (j == 0 && n1 > 0) load(smem + C::OFF_Q + C::kTileBytes, &p.tm_q, &qfull[1], beg + q0 + kTile, head);
-          if (!mbar_wait(&vempty[s], ph ^ 1, ctx, kSiteProdV)) {
-            mbar_drain(&kfull[s], ph, 200000000ull);
-            break;
-          }
-          load(smem + C::OFF_V + s * C::kTileBytes, &p.tm_v, &vfull[s], beg + j * kTile, kv);
+        }
+        __syncwarp();
+      };
+      int j = 0;
+      bool ok = true;
+      load(smem + C::OFF_Q, &p.tm_q, &qfull[0], beg + q0, head);
+      for (; j < n; ++j) {
+        const int s = j % NS, ph = (j / NS) & 1;
+        if (!(ok = warp_poll(&kempty[s], ph ^ 1, ctx, kSiteProdK))) break;
+        load(smem + C::OFF_K + s * C::kTileBytes, &p.tm_k, &kfull[s], beg + j * kTile, kv);
+        if (j == 0 && n1 > 0) load(smem + C::OFF_Q + C::kTileBytes, &p.tm_q, &qfull[1], beg + q0 + kTile, head);
+        if (!(ok = warp_poll(&vempty[s], ph ^ 1, ctx, kSiteProdV))) {
+          if (leader) mbar_drain(&kfull[s], ph, 200000000ull);
+          break;
+        }
+        load(smem + C::OFF_V + s * C::kTileBytes, &p.tm_v, &vfull[s], beg + j * kTile, kv);
       }
-        if (abort_sh) {
-          mbar_drain(&qfull[0], 0, 200000000ull);
-          if (n1 > 0 && j > 0) mbar_drain(&qfull[1], 0, 200000000ull);
-          for (int s = 0; s < NS; ++s) {
-            const int armed = j > s ? (j - s + NS - 1) / NS : 0;
-            if (armed) {
-              mbar_drain(&kfull[s], (armed - 1) & 1, 200000000ull);
-              mbar_drain(&vfull[s], (armed - 1) & 1, 200000000ull);
-            }
+      if (!ok && leader) {
+        mbar_drain(&qfull[0], 0, 200000000ull);
+        if (n1 > 0 && j > 0) mbar_drain(&qfull[1], 0, 200000000ull);
+        for (int s = 0; s < NS; ++s) {
+          const int armed = j > s ? (j - s + NS - 1) / NS : 0;
+          if (armed) {
+            mbar_drain(&kfull[s], (armed - 1) & 1, 200000000ull);
+            mbar_drain(&vfull[s], (armed - 1) & 1, 200000000ull);
           }
         }
       }
@@ -242,52 +246,67 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(&vfixed);
       }
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
       // ------------------------------ MMAs ------------------------------
-      constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+      constexpr bool kBf16 = !__is_same(T, __half);
+      const bool leader = elect_one();
       const int ksteps = (p.d + 15) / 16;
       const uint32_t id_s = kBf16 ? idesc_bf16_f32(128, 128, false, false) : idesc_f16_f32(128, 128, false, false);
       const uint32_t id_o = kBf16 ? idesc_bf16_f32(128, ksteps * 16, false, true) : idesc_f16_f32(128, ksteps * 16, false, true);
       const uint64_t qd = sdesc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
       const uint64_t kd = sdesc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
       const uint64_t vd = sdesc_sw128(smem_u32(smem + C::OFF_V), kAtom, 1024);
-      const int nx[2] = {n0, n1};
       auto issue_s = [&](int x, int j) {  // S_x(j) = Q_x K_j^T
         const int s = j % NS;
-        if (j == 0 && !mbar_wait(&qfull[x], 0, ctx, kSiteMmaQ)) return false;
-        if (!mbar_wait(&kfull[s], (j / NS) & 1, ctx, kSiteMmaK)) return false;
+        if (j == 0 && !warp_poll(&qfull[x], 0, ctx, kSiteMmaQ)) return false;
+        if (!warp_poll(&kfull[s], (j / NS) & 1, ctx, kSiteMmaK)) return false;
         tc_fence_after();
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * kAtom + (k & 3) * 32;
-          umma_f16(tmem + C::s_col(x), sdesc_add(qd, x * C::kTileBytes + off), sdesc_add(kd, s * C::kTileBytes + off), id_s,
-                   k > 0 ? 1u : 0u);
+        const uint64_t qs = sdesc_add(qd, x * C::kTileBytes), ks = sdesc_add(kd, s * C::kTileBytes);
+        const uint32_t d = tmem + C::s_col(x);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < ksteps)
+              umma_f16(d, sdesc_add(qs, (k >> 2) * kAtom + (k & 3) * 32), sdesc_add(ks, (k >> 2) * kAtom + (k & 3) * 32), id_s,
+                       k > 0 ? 1u : 0u);
+          umma_commit(&sfull[x]);
+          if (x == 1 || j >= n1) umma_commit(&kempty[s]);  // the last use of K_j
         }
-        umma_commit(&sfull[x]);
-        if (x == 1 || j >= n1) umma_commit(&kempty[s]);  // the last use of K_j
+        __syncwarp();
         return true;
+      };
+      // tile x's part of step j: S of the next step, and O += P V
+      auto tile_step = [&](int x, int j, int nx) {
+        const int s = j % NS;
+        if (C::kOwnP && j + 1 < nx)
+          if (!warp_poll(&sfree[x], j & 1, ctx, kSiteMmaS) || !issue_s(x, j + 1)) return false;
+        if (!warp_poll(&pfull[x], j & 1, ctx, kSiteMmaP)) return false;
+        tc_fence_after();
+        const uint64_t vs = sdesc_add(vd, s * C::kTileBytes);
+        const uint32_t d = tmem + C::o_col(x), a = tmem + C::p_col(x);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) umma_ts(d, a + k * 8, sdesc_add(vs, k * 2048), id_o, (j > 0 || k > 0) ? 1u : 0u);
+          umma_commit(&ofull[x]);
+        }
+        __syncwarp();
+        return C::kOwnP || j + 1 >= nx || issue_s(x, j + 1);
       };
       bool ok = issue_s(0, 0) && (n1 == 0 || issue_s(1, 0));
       for (int j = 0; ok && j < n; ++j) {
         const int s = j % NS;
-        if (!(ok = mbar_wait(&vfull[s], (j / NS) & 1, ctx, kSiteMmaV))) break;
-        if (fix && j == n - 1 && !(ok = mbar_wait(&vfixed, 0, ctx, kSiteMmaV))) break;
-        for (int x = 0; ok && x < 2; ++x) {
-          if (j >= nx[x]) continue;
-          if (C::kOwnP && j + 1 < nx[x]) {
-            if (!(ok = mbar_wait(&sfree[x], j & 1, ctx, kSiteMmaS) && issue_s(x, j + 1))) break;
-          }
-          if (!(ok = mbar_wait(&pfull[x], j & 1, ctx, kSiteMmaP))) break;
-          tc_fence_after();
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_ts(tmem + C::o_col(x), tmem + C::p_col(x) + k * 8, sdesc_add(vd, s * C::kTileBytes + k * 2048), id_o,
-                    (j > 0 || k > 0) ? 1u : 0u);
-          umma_commit(&ofull[x]);
-          if (!C::kOwnP && j + 1 < nx[x]) ok = issue_s(x, j + 1);
-        }
-        if (ok) umma_commit(&vempty[s]);
+        if (!(ok = warp_poll(&vfull[s], (j / NS) & 1, ctx, kSiteMmaV))) break;
+        if (fix && j == n - 1 && !(ok = warp_poll(&vfixed, 0, ctx, kSiteMmaV))) break;
+        if (j < n0 && !(ok = tile_step(0, j, n0))) break;
+        if (j < n1 && !(ok = tile_step(1, j, n1))) break;
+        if (leader) umma_commit(&vempty[s]);
+        __syncwarp();
       }
-      umma_commit(&drain_bar);
-      mbar_drain(&drain_bar, 0, 200000000ull);
+      if (leader) {
+        umma_commit(&drain_bar);
+        mbar_drain(&drain_bar, 0, 200000000ull);
+      }
+      __syncwarp();
     }
   } else {
     // ------------------------------ softmax ------------------------------

@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
   uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
   volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
   const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % p.split, tile = static_cast<int>(blockIdx.x) / p.split;
   const int m0 = tile % p.tiles_m * kTile, n0 = tile / p.tiles_m * kTile;
   const int b0 = static_cast<int>(static_cast<long long>(p.kb) * rank / p.split);
@@ -490,40 +490,59 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
 
   float sum[64];
   if (warp == 8) {
-    if (lane == 0) {
-      int i = 0;
-      for (int b = b0; b < b1; ++b, ++i) {
-        const int s = i % kStages;
-        if (!mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, ctx, kSiteProd)) break;
+    const bool leader = elect_one();
+    int s = 0, ph = 0, i = 0;
+    bool ok = true;
+    for (int b = b0; b < b1; ++b, ++i) {
+      if (!(ok = warp_poll(&empty[s], ph ^ 1, ctx, kSiteProd))) break;
+      if (leader) {
         mbar_arrive_expect_tx(&full[s], 2 * kOperand);
         tma_load_2d(smem + OFF_A + s * kOperand, &p.tm_x, &full[s], b * 128, m0);
         tma_load_2d(smem + OFF_B + s * kOperand, &p.tm_w, &full[s], b * 128, n0);
       }
-      if (abort_sh)
-        for (int s = 0; s < kStages; ++s) {
-          const int armed = i > s ? (i - s + kStages - 1) / kStages : 0;
-          if (armed) mbar_drain(&full[s], (armed - 1) & 1, 200000000ull);
-        }
-    }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_e4m3_f32(kTile, kTile);
-      const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
-      for (int i = 0; i < b1 - b0; ++i) {
-        const int s = i % kStages, c = i % kSlots;
-        if (!mbar_wait(&sempty[c], ((i / kSlots) & 1) ^ 1, ctx, kSiteSlot)) break;
-        if (!mbar_wait(&full[s], (i / kStages) & 1, ctx, kSiteMma)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f8(tmem + c * kTile, sdesc_add(ad, s * kOperand + k * 32), sdesc_add(bd, s * kOperand + k * 32), idesc,
-                  k > 0 ? 1u : 0u);
-        umma_commit(&empty[s]);
-        umma_commit(&sfull[c]);
+      __syncwarp();
+      if (++s == kStages) {
+        s = 0;
+        ph ^= 1;
       }
+    }
+    if (!ok && leader)
+      for (int r = 0; r < kStages; ++r) {
+        const int armed = i > r ? (i - r + kStages - 1) / kStages : 0;
+        if (armed) mbar_drain(&full[r], (armed - 1) & 1, 200000000ull);
+      }
+    __syncwarp();
+  } else if (warp == 9) {
+    const bool leader = elect_one();
+    const uint32_t idesc = idesc_e4m3_f32(kTile, kTile);
+    const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
+    int s = 0, ph = 0;
+    for (int i = 0; i < b1 - b0; ++i) {
+      const int c = i % kSlots;
+      if (!warp_poll(&full[s], ph, ctx, kSiteMma)) break;
+      if (!warp_poll(&sempty[c], ((i / kSlots) & 1) ^ 1, ctx, kSiteSlot)) break;
+      tc_fence_after();
+      const uint64_t as = sdesc_add(ad, s * kOperand), bs = sdesc_add(bd, s * kOperand);
+      const uint32_t d = tmem + c * kTile;
+      if (leader) {
+        umma_f8(d, as, bs, idesc, 0u);
+        umma_f8(d, sdesc_add(as, 32), sdesc_add(bs, 32), idesc, 1u);
+        umma_f8(d, sdesc_add(as, 64), sdesc_add(bs, 64), idesc, 1u);
+        umma_f8(d, sdesc_add(as, 96), sdesc_add(bs, 96), idesc, 1u);
+        umma_commit(&sfull[c]);
+        umma_commit(&empty[s]);
+      }
+      __syncwarp();
+      if (++s == kStages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    if (leader) {
       umma_commit(&drain_bar);
       mbar_drain(&drain_bar, 0, 200000000ull);
     }
+    __syncwarp();
   } else {
     const int q = warp & 3, half = warp >> 2;
     const uint32_t tl = tmem + (static_cast<uint32_t>(q * 32) << 16) + half * 64;
@@ -544,26 +563,26 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
       }
       const float sc = __shfl_sync(0xffffffffu, w0, i & 31) * ring.get(i);
       ring.fetch(b + kScaleAhead, i);
-      // one thread polls, the other warps park at the barrier: a warp's polls wait behind the MMAs'
-      // reads of shared memory.  After an abort every wait fails at once and the loop runs out.
-      if (threadIdx.x == 0) mbar_wait(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum);
-      named_bar_sync(1, 256);
+      if (!warp_poll(&sfull[c], (i / kSlots) & 1, ctx, kSiteSum)) break;
       tc_fence_after();
       const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t r[16];
-        tmem_ld16(tl + c * kTile + h * 16, r);
-        tmem_wait_ld16(r);
-        if (h == 3) {
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[16], r1[16];
+        tmem_ld16(tl + c * kTile + h * 32, r);
+        tmem_ld16(tl + c * kTile + h * 32 + 16, r1);
+        tmem_wait_ld16x2(r, r1);
+        if (h == 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sempty[c]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float2& a = reinterpret_cast<float2*>(sum)[h * 8 + e];
+          float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
           a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
+          float2& a1 = reinterpret_cast<float2*>(sum)[h * 16 + 8 + e];
+          a1 = __ffma2_rn(make_float2(__uint_as_float(r1[2 * e]), __uint_as_float(r1[2 * e + 1])), s2, a1);
         }
       }
     }
@@ -651,12 +670,6 @@ constexpr int SMEM_BYTES = OFF_BAR + 256;
 static_assert(SMEM_BYTES <= 232448, "K9 pair shared memory");
 
 enum Site : unsigned int { kSiteProd = 0x911, kSiteMma = 0x912, kSiteSlot = 0x913, kSiteSum = 0x914, kSiteLayout = 0x91f };
-
-__device__ __forceinline__ bool elect_one() {  // one lane of the warp
-  uint32_t on;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(on));
-  return on != 0;
-}
 
 __device__ __forceinline__ void named_bar_arrive(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
