@@ -49,30 +49,37 @@ struct Params {
   const int* cu;
   const void* bias;  // [S or 1, Hq, n, n] or null, the last axis contiguous
   long long bias_ss, bias_sh, bias_sr;
-  int bias_n;
+  int bias_n, bias_width;  // elements a copy of the bias may take: 8, 4 or 2, by its alignment
   int S, T, hq, group, d, causal;
   float scale_log2;  // scale * log2 e
   DeviceStatus* status;
   unsigned long long timeout_ns;
 };
 
-template <int DP>
+template <int DP, bool BIAS>
 struct Cfg {
   static constexpr int kAtoms = DP / 64;
   static constexpr int kTileBytes = kAtoms * kAtom;
-  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr int kStages = DP == 64 ? (BIAS ? 3 : 4) : 2;
   static constexpr bool kOwnP = DP == 64;  // P beside S instead of over it
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = 2 * kTileBytes;
   static constexpr int OFF_V = OFF_K + kStages * kTileBytes;
-  static constexpr int OFF_BAR = OFF_V + kStages * kTileBytes;
+  // bias of a warp's 32 rows: a step's 128 keys, or what fits beside the tiles; the rows' pitch makes
+  // the 16-byte accesses of eight rows meet 8 different bank groups
+  static constexpr int kBiasCols = DP == 64 ? 128 : 32;
+  static constexpr int kBiasPitch = kBiasCols * 2 + 16;
+  static constexpr int OFF_BIAS = OFF_V + kStages * kTileBytes;
+  static constexpr int OFF_BAR = OFF_BIAS + (BIAS ? 8 * 32 * kBiasPitch : 0);
   static constexpr int SMEM_BYTES = OFF_BAR + 512;
   // TMEM columns of tile x
   __device__ static constexpr uint32_t o_col(int x) { return x * DP; }
   __device__ static constexpr uint32_t s_col(int x) { return 2 * DP + x * 128; }
   __device__ static constexpr uint32_t p_col(int x) { return kOwnP ? 2 * DP + 256 + x * 64 : s_col(x); }
 };
-static_assert(Cfg<64>::SMEM_BYTES <= 232448 && Cfg<128>::SMEM_BYTES <= 232448, "K7 shared memory exceeds the limit");
+static_assert(Cfg<64, true>::SMEM_BYTES <= 232448 && Cfg<64, false>::SMEM_BYTES <= 232448 &&
+                  Cfg<128, true>::SMEM_BYTES <= 232448 && Cfg<128, false>::SMEM_BYTES <= 232448,
+              "K7 shared memory exceeds the limit");
 
 enum Site : unsigned int {
   kSiteProdK = 0x701, kSiteProdV = 0x702, kSiteMmaQ = 0x703, kSiteMmaK = 0x704, kSiteMmaV = 0x705, kSiteMmaS = 0x706,
@@ -120,7 +127,7 @@ __device__ __forceinline__ int find_sequence(const int* cu, int S, int T, int sl
 
 template <typename T, int DP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<DP>;
+  using C = Cfg<DP, BIAS>;
   constexpr int NS = C::kStages;
   extern __shared__ uint8_t smem[];
   DeviceStatus* const status = p.status != nullptr ? p.status : &g_own_status;
@@ -319,9 +326,39 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const bool flip = p.scale_log2 < 0.f;
     // a scale of 0 would turn a hidden key's -inf into a NaN
     const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);
-    const T* brow = nullptr;
-    if (BIAS && row < min(p.bias_n, len))
-      brow = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh + row * p.bias_sr;
+    // The bias of the warp's rows comes through shared memory, copied asynchronously a step ahead in
+    // whole rows: read by the row's thread from where it lies, 32 rows at a time, it cost
+    // 64 us at 4 x 384 tokens.  Copies take 16, 8 or 4 bytes, whatever the rows' alignment
+    // allows; a row that starts in the middle of a 4-byte word is shifted when it is read.  (An
+    // aligned word that holds a value of the bias lies inside its allocation.)
+    const int bn = min(p.bias_n, len);  // rows and keys that have a bias
+    uint8_t* bbuf = smem + C::OFF_BIAS + warp * (32 * C::kBiasPitch);
+    const T* bbase = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh;
+    auto odd = [&](int r) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(bbase + r * p.bias_sr) >> 1) & 1u; };
+    auto fetch_bias = [&](int k0) {
+      const int w = p.bias_width, lanes = min(32, C::kBiasCols / w), per = 32 / lanes;
+      const int c = (lane % lanes) * w, first = tile0 + (warp & 3) * 32;
+      for (int r = lane / lanes; r < 32; r += per) {
+        if (first + r >= bn) break;
+        const T* src = bbase + (first + r) * p.bias_sr + k0;
+        const int shift = w == 2 ? odd(first + r) : 0;
+        const uint32_t dst = smem_u32(bbuf + r * C::kBiasPitch);
+        if (w == 8) {
+          if (k0 + c < bn)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * 2), "l"(src + c) : "memory");
+        } else if (w == 4) {
+          if (k0 + c < bn)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + c * 2), "l"(src + c) : "memory");
+        } else {
+          for (int e = c; e < C::kBiasCols + shift; e += lanes * 2)
+            if (k0 + e - shift < bn)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + e * 2), "l"(src + e - shift) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const uint32_t bshift = BIAS && p.bias_width == 2 && row < bn ? odd(row) * 16u : 0u;
+    if (BIAS && nx > 0) fetch_bias(0);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nx; ++j) {
@@ -348,10 +385,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       float mul = c;
       if (BIAS) {  // x = s c + bias log2 e at once; without a bias the product is folded into the exponential
         mul = 1.f;
+        const int have = row < bn ? bn - k0 : 0;
 #pragma unroll
-        for (int e = 0; e < 128; ++e) {
-          const float b = brow != nullptr && k0 + e < min(p.bias_n, len) ? static_cast<float>(brow[k0 + e]) : 0.f;
-          v[e] = fmaf(v[e], c, b * kLog2e);
+        for (int b0 = 0; b0 < kTile; b0 += C::kBiasCols) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+          const uint4* src = reinterpret_cast<const uint4*>(bbuf + lane * C::kBiasPitch);
+          uint4 q = src[0];
+#pragma unroll
+          for (int g = 0; g < C::kBiasCols / 8; ++g) {
+            const uint4 next = src[g + 1];  // (the pitch has room for one more)
+            const uint32_t u[5] = {q.x, q.y, q.z, q.w, next.x};
+            q = next;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = k8::unpack2(__funnelshift_r(u[e], u[e + 1], bshift), T());
+              const int i = b0 + g * 8 + 2 * e;
+              v[i] = fmaf(v[i], c, i < have ? f.x * kLog2e : 0.f);
+              v[i + 1] = fmaf(v[i + 1], c, i + 1 < have ? f.y * kLog2e : 0.f);
+            }
+          }
+          __syncwarp();
+          if (b0 + C::kBiasCols < kTile || j + 1 < nx) fetch_bias(k0 + b0 + C::kBiasCols);
         }
       }
       if (k0 + kTile > len || (p.causal && k0 + kTile - 1 > tile0)) {

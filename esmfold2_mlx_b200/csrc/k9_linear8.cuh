@@ -567,22 +567,19 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
       tc_fence_after();
       const float2 s2 = make_float2(sc, sc);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t r[16], r1[16];
-        tmem_ld16(tl + c * kTile + h * 32, r);
-        tmem_ld16(tl + c * kTile + h * 32 + 16, r1);
-        tmem_wait_ld16x2(r, r1);
-        if (h == 1) {
+      for (int h = 0; h < 4; ++h) {
+        uint32_t r[16];
+        tmem_ld16(tl + c * kTile + h * 16, r);
+        tmem_wait_ld16(r);
+        if (h == 3) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&sempty[c]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float2& a = reinterpret_cast<float2*>(sum)[h * 16 + e];
+          float2& a = reinterpret_cast<float2*>(sum)[h * 8 + e];
           a = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), s2, a);
-          float2& a1 = reinterpret_cast<float2*>(sum)[h * 16 + 8 + e];
-          a1 = __ffma2_rn(make_float2(__uint_as_float(r1[2 * e]), __uint_as_float(r1[2 * e + 1])), s2, a1);
         }
       }
     }

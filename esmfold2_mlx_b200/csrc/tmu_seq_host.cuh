@@ -60,11 +60,12 @@ int launch_k7(const k7::Params& p, bool bf16, bool biased, int blocks, cudaStrea
   void (*kern)(k7::Params) =
       bf16 ? (biased ? k7::attention_kernel<__nv_bfloat16, DP, true> : k7::attention_kernel<__nv_bfloat16, DP, false>)
            : (biased ? k7::attention_kernel<__half, DP, true> : k7::attention_kernel<__half, DP, false>);
+  const int smem = biased ? k7::Cfg<DP, true>::SMEM_BYTES : k7::Cfg<DP, false>::SMEM_BYTES;
   Dev dev;
   const int bit = (DP == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (biased ? 1 : 0);
-  int st = seq_device(dev, bit, reinterpret_cast<const void*>(kern), k7::Cfg<DP>::SMEM_BYTES);
+  int st = seq_device(dev, bit, reinterpret_cast<const void*>(kern), smem);
   if (st) return st;
-  cudaError_t e = launch_pdl(kern, blocks, k7::kThreads, k7::Cfg<DP>::SMEM_BYTES, stream, p);
+  cudaError_t e = launch_pdl(kern, blocks, k7::kThreads, smem, stream, p);
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_kernel");
 }
 
@@ -315,6 +316,10 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
     p.bias_sh = bias->stride_head;
     p.bias_sr = bias->stride_row;
     p.bias_n = bias->n;
+    // the widest copy that every row allows: 16, 8 or (with a shift of odd rows) 4 bytes
+    const unsigned long long a = static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(bias->data)) |
+                                 2ull * bias->stride_seq | 2ull * bias->stride_head | 2ull * bias->stride_row;
+    p.bias_width = a % 16 == 0 ? 8 : a % 8 == 0 ? 4 : 2;
   }
   p.S = S;
   p.T = T;
