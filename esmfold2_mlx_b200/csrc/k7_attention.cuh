@@ -51,7 +51,7 @@ struct Params {
   long long bias_ss, bias_sh, bias_sr;
   int bias_n, bias_width;  // elements a copy of the bias may take: 8, 4 or 2, by its alignment
   int S, T, hq, group, d, causal;
-  float scale_log2;  // scale * log2 e
+  float scale;
   DeviceStatus* status;
   unsigned long long timeout_ns;
 };
@@ -107,6 +107,11 @@ __device__ __forceinline__ void tie(uint32_t (&r)[32]) {
                :
                : "memory");
 }
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
 
 __device__ __forceinline__ int clamp_token(int t, int T) { return min(max(t, 0), T); }
 
@@ -323,9 +328,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int tile0 = q0 + x * kTile;
     const int row = tile0 + (warp & 3) * 32 + lane;  // within the sequence
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const bool flip = p.scale_log2 < 0.f;
+    const bool flip = p.scale < 0.f;
     // a scale of 0 would turn a hidden key's -inf into a NaN
-    const float c = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const float c = fmaxf(fabsf(p.scale) * (BIAS ? 1.f : kLog2e), 1e-30f);
     // The bias of the warp's rows comes through shared memory, copied asynchronously a step ahead in
     // whole rows: read by the row's thread from where it lies, 32 rows at a time, it cost
     // 64 us at 4 x 384 tokens.  Copies take 16, 8 or 4 bytes, whatever the rows' alignment
@@ -334,30 +339,41 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int bn = min(p.bias_n, len);  // rows and keys that have a bias
     uint8_t* bbuf = smem + C::OFF_BIAS + warp * (32 * C::kBiasPitch);
     const T* bbase = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh;
-    auto odd = [&](int r) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(bbase + r * p.bias_sr) >> 1) & 1u; };
-    auto fetch_bias = [&](int k0) {
-      const int w = p.bias_width, lanes = min(32, C::kBiasCols / w), per = 32 / lanes;
-      const int c = (lane % lanes) * w, first = tile0 + (warp & 3) * 32;
-      for (int r = lane / lanes; r < 32; r += per) {
-        if (first + r >= bn) break;
-        const T* src = bbase + (first + r) * p.bias_sr + k0;
-        const int shift = w == 2 ? odd(first + r) : 0;
-        const uint32_t dst = smem_u32(bbuf + r * C::kBiasPitch);
-        if (w == 8) {
-          if (k0 + c < bn)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c * 2), "l"(src + c) : "memory");
-        } else if (w == 4) {
-          if (k0 + c < bn)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + c * 2), "l"(src + c) : "memory");
+    // copies of W values, kBiasCols / W lanes a row (W = 2: 32 lanes, and one value more in shifted rows)
+    auto copy_rows = [&](int k0, auto width) {
+      constexpr int W = decltype(width)::value, kLanes = C::kBiasCols / W < 32 ? C::kBiasCols / W : 32;
+      const int first = tile0 + (warp & 3) * 32, r0 = lane / kLanes, c = lane % kLanes * W;
+      const T* src = bbase + (first + r0) * p.bias_sr + k0 + c;
+      uint32_t dst = smem_u32(bbuf + r0 * C::kBiasPitch) + c * 2;
+      const int rows = bn - first, left = bn - k0 - c;  // values of this lane's columns that are there
+#pragma unroll 4
+      for (int r = r0; r < 32; r += 32 / kLanes) {
+        if (r >= rows) break;
+        if (W == 8) {
+          if (left > 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+        } else if (W == 4) {
+          if (left > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
         } else {
-          for (int e = c; e < C::kBiasCols + shift; e += lanes * 2)
-            if (k0 + e - shift < bn)
+          const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(src) >> 1) & 1;
+#pragma unroll
+          for (int e = 0; e <= C::kBiasCols; e += kLanes * 2)
+            if (c + e < C::kBiasCols + shift && left + shift > e)
               asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + e * 2), "l"(src + e - shift) : "memory");
         }
+        src += (32 / kLanes) * p.bias_sr;
+        dst += (32 / kLanes) * C::kBiasPitch;
       }
+    };
+    auto fetch_bias = [&](int k0) {
+      if (p.bias_width == 8) copy_rows(k0, Int<8>());
+      else if (p.bias_width == 4) copy_rows(k0, Int<4>());
+      else copy_rows(k0, Int<2>());
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const uint32_t bshift = BIAS && p.bias_width == 2 && row < bn ? odd(row) * 16u : 0u;
+    const uint32_t bshift =
+        BIAS && p.bias_width == 2 ? (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(bbase + row * p.bias_sr) >> 1) & 1u) * 16u : 0u;
+    const bool shifted = BIAS && __any_sync(0xffffffffu, bshift != 0u);
+    const float2 c2 = make_float2(flip ? -c : c, flip ? -c : c);
     if (BIAS && nx > 0) fetch_bias(0);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -377,37 +393,45 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         if (lane == 0) mbar_arrive(&sfree[x]);
       }
       float* v = reinterpret_cast<float*>(&r[0][0]);
-      if (flip) {
-#pragma unroll
-        for (int e = 0; e < 128; ++e) v[e] = -v[e];
-      }
       const int k0 = j * kTile;
       float mul = c;
-      if (BIAS) {  // x = s c + bias log2 e at once; without a bias the product is folded into the exponential
-        mul = 1.f;
+      if (BIAS) {
+        // x = s scale + bias, the exponential's factor is log2 e (without a bias the scale is folded into it)
+        mul = kLog2e;
         const int have = row < bn ? bn - k0 : 0;
+        const bool whole = __all_sync(0xffffffffu, have >= kTile);
 #pragma unroll
         for (int b0 = 0; b0 < kTile; b0 += C::kBiasCols) {
           asm volatile("cp.async.wait_all;" ::: "memory");
           __syncwarp();
           const uint4* src = reinterpret_cast<const uint4*>(bbuf + lane * C::kBiasPitch);
-          uint4 q = src[0];
+          auto add = [&](auto check) {
+            constexpr bool kCheck = decltype(check)::value != 0;  // rows that start in a word, or end in the tile
+            uint4 q = src[0];
 #pragma unroll
-          for (int g = 0; g < C::kBiasCols / 8; ++g) {
-            const uint4 next = src[g + 1];  // (the pitch has room for one more)
-            const uint32_t u[5] = {q.x, q.y, q.z, q.w, next.x};
-            q = next;
+            for (int g = 0; g < C::kBiasCols / 8; ++g) {
+              const uint4 next = kCheck || g + 1 < C::kBiasCols / 8 ? src[g + 1] : q;  // (the pitch has room for one more)
+              const uint32_t u[5] = {q.x, q.y, q.z, q.w, next.x};
+              q = next;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = k8::unpack2(__funnelshift_r(u[e], u[e + 1], bshift), T());
-              const int i = b0 + g * 8 + 2 * e;
-              v[i] = fmaf(v[i], c, i < have ? f.x * kLog2e : 0.f);
-              v[i + 1] = fmaf(v[i + 1], c, i + 1 < have ? f.y * kLog2e : 0.f);
+              for (int e = 0; e < 4; ++e) {
+                const int i = b0 + g * 8 + 2 * e;
+                float2 f = k8::unpack2(kCheck ? __funnelshift_r(u[e], u[e + 1], bshift) : u[e], T());
+                if (kCheck) f = make_float2(i < have ? f.x : 0.f, i + 1 < have ? f.y : 0.f);
+                const float2 x = __ffma2_rn(make_float2(v[i], v[i + 1]), c2, f);
+                v[i] = x.x;
+                v[i + 1] = x.y;
+              }
             }
-          }
+          };
+          if (whole && !shifted) add(Int<0>());
+          else add(Int<1>());
           __syncwarp();
           if (b0 + C::kBiasCols < kTile || j + 1 < nx) fetch_bias(k0 + b0 + C::kBiasCols);
         }
+      } else if (flip) {
+#pragma unroll
+        for (int e = 0; e < 128; ++e) v[e] = -v[e];
       }
       if (k0 + kTile > len || (p.causal && k0 + kTile - 1 > tile0)) {
         const int lim = (p.causal ? min(len, row + 1) : len) - k0;

@@ -327,7 +327,7 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
   p.group = Hq / Hkv;
   p.d = D;
   p.causal = causal != 0;
-  p.scale_log2 = scale * k7::kLog2e;
+  p.scale = scale;
   p.status = static_cast<DeviceStatus*>(status);
   p.timeout_ns = g_timeout_ns;
   const long long blocks = (static_cast<long long>(T) / k7::kRows + S) * Hq;
