@@ -11,13 +11,16 @@
 // and the result, O / l, does not depend on when it moved.
 //
 // A block takes 256 rows of one head and sequence as two tiles A and B of 128 rows; a step takes
-// 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the softmax of S's rows (one thread a row), P in
-// TMEM in the inputs' type, and O += P V with P as the MMA's A operand out of TMEM.  While one
-// tile's softmax runs, the tensor cores work for the other.
-//   warps 0-3   softmax of tile A (warp w: TMEM lanes 32 w ..)     warps 4-7   softmax of tile B
-//   warp 8      TMA: Q, then K and V through rings of kStages tiles
-//   warp 9      TMEM and the MMAs (one thread)
-//   warps 10-11 idle (they complete the warpgroup that gives its registers to the softmax)
+// 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the softmax of S's rows (two threads a row, 64 keys
+// each, that tell each other their maximum), P in TMEM in the inputs' type, and O += P V with P as the
+// MMA's A operand out of TMEM.  While one tile's softmax runs, the tensor cores work for the
+// other; what bounds a step is the way of one tile through both, S to P to O to S, so its longest
+// part, the exponentials, is spread over two threads a row.
+//   warps 0-7   softmax of tile A: half h of the keys = warps 4 h .., TMEM lanes 32 (warp % 4) ..
+//   warps 8-15  softmax of tile B
+//   warp 16     TMA: Q, then K and V through rings of kStages tiles
+//   warp 17     TMEM and the MMAs
+//   warps 18-19 idle (they complete the warpgroup that gives its registers to the softmax)
 // TMEM (512 columns): D <= 64: O 2 x 64, S 2 x 128, P 2 x 64: S has its own columns, so the next
 // S is made while the softmax works on this one.  D > 64: O 2 x 128, S 2 x 128, and P overwrites S;
 // the MMAs of a block execute in issue order, so S of step j + 1 follows the P V that reads them.
@@ -37,9 +40,9 @@ namespace k7 {
 
 constexpr int kRows = 256;     // query rows of a block
 constexpr int kTile = 128;     // query rows of a tile, keys of a step
-constexpr int kThreads = 384;
+constexpr int kThreads = 640, kSoftmaxWarps = 16;
 constexpr int kAtom = kTile * 128;  // 64 values of 128 rows
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 256 * 208 + 128 * 88 = 384 * 168
+constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;  // 512 * 104 + 128 * 64 = 640 * 96
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMoveMax = 8.f;
 
@@ -65,12 +68,13 @@ struct Cfg {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = 2 * kTileBytes;
   static constexpr int OFF_V = OFF_K + kStages * kTileBytes;
-  // bias of a warp's 32 rows: a step's 128 keys, or what fits beside the tiles; the rows' pitch makes
-  // the 16-byte accesses of eight rows meet 8 different bank groups
-  static constexpr int kBiasCols = DP == 64 ? 128 : 32;
+  // bias of a warp's 32 rows: its 64 keys of a step, or what fits beside the tiles; the rows' pitch
+  // makes the 16-byte accesses of eight rows meet 8 different bank groups
+  static constexpr int kBiasCols = DP == 64 ? 64 : 16;
   static constexpr int kBiasPitch = kBiasCols * 2 + 16;
   static constexpr int OFF_BIAS = OFF_V + kStages * kTileBytes;
-  static constexpr int OFF_BAR = OFF_BIAS + (BIAS ? 8 * 32 * kBiasPitch : 0);
+  static constexpr int OFF_ROW = OFF_BIAS + (BIAS ? kSoftmaxWarps * 32 * kBiasPitch : 0);  // a float a softmax thread
+  static constexpr int OFF_BAR = OFF_ROW + kSoftmaxWarps * 128;
   static constexpr int SMEM_BYTES = OFF_BAR + 512;
   // TMEM columns of tile x
   __device__ static constexpr uint32_t o_col(int x) { return x * DP; }
@@ -93,6 +97,15 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {  // as tmem_st32, 16 columns
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 
@@ -187,15 +200,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     for (int x = 0; x < 2; ++x) {
       mbar_init(&qfull[x], 1);
       mbar_init(&sfull[x], 1);
-      mbar_init(&sfree[x], 4);  // the tile's four warps
-      mbar_init(&pfull[x], 4);
+      mbar_init(&sfree[x], 8);  // the tile's eight warps
+      mbar_init(&pfull[x], 8);
       mbar_init(&ofull[x], 1);
     }
     mbar_init(&vfixed, 1);
     mbar_init(&drain_bar, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == kSoftmaxWarps + 1) {
     tmem_alloc(&tmem_base_sh, 512);
     tmem_relinquish();
   }
@@ -206,9 +219,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   griddep_trigger();
   const bool fix = n * kTile > len;  // the last step's keys end inside the tile
 
-  if (warp >= 8) {
+  if (warp >= kSoftmaxWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    if (warp == 8) {
+    if (warp == kSoftmaxWarps) {
       // ------------------------------ loads ------------------------------
       const bool leader = elect_one();
       const int kv = head / p.group;
@@ -258,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(&vfixed);
       }
-    } else if (warp == 9) {
+    } else if (warp == kSoftmaxWarps + 1) {
       // ------------------------------ MMAs ------------------------------
       constexpr bool kBf16 = !__is_same(T, __half);
       const bool leader = elect_one();
@@ -323,11 +336,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   } else {
     // ------------------------------ softmax ------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int x = warp >> 2;
+    constexpr int kKeys = kTile / 2;  // of a thread
+    const int x = warp >> 3, half = (warp >> 2) & 1;
     const int nx = x == 0 ? n0 : n1;
     const int tile0 = q0 + x * kTile;
     const int row = tile0 + (warp & 3) * 32 + lane;  // within the sequence
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // the row's other half: a float of shared memory each, and a barrier of the two warps
+    float* const mine_f = reinterpret_cast<float*>(smem + C::OFF_ROW) + warp * 32 + lane;
+    const float* const other_f = reinterpret_cast<const float*>(smem + C::OFF_ROW) + (warp ^ 4) * 32 + lane;
+    auto exchange = [&](float f) {
+      *mine_f = f;
+      named_bar_sync(1 + x * 4 + (warp & 3), 64);
+      return *other_f;
+    };
     const bool flip = p.scale < 0.f;
     // a scale of 0 would turn a hidden key's -inf into a NaN
     const float c = fmaxf(fabsf(p.scale) * (BIAS ? 1.f : kLog2e), 1e-30f);
@@ -374,34 +396,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         BIAS && p.bias_width == 2 ? (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(bbase + row * p.bias_sr) >> 1) & 1u) * 16u : 0u;
     const bool shifted = BIAS && __any_sync(0xffffffffu, bshift != 0u);
     const float2 c2 = make_float2(flip ? -c : c, flip ? -c : c);
-    if (BIAS && nx > 0) fetch_bias(0);
+    if (BIAS && nx > 0) fetch_bias(half * kKeys);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nx; ++j) {
       if (!(ok = warp_poll(&sfull[x], j & 1, ctx, kSiteSoftS))) break;
       tc_fence_after();
-      uint32_t r[4][32];
+      uint32_t r[2][32];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) tmem_ld32(tl + C::s_col(x) + b * 32, r[b]);
+      for (int b = 0; b < 2; ++b) tmem_ld32(tl + C::s_col(x) + half * kKeys + b * 32, r[b]);
       tmem_wait_ld(r[0]);
       tie(r[1]);
-      tie(r[2]);
-      tie(r[3]);
       if (C::kOwnP) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sfree[x]);
       }
       float* v = reinterpret_cast<float*>(&r[0][0]);
-      const int k0 = j * kTile;
+      const int k0 = j * kTile + half * kKeys;
       float mul = c;
       if (BIAS) {
         // x = s scale + bias, the exponential's factor is log2 e (without a bias the scale is folded into it)
         mul = kLog2e;
         const int have = row < bn ? bn - k0 : 0;
-        const bool whole = __all_sync(0xffffffffu, have >= kTile);
+        const bool whole = __all_sync(0xffffffffu, have >= kKeys);
 #pragma unroll
-        for (int b0 = 0; b0 < kTile; b0 += C::kBiasCols) {
+        for (int b0 = 0; b0 < kKeys; b0 += C::kBiasCols) {
           asm volatile("cp.async.wait_all;" ::: "memory");
           __syncwarp();
           const uint4* src = reinterpret_cast<const uint4*>(bbuf + lane * C::kBiasPitch);
@@ -427,21 +447,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           if (whole && !shifted) add(Int<0>());
           else add(Int<1>());
           __syncwarp();
-          if (b0 + C::kBiasCols < kTile || j + 1 < nx) fetch_bias(k0 + b0 + C::kBiasCols);
+          if (b0 + C::kBiasCols < kKeys) fetch_bias(k0 + b0 + C::kBiasCols);
+          else if (j + 1 < nx) fetch_bias(k0 + kTile);
         }
       } else if (flip) {
 #pragma unroll
-        for (int e = 0; e < 128; ++e) v[e] = -v[e];
+        for (int e = 0; e < kKeys; ++e) v[e] = -v[e];
       }
-      if (k0 + kTile > len || (p.causal && k0 + kTile - 1 > tile0)) {
+      if (k0 + kKeys > len || (p.causal && k0 + kKeys - 1 > tile0)) {
         const int lim = (p.causal ? min(len, row + 1) : len) - k0;
 #pragma unroll
-        for (int e = 0; e < 128; ++e) v[e] = e < lim ? v[e] : -INFINITY;
+        for (int e = 0; e < kKeys; ++e) v[e] = e < lim ? v[e] : -INFINITY;
       }
       float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-      for (int e = 4; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+      for (int e = 4; e < kKeys; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
+      const float part = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const float top = fmaxf(part, exchange(part)) * mul;
       if (j > 0 && C::kOwnP) {  // P's columns and O belong to P V of the last step (else S's being there says so)
         if (!(ok = warp_poll(&ofull[x], (j - 1) & 1, ctx, kSiteSoftO))) break;
         tc_fence_after();
@@ -453,30 +475,31 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const float f = move ? ex2_approx(m - top) : 1.f;
         if (move) m = top;
         l *= f;
+#pragma unroll 1
+        for (int b = 0; b < DP / 32; ++b) {  // a half of O's columns each
+          uint32_t o[16];
+          const uint32_t at = tl + C::o_col(x) + half * (DP / 2) + b * 16;
+          tmem_ld16(at, o);
+          tmem_wait_ld16(o);
 #pragma unroll
-        for (int b = 0; b < DP / 32; ++b) {
-          uint32_t o[32];
-          tmem_ld32(tl + C::o_col(x) + b * 32, o);
-          tmem_wait_ld(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(tl + C::o_col(x) + b * 32, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st16(at, o);
         }
       }
       const float neg = m == -INFINITY ? 0.f : -m;
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        uint32_t w[32];
+        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 t = __ffma2_rn(make_float2(v[b * 64 + 2 * e], v[b * 64 + 2 * e + 1]), make_float2(mul, mul),
+        for (int e = 0; e < 16; ++e) {
+          const float2 t = __ffma2_rn(make_float2(v[b * 32 + 2 * e], v[b * 32 + 2 * e + 1]), make_float2(mul, mul),
                                       make_float2(neg, neg));
           const float2 q = make_float2(ex2_approx(t.x), ex2_approx(t.y));
           sum = __fadd2_rn(sum, q);
           w[e] = k8::pack2(q.x, q.y, T());
         }
-        tmem_st32(tl + C::p_col(x) + b * 32, w);
+        tmem_st16(tl + C::p_col(x) + half * 32 + b * 16, w);
       }
       l += sum.x + sum.y;
       tmem_wait_st();
@@ -486,22 +509,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
     if (ok && nx > 0 && warp_poll(&ofull[x], (nx - 1) & 1, ctx, kSiteEpi)) {
       tc_fence_after();
+      l += exchange(l);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.o.p) + static_cast<long long>(beg + row) * p.o.st + head * p.o.sh;
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) {
+      for (int b = 0; b < DP / 64; ++b) {
+        const int c0 = half * (DP / 2) + b * 32;
         uint32_t o[32];
-        tmem_ld32(tl + C::o_col(x) + b * 32, o);
+        tmem_ld32(tl + C::o_col(x) + c0, o);
         tmem_wait_ld(o);
         if (row >= len) continue;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          if (b * 32 + g * 8 >= p.d) break;
+          if (c0 + g * 8 >= p.d) break;
           uint32_t u[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             u[e] = k8::pack2(__uint_as_float(o[g * 8 + 2 * e]) * inv, __uint_as_float(o[g * 8 + 2 * e + 1]) * inv, T());
-          *reinterpret_cast<uint4*>(out + b * 32 + g * 8) = make_uint4(u[0], u[1], u[2], u[3]);
+          *reinterpret_cast<uint4*>(out + c0 + g * 8) = make_uint4(u[0], u[1], u[2], u[3]);
         }
       }
     }
@@ -509,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kSoftmaxWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
