@@ -13,11 +13,13 @@
 // of positions has to be kept or bounded.  (An fp32 product pos * f_i is off by up to pos * 2^-24 rad.)
 //
 // Bound: HBM (each value is read once and written once, 4 bytes moved for about 20 operations).
-// Split: 16 bytes a lane and LPH = D / 8 lanes (rounded up to a power of two) a head, so a warp
-// reads 32 / LPH heads at a time and the sums over a head are shuffles inside its lanes; a lane's
-// eight values belong to the same pairs in every head, so the sines of a token are computed once
-// for all the heads that the warp visits.  The partner of a half-layout pair sits rot / 16 lanes
-// away: one shuffle a value.  Few tokens: the heads are split over more warps (the host's `slices`).
+// Split: D / 8 lanes (rounded up to a power of two, LPH) a head and 8 values a lane, as two runs of
+// four: in the half layout the runs of both members of four pairs, so no value leaves its lane for
+// its rotation; else eight in a row.  A warp takes 32 / LPH heads at a time and the sums over a
+// head are shuffles inside its lanes.  A lane's values belong to the same four pairs in every
+// head, so the sines of a token, and a tensor's weights, are made once for all the heads that the
+// warp visits.  The loads of kBatch turns are issued before the first is worked on.  Few tokens: the
+// heads are split over more warps (the host's `slices`).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -69,8 +71,12 @@ struct Params {
   const unsigned long long* turns;  // [rot / 2]
   const float *qw, *qb, *kw, *kb;   // [D] or null
   float gain, eps, inv_d;
-  int pos64, rot, T, hq, heads, d, slices, passes;  // a warp makes `passes` passes of 32 / LPH heads
+  int pos64, rot, T, hq, hk, d;
+  int q_turns, all_turns;  // turns of 32 / LPH heads that q, and q and k, take
+  int slices, turns_each;  // warps of a token, and the turns that each takes
 };
+
+constexpr int kBatch = 4;
 
 __device__ __forceinline__ float2 unpack2(uint32_t u, __half) { return unpack_half2(u); }
 __device__ __forceinline__ float2 unpack2(uint32_t u, __nv_bfloat16) {
@@ -93,106 +99,109 @@ template <typename T, int LPH, int NORM, bool INTER>
 __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant__ Params p) {
   constexpr int HPW = 32 / LPH;
   const int lane = threadIdx.x & 31;
-  const int c = lane & (LPH - 1);
+  const int c = lane & (LPH - 1), sub = lane / LPH;
   const long long item = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const long long t = item / p.slices;
   if (t >= p.T) return;  // a whole warp
-  const int slice = static_cast<int>(item - t * p.slices);
-  const bool act = c * 8 < p.d;
-  const int d0 = act ? c * 8 : 0;
+  const int first = static_cast<int>(item - t * p.slices) * p.turns_each, last = min(first + p.turns_each, p.all_turns);
+  const bool act = c * 8 < p.d, turned = c * 8 < p.rot;  // (rot <= d)
+  // the lane's two runs of four values
+  int d0 = c * 8, d1 = c * 8 + 4;
+  if (!INTER && turned) {
+    d0 = c * 4;
+    d1 = (p.rot >> 1) + c * 4;
+  }
   griddep_wait();
 
-  // cos, sin of this lane's values (cos = 1, sin = 0 past the rotated part)
-  constexpr int NA = INTER ? 4 : 8;
-  float cs[NA], sn[NA];
-  const bool turned = act && c * 8 < p.rot;
+  // cos, sin of the lane's four pairs
+  float cs[4], sn[4];
 #pragma unroll
-  for (int e = 0; e < NA; ++e) {
+  for (int e = 0; e < 4; ++e) {
     cs[e] = 1.f;
     sn[e] = 0.f;
   }
   if (turned) {
-    const unsigned long long pos = p.pos64 ? static_cast<unsigned long long>(static_cast<const long long*>(p.pos)[t])
-                                           : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(p.pos)[t]));
-    const int half = p.rot >> 1;
-    const int i0 = INTER ? c * 4 : (c * 8 < half ? c * 8 : c * 8 - half);
-    const bool second = !INTER && c * 8 >= half;
-#pragma unroll
-    for (int e = 0; e < NA; ++e) {
-      const long long turn = static_cast<long long>(pos * __ldg(p.turns + i0 + e));
-      sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 0x1p-31f, &sn[e], &cs[e]);
-      cs[e] *= p.gain;
-      sn[e] *= second || INTER ? p.gain : -p.gain;  // y1 cos - y2 sin, y2 cos + y1 sin
-    }
-  }
-  const int shift = p.rot >> 4;
-  const int src = turned && !INTER ? (c < shift ? lane + shift : lane - shift) : lane;
-
-  const int h_begin = slice * p.passes * HPW + lane / LPH;
-#pragma unroll 2
-  for (int k = 0; k < p.passes; ++k) {
-    const int h = h_begin + k * HPW;
-    const bool isq = h < p.hq;
-    const bool on = act && h < p.heads;
-    const int hh = isq ? h : h - p.hq;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (on) {
-      const View& in = isq ? p.q : p.k;
-      raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(in.p) + t * in.st + hh * in.sh + d0);
-    }
-    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-    float y[8];
+    const long long pos = p.pos64 ? static_cast<const long long*>(p.pos)[t] : static_cast<const int*>(p.pos)[t];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack2(u[e], T());
-      y[2 * e] = f.x;
-      y[2 * e + 1] = f.y;
-    }
-    if (NORM != kNone) {
-      if (NORM == kLayer) {
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += y[e];
-        const float mean = head_sum<LPH>(s) * p.inv_d;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = act ? y[e] - mean : 0.f;
-      }
-      float s2 = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s2 = fmaf(y[e], y[e], s2);
-      const float r = rsqrtf(fmaf(head_sum<LPH>(s2), p.inv_d, p.eps));
-      const float* w = isq ? p.qw : p.kw;
-      const float* b = isq ? p.qb : p.kb;
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const float4 ww = w ? __ldg(reinterpret_cast<const float4*>(w + d0) + v) : make_float4(1.f, 1.f, 1.f, 1.f);
-        const float4 bb = b ? __ldg(reinterpret_cast<const float4*>(b + d0) + v) : make_float4(0.f, 0.f, 0.f, 0.f);
-        y[4 * v] = fmaf(y[4 * v] * r, ww.x, bb.x);
-        y[4 * v + 1] = fmaf(y[4 * v + 1] * r, ww.y, bb.y);
-        y[4 * v + 2] = fmaf(y[4 * v + 2] * r, ww.z, bb.z);
-        y[4 * v + 3] = fmaf(y[4 * v + 3] * r, ww.w, bb.w);
-      }
-    }
-    float o[8];
-    if (INTER) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[2 * e] = turned ? y[2 * e] * cs[e] - y[2 * e + 1] * sn[e] : y[2 * e];
-        o[2 * e + 1] = turned ? y[2 * e + 1] * cs[e] + y[2 * e] * sn[e] : y[2 * e + 1];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_sync(0xffffffffu, y[e], src);
-        o[e] = turned ? fmaf(y[e], cs[e], other * sn[e]) : y[e];
-      }
-    }
-    if (on) {
-      const View& out = isq ? p.qo : p.ko;
-      *reinterpret_cast<uint4*>(static_cast<T*>(out.p) + t * out.st + hh * out.sh + d0) =
-          make_uint4(pack2(o[0], o[1], T()), pack2(o[2], o[3], T()), pack2(o[4], o[5], T()), pack2(o[6], o[7], T()));
+      const long long turn = static_cast<long long>(static_cast<unsigned long long>(pos) * __ldg(p.turns + c * 4 + e));
+      sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 0x1p-31f, &sn[e], &cs[e]);
+      cs[e] *= p.gain;
+      sn[e] *= p.gain;
     }
   }
+
+  // turns [begin, end) of one tensor
+  auto run = [&](const View& in, const View& out, int heads, int begin, int end, const float* w, const float* b) {
+    if (begin >= end) return;
+    float2 ww[4], bb[4];
+    if (NORM != kNone) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int at = (v < 2 ? d0 : d1) + (v & 1) * 2;
+        ww[v] = w != nullptr && act ? __ldg(reinterpret_cast<const float2*>(w + at)) : make_float2(1.f, 1.f);
+        bb[v] = b != nullptr && act ? __ldg(reinterpret_cast<const float2*>(b + at)) : make_float2(0.f, 0.f);
+      }
+    }
+    const T* src = static_cast<const T*>(in.p) + t * in.st;
+    T* dst = static_cast<T*>(out.p) + t * out.st;
+    for (int k0 = begin; k0 < end; k0 += kBatch) {
+      uint2 raw[kBatch][2];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = (k0 + i) * HPW + sub;
+        raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
+        if (act && k0 + i < end && h < heads) {
+          raw[i][0] = *reinterpret_cast<const uint2*>(src + h * in.sh + d0);
+          raw[i][1] = *reinterpret_cast<const uint2*>(src + h * in.sh + d1);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (k0 + i >= end) break;
+        const int h = (k0 + i) * HPW + sub;
+        float2 y[4] = {unpack2(raw[i][0].x, T()), unpack2(raw[i][0].y, T()), unpack2(raw[i][1].x, T()),
+                       unpack2(raw[i][1].y, T())};
+        if (NORM == kLayer) {
+          const float2 s = __fadd2_rn(__fadd2_rn(y[0], y[1]), __fadd2_rn(y[2], y[3]));
+          const float m = -head_sum<LPH>(s.x + s.y) * p.inv_d;
+          const float2 m2 = act ? make_float2(m, m) : make_float2(0.f, 0.f);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) y[v] = __fadd2_rn(y[v], m2);
+        }
+        if (NORM != kNone) {
+          float2 s2 = __fmul2_rn(y[0], y[0]);
+#pragma unroll
+          for (int v = 1; v < 4; ++v) s2 = __ffma2_rn(y[v], y[v], s2);
+          const float r = rsqrtf(fmaf(head_sum<LPH>(s2.x + s2.y), p.inv_d, p.eps));
+#pragma unroll
+          for (int v = 0; v < 4; ++v) y[v] = __ffma2_rn(__fmul2_rn(y[v], make_float2(r, r)), ww[v], bb[v]);
+        }
+        if (turned) {
+          if (INTER) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              y[v] = make_float2(y[v].x * cs[v] - y[v].y * sn[v], y[v].y * cs[v] + y[v].x * sn[v]);
+          } else {
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+              const float2 cc = make_float2(cs[2 * v], cs[2 * v + 1]), ss = make_float2(sn[2 * v], sn[2 * v + 1]);
+              const float2 a = y[v], o = y[v + 2];
+              y[v] = __ffma2_rn(a, cc, __fmul2_rn(o, make_float2(-ss.x, -ss.y)));
+              y[v + 2] = __ffma2_rn(o, cc, __fmul2_rn(a, ss));
+            }
+          }
+        }
+        if (act && h < heads) {
+          T* to = dst + h * out.sh;
+          *reinterpret_cast<uint2*>(to + d0) = make_uint2(pack2(y[0].x, y[0].y, T()), pack2(y[1].x, y[1].y, T()));
+          *reinterpret_cast<uint2*>(to + d1) = make_uint2(pack2(y[2].x, y[2].y, T()), pack2(y[3].x, y[3].y, T()));
+        }
+      }
+    }
+  };
+  run(p.q, p.qo, p.hq, first, min(last, p.q_turns), p.qw, p.qb);
+  run(p.k, p.ko, p.hk, max(first, p.q_turns) - p.q_turns, last - p.q_turns, p.kw, p.kb);
   griddep_trigger();
 }
 

@@ -258,14 +258,16 @@ int tmu_qk_norm_rope(const tmu_heads* q, const tmu_heads* k, const tmu_heads* q_
   p.inv_d = 1.0f / static_cast<float>(D);
   p.T = T;
   p.hq = Hq;
-  p.heads = Hq + Hkv;
+  p.hk = Hkv;
   p.d = D;
-  // passes of 32 / lph heads; split over more warps until the card has 16 warps an SM
-  const int passes = (p.heads * lph + 31) / 32;
+  // turns of 32 / lph heads; split over more warps until the card has 16 warps an SM
+  const int hpw = 32 / lph;
+  p.q_turns = (Hq + hpw - 1) / hpw;
+  p.all_turns = p.q_turns + (Hkv + hpw - 1) / hpw;
   const long long want = 16ll * dev.sms;
-  const long long slices = std::min<long long>(passes, std::max<long long>(1, (want + T - 1) / T));
-  p.passes = static_cast<int>((passes + slices - 1) / slices);
-  p.slices = (passes + p.passes - 1) / p.passes;
+  const long long slices = std::min<long long>(p.all_turns, std::max<long long>(1, (want + T - 1) / T));
+  p.turns_each = static_cast<int>((p.all_turns + slices - 1) / slices);
+  p.slices = (p.all_turns + p.turns_each - 1) / p.turns_each;
   const long long blocks = (static_cast<long long>(T) * p.slices + k8::kThreads / 32 - 1) / (k8::kThreads / 32);
   if (blocks > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "too many tokens");
   const bool inter = rot->interleaved != 0;
