@@ -329,8 +329,9 @@ constexpr int OFF_XS = 2 * kStages * kOperand;  // the warps' rings of scales
 constexpr int OFF_BAR = OFF_XS + 8 * 4 * 128;
 constexpr int SMEM_BYTES = OFF_BAR + 256;
 constexpr int kOutPitch = 80, kOutBytes = 32 * kOutPitch;  // a warp's staged rows of the output
+constexpr int kMaxSplit = 8;        // blocks of a cluster
 constexpr int kSumPitch = kTile + 4;  // floats of a row of sums in shared memory (over the ring)
-static_assert(2 * (SMEM_BYTES + 1024) <= 233472 && kTile * kSumPitch * 4 + 8 * kOutBytes <= OFF_BAR, "K9 shared memory");
+static_assert(2 * (SMEM_BYTES + 1024) <= 233472 && kTile * kSumPitch * 4 <= OFF_BAR && 8 * kOutBytes <= OFF_BAR, "K9 shared memory");
 
 struct Params {
   CUtensorMap tm_x, tm_w;  // [rows, K] bytes: box {128, 128}, 128B swizzle, zero past the ends
@@ -422,10 +423,10 @@ __device__ __forceinline__ void store_rows(const Params& p, uint8_t* buf, int m0
     if (p.vec && c0 + cols <= p.N) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
+        const int r = i * 8 + (lane >> 2), c = lane & 3;
         if (m0 + r < p.M)
-          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + ((m0 + r) * p.ldo + c0) * es + (lane & 3) * 16) =
-              *reinterpret_cast<const uint4*>(buf + r * kOutPitch + (lane & 3) * 16);
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + ((m0 + r) * p.ldo + c0) * es + c * 16) =
+              *reinterpret_cast<const uint4*>(buf + r * kOutPitch + c * 16);
       }
     } else {
       for (int i = lane; i < 32 * cols; i += 32) {
@@ -597,27 +598,45 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
         *reinterpret_cast<float4*>(sums + row * kSumPitch + c0 + 4 * e) = make_float4(sum[4 * e], sum[4 * e + 1], sum[4 * e + 2], sum[4 * e + 3]);
     }
     cluster_sync_all();
-    // pieces of 32 rows by 64 columns, dealt over the cluster's warps
-    for (int i = rank * 8 + warp; warp < 8 && i < 8; i += p.split * 8) {
-      const int row = (i & 3) * 32 + lane, c = (i >> 2) * 64;
+    // rows dealt over the cluster's warps, four columns a lane: a warp reads whole rows of the other
+    // blocks' sums (read 16 bytes a row, the exchange alone took 6 us)
+    const int n = n0 + lane * 4;
+    float bias[4];
 #pragma unroll
-      for (int e = 0; e < 64; ++e) sum[e] = 0.f;
-      for (int r = 0; r < p.split; ++r) {
-        const uint32_t src = cluster_addr(sums + row * kSumPitch + c, r);
+    for (int e = 0; e < 4; ++e) bias[e] = p.bias != nullptr && n + e < p.N ? __ldg(p.bias + n + e) : 0.f;
+    for (int row = rank * 8 + warp; warp < 8 && row < kTile && m0 + row < p.M; row += p.split * 8) {
+      float4 f[kMaxSplit];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float4 f;
+      for (int r = 0; r < kMaxSplit; ++r)
+        if (r < p.split)
           asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
-                       : "r"(src + e * 16)
-                       : "memory");
-          sum[4 * e] += f.x;
-          sum[4 * e + 1] += f.y;
-          sum[4 * e + 2] += f.z;
-          sum[4 * e + 3] += f.w;
+                       : "=f"(f[r].x), "=f"(f[r].y), "=f"(f[r].z), "=f"(f[r].w)
+                       : "r"(cluster_addr(sums + row * kSumPitch + lane * 4, r)));
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        if (r < p.split) {
+          v[0] += f[r].x;
+          v[1] += f[r].y;
+          v[2] += f[r].z;
+          v[3] += f[r].w;
         }
+      const long long at = (m0 + row) * p.ldo + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += bias[e];
+      if (p.vec && n + 4 <= p.N) {
+        if (p.out_type == kF32) {
+          *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+          const uint2 u = p.out_type == kF16 ? make_uint2(k8::pack2(v[0], v[1], __half()), k8::pack2(v[2], v[3], __half()))
+                                             : make_uint2(k8::pack2(v[0], v[1], __nv_bfloat16()), k8::pack2(v[2], v[3], __nv_bfloat16()));
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = u;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < p.N) store_out(p.out, p.out_type, at + e, v[e]);
       }
-      store_rows(p, smem + kTile * kSumPitch * 4 + warp * kOutBytes, m0 + (i & 3) * 32, n0 + c, sum);
     }
     __syncwarp();
     cluster_sync_all();  // nobody leaves while its sums are being read
