@@ -10,25 +10,26 @@
 // 8, so weights reach at most 2^8 (exact in fp32 sums, and a common factor of the 16-bit weights),
 // and the result, O / l, does not depend on when it moved.
 //
-// A block takes 256 rows of one head and sequence as two tiles A and B of 128 rows; a step takes
-// 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the softmax of S's rows (two threads a row, 64 keys
-// each, that tell each other their maximum), P in TMEM in the inputs' type, and O += P V with P as the
-// MMA's A operand out of TMEM.  While one tile's softmax runs, the tensor cores work for the
-// other; what bounds a step is the way of one tile through both, S to P to O to S, so its longest
-// part, the exponentials, is spread over two threads a row.
-//   warps 0-7   softmax of tile A: half h of the keys = warps 4 h .., TMEM lanes 32 (warp % 4) ..
-//   warps 8-15  softmax of tile B
-//   warp 16     TMA: Q, then K and V through rings of kStages tiles
-//   warp 17     TMEM and the MMAs
-//   warps 18-19 idle (they complete the warpgroup that gives its registers to the softmax)
-// TMEM (512 columns): D <= 64: O 2 x 64, S 2 x 128, P 2 x 64: S has its own columns, so the next
-// S is made while the softmax works on this one.  D > 64: O 2 x 128, S 2 x 128, and P overwrites S;
-// the MMAs of a block execute in issue order, so S of step j + 1 follows the P V that reads them.
+// A tile is 128 rows of one head; a step takes 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the
+// softmax of S's rows, P in TMEM in the inputs' type, and O += P V with P as the MMA's A operand out of
+// TMEM.  A tile's step is a chain, S to P to O to S, so an SM always has two tiles in hand, and the
+// tensor cores work for one while the softmax of the other runs:
+//   D <= 64  two blocks an SM, of one tile each: with sequences of a few hundred tokens, two tiles of one
+//            sequence would often be one, and with equal blocks the last round is half as long
+//   D > 64   one block an SM, of two tiles A and B of one sequence that share their keys and values,
+//            which two blocks would not find room for
+// (A row's softmax spread over two threads was no faster at D = 64 and 8 % slower at 128.)
+// Warps of a block: the softmax, a thread a row (warp w: tile w / 4, TMEM lanes 32 (w % 4) ..), then one for TMA (Q, then K and V through rings of kStages tiles), one
+// for TMEM and the MMAs, and two idle ones that complete the warpgroup which gives its registers to
+// the softmax.
+// TMEM columns: D <= 64: O 64, S 128, P 64: S has its own columns, so the next S is made while the
+// softmax works on this one.  D > 64: O 2 x 128, S 2 x 128, and P overwrites S; the MMAs of a block
+// execute in issue order, so S of step j + 1 follows the P V that reads them.
 //
 // Blocks find their sequence without a prefix sum over the lengths: sequence s owns the slots
-// from floor(cu[s] / 256) + s, at least as many as it has tile pairs, and the slots it does not
-// need return at once.  The heads are the grid's fast axis, and later rows come first when causal,
-// so the long blocks start first.
+// from floor(cu[s] / R) + s (R rows a block), at least as many as it has blocks, and the slots it does
+// not need return at once.  The heads are the grid's fast axis, and later rows come first when
+// causal, so the long blocks start first.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -38,11 +39,8 @@
 namespace tmu {
 namespace k7 {
 
-constexpr int kRows = 256;     // query rows of a block
 constexpr int kTile = 128;     // query rows of a tile, keys of a step
-constexpr int kThreads = 640, kSoftmaxWarps = 16;
 constexpr int kAtom = kTile * 128;  // 64 values of 128 rows
-constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;  // 512 * 104 + 128 * 64 = 640 * 96
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMoveMax = 8.f;
 
@@ -61,29 +59,40 @@ struct Params {
 
 template <int DP, bool BIAS>
 struct Cfg {
+  static constexpr int kTiles = DP == 64 ? 1 : 2;       // of a block
+  static constexpr int kBlocks = DP == 64 ? 2 : 1;      // an SM
+  static constexpr int kRows = kTiles * kTile;
+  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4);
+  // 128 * 200 + 128 * 56 = 256 * 128, 256 * 208 + 128 * 88 = 384 * 168
+  static constexpr int kSoftmaxRegs = DP == 64 ? 200 : 208, kOtherRegs = DP == 64 ? 56 : 88;
   static constexpr int kAtoms = DP / 64;
   static constexpr int kTileBytes = kAtoms * kAtom;
-  static constexpr int kStages = DP == 64 ? (BIAS ? 3 : 4) : 2;
+  static constexpr int kStages = DP == 64 && !BIAS ? 3 : 2;
   static constexpr bool kOwnP = DP == 64;  // P beside S instead of over it
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = 2 * kTileBytes;
+  static constexpr int OFF_K = kTiles * kTileBytes;
   static constexpr int OFF_V = OFF_K + kStages * kTileBytes;
-  // bias of a warp's 32 rows: its 64 keys of a step, or what fits beside the tiles; the rows' pitch
-  // makes the 16-byte accesses of eight rows meet 8 different bank groups
-  static constexpr int kBiasCols = DP == 64 ? 64 : 16;
-  static constexpr int kBiasPitch = kBiasCols * 2 + 16;
+  // A quarter of the exponentials on the FMA units, where two of the special function unit's 16 a
+  // cycle and SM are as long as the products (a half as long at D > 64): 108 -> 100 us at 4096 tokens,
+  // 18 heads of 64; 128 heads' values: 629 -> 643 us of the causal prompts.
+  static constexpr bool kMixedExp = DP == 64;
+  // Bias of a warp's 32 rows: a step's 128 keys, or as many as fit beside the tiles.  The rows' 16-byte
+  // accesses of eight rows meet 8 different bank groups by a swizzle (128 keys: no room for more than
+  // the word behind each row, kept apart) or by the rows' pitch.
+  static constexpr int kBiasCols = DP == 64 ? 128 : 32;
+  static constexpr int kBiasPitch = DP == 64 ? 256 : 80;
   static constexpr int OFF_BIAS = OFF_V + kStages * kTileBytes;
-  static constexpr int OFF_ROW = OFF_BIAS + (BIAS ? kSoftmaxWarps * 32 * kBiasPitch : 0);  // a float a softmax thread
-  static constexpr int OFF_BAR = OFF_ROW + kSoftmaxWarps * 128;
-  static constexpr int SMEM_BYTES = OFF_BAR + 512;
+  static constexpr int OFF_ROW = OFF_BIAS + (BIAS ? kSoftmaxWarps * 32 * kBiasPitch : 0);  // a word a softmax thread
+  static constexpr int OFF_BAR = OFF_ROW + (BIAS && DP == 64 ? kSoftmaxWarps * 128 : 0);
+  static constexpr int SMEM_BYTES = OFF_BAR + 256;
+  static_assert(kBlocks * (SMEM_BYTES + 1024) <= 233472, "K7 shared memory");
   // TMEM columns of tile x
+  static constexpr uint32_t kColumns = kTiles * 256;
   __device__ static constexpr uint32_t o_col(int x) { return x * DP; }
-  __device__ static constexpr uint32_t s_col(int x) { return 2 * DP + x * 128; }
-  __device__ static constexpr uint32_t p_col(int x) { return kOwnP ? 2 * DP + 256 + x * 64 : s_col(x); }
+  __device__ static constexpr uint32_t s_col(int x) { return kTiles * DP + x * 128; }
+  __device__ static constexpr uint32_t p_col(int x) { return kOwnP ? DP + 128 : s_col(x); }
 };
-static_assert(Cfg<64, true>::SMEM_BYTES <= 232448 && Cfg<64, false>::SMEM_BYTES <= 232448 &&
-                  Cfg<128, true>::SMEM_BYTES <= 232448 && Cfg<128, false>::SMEM_BYTES <= 232448,
-              "K7 shared memory exceeds the limit");
 
 enum Site : unsigned int {
   kSiteProdK = 0x701, kSiteProdV = 0x702, kSiteMmaQ = 0x703, kSiteMmaK = 0x704, kSiteMmaV = 0x705, kSiteMmaS = 0x706,
@@ -121,6 +130,32 @@ __device__ __forceinline__ void tie(uint32_t (&r)[32]) {
                : "memory");
 }
 
+// max of three that keeps a NaN
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^t of a pair, t <= kMoveMax or so, on the fused multiply-add units: t = n + f with n the nearest
+// integer (adding 1.5 * 2^23 leaves it in the low bits) and |f| <= 1/2, 2^f by a polynomial of degree 4
+// with constant term 1 (minimax in the relative error, 2^-18.4, against 2^-9 and 2^-11 of the weights'
+// types), n added to the exponent.  t is held at -127 or above, where the sum of exponents is
+// exactly 0: -inf gives +0.  A NaN is lost.
+__device__ __forceinline__ float2 exp2_fma(float2 t) {
+  t = make_float2(fmaxf(t.x, -127.f), fmaxf(t.y, -127.f));
+  const float2 r = __fadd2_rn(t, make_float2(12582912.f, 12582912.f));
+  const float2 n = __fadd2_rn(r, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), t);
+  float2 p = make_float2(0.009581047110259533f, 0.009581047110259533f);
+  p = __ffma2_rn(p, f, make_float2(0.05590597167611122f, 0.05590597167611122f));
+  p = __ffma2_rn(p, f, make_float2(0.24024145305156708f, 0.24024145305156708f));
+  p = __ffma2_rn(p, f, make_float2(0.6931243538856506f, 0.6931243538856506f));
+  p = __ffma2_rn(p, f, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+
 template <int N>
 struct Int {
   static constexpr int value = N;
@@ -128,14 +163,15 @@ struct Int {
 
 __device__ __forceinline__ int clamp_token(int t, int T) { return min(max(t, 0), T); }
 
-// The sequence that owns `slot` (a warp searches 32-ary): the last s with floor(cu[s] / kRows) + s <= slot.
+// The sequence that owns `slot` (a warp searches 32-ary): the last s with floor(cu[s] / R) + s <= slot.
+template <int R>
 __device__ __forceinline__ int find_sequence(const int* cu, int S, int T, int slot) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = S;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32;
     const long long s = lo + static_cast<long long>(lane) * step;
-    const bool in = s < hi && (lane == 0 || clamp_token(__ldg(cu + s), T) / kRows + s <= slot);
+    const bool in = s < hi && (lane == 0 || clamp_token(__ldg(cu + s), T) / R + s <= slot);
     const int b = 31 - __clz(__ballot_sync(0xffffffffu, in));
     lo += b * step;
     hi = min(hi, lo + step);
@@ -144,9 +180,9 @@ __device__ __forceinline__ int find_sequence(const int* cu, int S, int T, int sl
 }
 
 template <typename T, int DP, bool BIAS>
-__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlocks) attention_kernel(const __grid_constant__ Params p) {
   using C = Cfg<DP, BIAS>;
-  constexpr int NS = C::kStages;
+  constexpr int NS = C::kStages, kSoftmaxWarps = C::kSoftmaxWarps, kRows = C::kRows;
   extern __shared__ uint8_t smem[];
   DeviceStatus* const status = p.status != nullptr ? p.status : &g_own_status;
   if (smem_u32(smem) & 1023) {
@@ -158,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   griddep_wait();
 
   const int slot = blockIdx.x / p.hq, head = blockIdx.x - slot * p.hq;
-  const int seq = find_sequence(p.cu, p.S, p.T, slot);
+  const int seq = find_sequence<kRows>(p.cu, p.S, p.T, slot);
   const int beg = clamp_token(__ldg(p.cu + seq), p.T);
   const int len = max(clamp_token(__ldg(p.cu + seq + 1), p.T) - beg, 0);
   const int blocks = (len + kRows - 1) / kRows;
@@ -172,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int keys = p.causal ? min(len, first + kTile) : len;
     return (keys + kTile - 1) / kTile;
   };
-  const int n0 = steps(0), n1 = steps(1), n = max(n0, n1);
+  const int n0 = steps(0), n1 = C::kTiles == 2 ? steps(1) : 0, n = max(n0, n1);
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* kfull = bars;
@@ -200,8 +236,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     for (int x = 0; x < 2; ++x) {
       mbar_init(&qfull[x], 1);
       mbar_init(&sfull[x], 1);
-      mbar_init(&sfree[x], 8);  // the tile's eight warps
-      mbar_init(&pfull[x], 8);
+      mbar_init(&sfree[x], 4);  // the tile's warps
+      mbar_init(&pfull[x], 4);
       mbar_init(&ofull[x], 1);
     }
     mbar_init(&vfixed, 1);
@@ -209,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     fence_mbar_init();
   }
   if (warp == kSoftmaxWarps + 1) {
-    tmem_alloc(&tmem_base_sh, 512);
+    tmem_alloc(&tmem_base_sh, C::kColumns);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -220,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   const bool fix = n * kTile > len;  // the last step's keys end inside the tile
 
   if (warp >= kSoftmaxWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
     if (warp == kSoftmaxWarps) {
       // ------------------------------ loads ------------------------------
       const bool leader = elect_one();
@@ -335,21 +371,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
   } else {
     // ------------------------------ softmax ------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    constexpr int kKeys = kTile / 2;  // of a thread
-    const int x = warp >> 3, half = (warp >> 2) & 1;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+    const int x = warp >> 2;
     const int nx = x == 0 ? n0 : n1;
     const int tile0 = q0 + x * kTile;
     const int row = tile0 + (warp & 3) * 32 + lane;  // within the sequence
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // the row's other half: a float of shared memory each, and a barrier of the two warps
-    float* const mine_f = reinterpret_cast<float*>(smem + C::OFF_ROW) + warp * 32 + lane;
-    const float* const other_f = reinterpret_cast<const float*>(smem + C::OFF_ROW) + (warp ^ 4) * 32 + lane;
-    auto exchange = [&](float f) {
-      *mine_f = f;
-      named_bar_sync(1 + x * 4 + (warp & 3), 64);
-      return *other_f;
-    };
     const bool flip = p.scale < 0.f;
     // a scale of 0 would turn a hidden key's -inf into a NaN
     const float c = fmaxf(fabsf(p.scale) * (BIAS ? 1.f : kLog2e), 1e-30f);
@@ -361,29 +388,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int bn = min(p.bias_n, len);  // rows and keys that have a bias
     uint8_t* bbuf = smem + C::OFF_BIAS + warp * (32 * C::kBiasPitch);
     const T* bbase = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh;
+    auto bias_at = [&](int r, int byte) {  // address of a staged byte of row r
+      if (C::kBiasCols == 128) {
+        if (byte == 256) return smem_u32(smem + C::OFF_ROW) + (warp * 32 + r) * 4u;
+        return smem_u32(bbuf) + r * 256u + ((((byte >> 4) ^ (r & 7)) << 4) | (byte & 15));
+      }
+      return smem_u32(bbuf) + r * static_cast<uint32_t>(C::kBiasPitch) + byte;
+    };
     // copies of W values, kBiasCols / W lanes a row (W = 2: 32 lanes, and one value more in shifted rows)
     auto copy_rows = [&](int k0, auto width) {
       constexpr int W = decltype(width)::value, kLanes = C::kBiasCols / W < 32 ? C::kBiasCols / W : 32;
       const int first = tile0 + (warp & 3) * 32, r0 = lane / kLanes, c = lane % kLanes * W;
       const T* src = bbase + (first + r0) * p.bias_sr + k0 + c;
-      uint32_t dst = smem_u32(bbuf + r0 * C::kBiasPitch) + c * 2;
       const int rows = bn - first, left = bn - k0 - c;  // values of this lane's columns that are there
 #pragma unroll 4
       for (int r = r0; r < 32; r += 32 / kLanes) {
         if (r >= rows) break;
         if (W == 8) {
-          if (left > 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+          if (left > 0) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(bias_at(r, c * 2)), "l"(src) : "memory");
         } else if (W == 4) {
-          if (left > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+          if (left > 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(bias_at(r, c * 2)), "l"(src) : "memory");
         } else {
           const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(src) >> 1) & 1;
 #pragma unroll
           for (int e = 0; e <= C::kBiasCols; e += kLanes * 2)
             if (c + e < C::kBiasCols + shift && left + shift > e)
-              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + e * 2), "l"(src + e - shift) : "memory");
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(bias_at(r, (c + e) * 2)), "l"(src + e - shift)
+                           : "memory");
         }
         src += (32 / kLanes) * p.bias_sr;
-        dst += (32 / kLanes) * C::kBiasPitch;
       }
     };
     auto fetch_bias = [&](int k0) {
@@ -396,41 +429,52 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         BIAS && p.bias_width == 2 ? (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(bbase + row * p.bias_sr) >> 1) & 1u) * 16u : 0u;
     const bool shifted = BIAS && __any_sync(0xffffffffu, bshift != 0u);
     const float2 c2 = make_float2(flip ? -c : c, flip ? -c : c);
-    if (BIAS && nx > 0) fetch_bias(half * kKeys);
+    if (BIAS && nx > 0) fetch_bias(0);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nx; ++j) {
       if (!(ok = warp_poll(&sfull[x], j & 1, ctx, kSiteSoftS))) break;
       tc_fence_after();
-      uint32_t r[2][32];
+      uint32_t r[kTile / 32][32];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) tmem_ld32(tl + C::s_col(x) + half * kKeys + b * 32, r[b]);
+      for (int b = 0; b < kTile / 32; ++b) tmem_ld32(tl + C::s_col(x) + b * 32, r[b]);
       tmem_wait_ld(r[0]);
-      tie(r[1]);
+#pragma unroll
+      for (int b = 1; b < kTile / 32; ++b) tie(r[b]);
       if (C::kOwnP) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sfree[x]);
       }
       float* v = reinterpret_cast<float*>(&r[0][0]);
-      const int k0 = j * kTile + half * kKeys;
+      const int k0 = j * kTile;
       float mul = c;
       if (BIAS) {
         // x = s scale + bias, the exponential's factor is log2 e (without a bias the scale is folded into it)
         mul = kLog2e;
         const int have = row < bn ? bn - k0 : 0;
-        const bool whole = __all_sync(0xffffffffu, have >= kKeys);
+        const bool whole = __all_sync(0xffffffffu, have >= kTile);
 #pragma unroll
-        for (int b0 = 0; b0 < kKeys; b0 += C::kBiasCols) {
+        for (int b0 = 0; b0 < kTile; b0 += C::kBiasCols) {
           asm volatile("cp.async.wait_all;" ::: "memory");
           __syncwarp();
-          const uint4* src = reinterpret_cast<const uint4*>(bbuf + lane * C::kBiasPitch);
+          auto staged = [&](int g) {  // 16 bytes of the row, or the word behind it
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (C::kBiasCols == 128 && g == 16)
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(u.x) : "r"(bias_at(lane, 256)) : "memory");
+            else
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                           : "r"(bias_at(lane, g * 16))
+                           : "memory");
+            return u;
+          };
           auto add = [&](auto check) {
             constexpr bool kCheck = decltype(check)::value != 0;  // rows that start in a word, or end in the tile
-            uint4 q = src[0];
+            uint4 q = staged(0);
 #pragma unroll
             for (int g = 0; g < C::kBiasCols / 8; ++g) {
-              const uint4 next = kCheck || g + 1 < C::kBiasCols / 8 ? src[g + 1] : q;  // (the pitch has room for one more)
+              const uint4 next = kCheck || g + 1 < C::kBiasCols / 8 ? staged(g + 1) : q;
               const uint32_t u[5] = {q.x, q.y, q.z, q.w, next.x};
               q = next;
 #pragma unroll
@@ -447,23 +491,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
           if (whole && !shifted) add(Int<0>());
           else add(Int<1>());
           __syncwarp();
-          if (b0 + C::kBiasCols < kKeys) fetch_bias(k0 + b0 + C::kBiasCols);
-          else if (j + 1 < nx) fetch_bias(k0 + kTile);
+          if (b0 + C::kBiasCols < kTile || j + 1 < nx) fetch_bias(k0 + b0 + C::kBiasCols);
         }
       } else if (flip) {
 #pragma unroll
-        for (int e = 0; e < kKeys; ++e) v[e] = -v[e];
+        for (int e = 0; e < kTile; ++e) v[e] = -v[e];
       }
-      if (k0 + kKeys > len || (p.causal && k0 + kKeys - 1 > tile0)) {
+      if (k0 + kTile > len || (p.causal && k0 + kTile - 1 > tile0)) {
         const int lim = (p.causal ? min(len, row + 1) : len) - k0;
 #pragma unroll
-        for (int e = 0; e < kKeys; ++e) v[e] = e < lim ? v[e] : -INFINITY;
+        for (int e = 0; e < kTile; ++e) v[e] = e < lim ? v[e] : -INFINITY;
       }
       float mx[4] = {v[0], v[1], v[2], v[3]};
+      float part;
+      if (C::kMixedExp) {
 #pragma unroll
-      for (int e = 4; e < kKeys; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
-      const float part = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const float top = fmaxf(part, exchange(part)) * mul;
+        for (int e = 4; e < kTile - 4; e += 8)
+#pragma unroll
+          for (int f = 0; f < 4; ++f) mx[f] = max3_nan(mx[f], v[e + f], v[e + 4 + f]);
+        mx[0] = max3_nan(mx[0], v[kTile - 4], v[kTile - 3]);
+        mx[1] = max3_nan(mx[1], v[kTile - 2], v[kTile - 1]);
+        part = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+      } else {
+#pragma unroll
+        for (int e = 4; e < kTile; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
+        part = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      }
+      const float top = part * mul;
       if (j > 0 && C::kOwnP) {  // P's columns and O belong to P V of the last step (else S's being there says so)
         if (!(ok = warp_poll(&ofull[x], (j - 1) & 1, ctx, kSiteSoftO))) break;
         tc_fence_after();
@@ -476,9 +530,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         if (move) m = top;
         l *= f;
 #pragma unroll 1
-        for (int b = 0; b < DP / 32; ++b) {  // a half of O's columns each
+        for (int b = 0; b < DP / 16; ++b) {
           uint32_t o[16];
-          const uint32_t at = tl + C::o_col(x) + half * (DP / 2) + b * 16;
+          const uint32_t at = tl + C::o_col(x) + b * 16;
           tmem_ld16(at, o);
           tmem_wait_ld16(o);
 #pragma unroll
@@ -489,19 +543,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       const float neg = m == -INFINITY ? 0.f : -m;
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < kTile / 32; ++b) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float2 t = __ffma2_rn(make_float2(v[b * 32 + 2 * e], v[b * 32 + 2 * e + 1]), make_float2(mul, mul),
                                       make_float2(neg, neg));
-          const float2 q = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+          const float2 q = C::kMixedExp && (e & 3) == 3 ? exp2_fma(t) : make_float2(ex2_approx(t.x), ex2_approx(t.y));
           sum = __fadd2_rn(sum, q);
           w[e] = k8::pack2(q.x, q.y, T());
         }
-        tmem_st16(tl + C::p_col(x) + half * 32 + b * 16, w);
+        tmem_st16(tl + C::p_col(x) + b * 16, w);
       }
       l += sum.x + sum.y;
+      // a NaN or an infinite score: its row is NaN, whichever way its exponential went
+      if (C::kMixedExp && !(top < INFINITY)) l = NAN;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -509,12 +565,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     }
     if (ok && nx > 0 && warp_poll(&ofull[x], (nx - 1) & 1, ctx, kSiteEpi)) {
       tc_fence_after();
-      l += exchange(l);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.o.p) + static_cast<long long>(beg + row) * p.o.st + head * p.o.sh;
 #pragma unroll
-      for (int b = 0; b < DP / 64; ++b) {
-        const int c0 = half * (DP / 2) + b * 32;
+      for (int b = 0; b < DP / 32; ++b) {
+        const int c0 = b * 32;
         uint32_t o[32];
         tmem_ld32(tl + C::o_col(x) + c0, o);
         tmem_wait_ld(o);
@@ -536,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
   __syncthreads();
   if (warp == kSoftmaxWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, C::kColumns);
   }
 }
 

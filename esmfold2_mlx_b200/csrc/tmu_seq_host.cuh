@@ -65,7 +65,7 @@ int launch_k7(const k7::Params& p, bool bf16, bool biased, int blocks, cudaStrea
   const int bit = (DP == 128 ? 4 : 0) + (bf16 ? 2 : 0) + (biased ? 1 : 0);
   int st = seq_device(dev, bit, reinterpret_cast<const void*>(kern), smem);
   if (st) return st;
-  cudaError_t e = launch_pdl(kern, blocks, k7::kThreads, smem, stream, p);
+  cudaError_t e = launch_pdl(kern, blocks, k7::Cfg<DP, true>::kThreads, smem, stream, p);
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch attention_kernel");
 }
 
@@ -332,7 +332,8 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
   p.scale = scale;
   p.status = static_cast<DeviceStatus*>(status);
   p.timeout_ns = g_timeout_ns;
-  const long long blocks = (static_cast<long long>(T) / k7::kRows + S) * Hq;
+  const int rows = D <= 64 ? k7::Cfg<64, false>::kRows : k7::Cfg<128, false>::kRows;
+  const long long blocks = (static_cast<long long>(T) / rows + S) * Hq;
   if (blocks > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "too many sequences and heads");
   return D <= 64 ? launch_k7<64>(p, bf16, biased, static_cast<int>(blocks), static_cast<cudaStream_t>(stream))
                  : launch_k7<128>(p, bf16, biased, static_cast<int>(blocks), static_cast<cudaStream_t>(stream));
