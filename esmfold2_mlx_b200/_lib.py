@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib")
@@ -113,7 +114,27 @@ class TmuAttnBias(ctypes.Structure):
                 ("stride_row", ctypes.c_longlong), ("n", _i)]
 
 
-_H = ctypes.POINTER(TmuHeads)
+class TmuQkNormRopeArgs(ctypes.Structure):
+    """Mirror of ``tmu_qk_norm_rope_args``."""
+
+    _fields_ = [("q", TmuHeads), ("k", TmuHeads), ("q_out", TmuHeads), ("k_out", TmuHeads), ("norm", TmuQkNorm),
+                ("rotary", TmuRotary), ("T", _i), ("Hq", _i), ("Hkv", _i), ("D", _i), ("dtype", _i)]
+
+
+class TmuAttentionArgs(ctypes.Structure):
+    """Mirror of ``tmu_attention_args``."""
+
+    _fields_ = [("q", TmuHeads), ("k", TmuHeads), ("v", TmuHeads), ("out", TmuHeads), ("cu_seqlens", _vp),
+                ("bias", TmuAttnBias), ("S", _i), ("T", _i), ("Hq", _i), ("Hkv", _i), ("D", _i), ("dtype", _i),
+                ("causal", _i), ("scale", _f), ("status", _vp)]
+
+
+# The same layouts for struct.pack, which fills one in a tenth of the time of a ctypes structure:
+# these calls come once a layer and are often bound by what the host does.
+_HEADS = "Pqq"
+QK_NORM_ROPE_ARGS = struct.Struct("@" + 4 * _HEADS + "ifPPPP" + "PiPfii4x" + "iiiii4x")
+ATTENTION_ARGS = struct.Struct("@" + 4 * _HEADS + "P" + "Pqqqi4x" + "iiiiiiifP")
+
 _ll = ctypes.c_longlong
 _W = ctypes.POINTER(TmuTrimulWeights)
 _G = ctypes.POINTER(TmuPairLayout)
@@ -149,9 +170,8 @@ SIGNATURES = {
                            _sz, _vp, _vp]),
     "tmu_parcae_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmu_parcae_step": (_i, [_vp, _vp, _vp, ctypes.POINTER(TmuParcaeWeights), _vp, _i, _i, _i, _vp, _sz, _vp, _vp]),
-    "tmu_qk_norm_rope": (_i, [_H, _H, _H, _H, ctypes.POINTER(TmuQkNorm), ctypes.POINTER(TmuRotary), _i, _i, _i, _i, _i,
-                              _vp]),
-    "tmu_attention": (_i, [_H, _H, _H, _H, _vp, ctypes.POINTER(TmuAttnBias), _i, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
+    "tmu_qk_norm_rope": (_i, [_vp, _vp]),
+    "tmu_attention": (_i, [_vp, _vp]),
     "tmu_quantize_rows": (_i, [_vp, _i, _ll, _i, _i, _vp, _vp, _vp]),
     "tmu_linear_fp8_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmu_linear_fp8": (_i, [_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _i, _ll, _i, _i, _i, _vp, _sz, _vp, _vp]),

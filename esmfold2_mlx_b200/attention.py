@@ -33,7 +33,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 def launch(device: torch.device, where: str, *args) -> None:
     """Call the C entry ``where`` with ``args`` and the current stream of ``device``, which is made the
     current device for the call if it is not."""
-    fn = getattr(_lib.load(), where)
+    fn = getattr(_lib._lib or _lib.load(), where)
     index = device.index
     if torch.cuda.current_device() == index:
         code = fn(*args, _raw_stream(index))
@@ -44,8 +44,8 @@ def launch(device: torch.device, where: str, *args) -> None:
         _lib.check(code, where)
 
 
-def pointer(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def pointer(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def refuse_grad(where: str, *tensors) -> None:
@@ -67,28 +67,27 @@ def spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() < b.data_ptr() + span(b) and b.data_ptr() < a.data_ptr() + span(a)
 
 
-def _check_heads(name: str, t: torch.Tensor, T: int, D: int, like: torch.Tensor) -> None:
-    shape = t.shape
+def _view(name: str, t: torch.Tensor, T: int, D: int, like: torch.Tensor) -> tuple[int, int, int, int]:
+    """Address, token stride, head stride and heads of a [T, H, D] view of ``like``'s type and device."""
+    shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[0] != T or shape[2] != D:
         raise ValueError(f"{name} must be [{T}, heads, {D}], got {tuple(shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
+    if t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{name} must have q's type and device")
-    if t.stride(2) != 1 and D > 1:
+    if stride[2] != 1 and D > 1:
         raise ValueError(f"the values of a head of {name} must be contiguous")
-
-
-def _heads(t: torch.Tensor) -> _lib.TmuHeads:
+    heads = shape[1]
     # an axis of length one is never stepped along: its stride is whatever the view happened to have
-    (T, H, _), (st, sh, _) = t.shape, t.stride()
-    return _lib.TmuHeads(t.data_ptr(), st if T > 1 else 0, sh if H > 1 else 0)
+    return t.data_ptr(), stride[0] if T > 1 else 0, stride[1] if heads > 1 else 0, heads
 
 
 def _check_first(name: str, q: torch.Tensor) -> int:
-    if not q.is_cuda or q.dtype not in _DTYPES:
+    code = _DTYPES.get(q.dtype)
+    if code is None or not q.is_cuda:
         raise TypeError(f"{name} must be a CUDA fp16 or bf16 tensor")
     if q.dim() != 3:
         raise ValueError(f"{name} must be [T, heads, D], got {tuple(q.shape)}")
-    return _DTYPES[q.dtype]
+    return code
 
 
 class Rotary:
@@ -160,9 +159,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
     ``k_out`` may be ``k``; other overlaps are refused."""
     dtype = _check_first("q", q)
     T, hq, D = q.shape
-    _check_heads("k", k, T, D, q)
-    _check_heads("q", q, T, D, q)
-    if norm not in _NORMS:
+    qp, qt, qh, _ = _view("q", q, T, D, q)
+    kp, kt, kh, hk = _view("k", k, T, D, q)
+    kind = _NORMS.get(norm)
+    if kind is None:
         raise ValueError("norm must be None, 'rms' or 'layer'")
     refuse_grad("qk_norm_rope", q, k, q_weight, k_weight, q_bias, k_bias)
     if norm is None:
@@ -170,29 +170,30 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
             raise ValueError("weights and biases need a norm")
     else:
         for p in (q_weight, k_weight, q_bias, k_bias):
-            if p is not None and (p.dtype != torch.float32 or p.device != q.device or p.shape != (D,)
-                                  or not p.is_contiguous()):
+            if p is not None and (p.dtype is not torch.float32 or p.dim() != 1 or p.shape[0] != D
+                                  or p.device != q.device or not p.is_contiguous()):
                 raise ValueError(f"weights and biases must be contiguous fp32 [{D}] tensors on q's device")
-    rot = _lib.TmuRotary(None, 4, None, 1.0, 0, 0)
+    rot = (0, 4, 0, 1.0, 0, 0)
     if rotary is not None:
         if rotary.rot > D:
             raise ValueError(f"the rotary's {rotary.rot} values exceed the head's {D}")
         if positions is None:
             raise ValueError("a rotary needs positions")
-        if (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (T,)
+        if (positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 1 or positions.shape[0] != T
                 or positions.device != q.device or not positions.is_contiguous()):
             raise ValueError(f"positions must be a contiguous int32 or int64 [{T}] tensor on q's device")
         if rotary.turns.device != q.device:
             raise ValueError("the rotary must be on q's device")
-        rot = _lib.TmuRotary(positions.data_ptr(), positions.element_size(), rotary.turns.data_ptr(), rotary.gain,
-                             rotary.rot, 1 if rotary.layout == "interleaved" else 0)
+        rot = (positions.data_ptr(), positions.element_size(), rotary.turns.data_ptr(), rotary.gain, rotary.rot,
+               1 if rotary.layout == "interleaved" else 0)
     if q_out is not None or k_out is not None:
         _check_rope_outputs(q, k, q_out, k_out)
-    q_out = q.new_empty(q.shape) if q_out is None else q_out
-    k_out = k.new_empty(k.shape) if k_out is None else k_out
-    nrm = _lib.TmuQkNorm(_NORMS[norm], eps, pointer(q_weight), pointer(q_bias), pointer(k_weight), pointer(k_bias))
-    launch(q.device, "tmu_qk_norm_rope", _heads(q), _heads(k), _heads(q_out), _heads(k_out), nrm, rot, T, hq,
-           k.shape[1], D, dtype)
+    q_out = q.new_empty((T, hq, D)) if q_out is None else q_out
+    k_out = q.new_empty((T, hk, D)) if k_out is None else k_out
+    args = _lib.QK_NORM_ROPE_ARGS.pack(qp, qt, qh, kp, kt, kh, *_view("q_out", q_out, T, D, q)[:3],
+                                       *_view("k_out", k_out, T, D, q)[:3], kind, eps, pointer(q_weight), pointer(q_bias),
+                                       pointer(k_weight), pointer(k_bias), *rot, T, hq, hk, D, dtype)
+    launch(q.device, "tmu_qk_norm_rope", args)
     return q_out, k_out
 
 
@@ -201,7 +202,7 @@ def _check_rope_outputs(q, k, q_out, k_out) -> None:
     for name, src, dst, other in (("q_out", q, q_out, k), ("k_out", k, k_out, q)):
         if dst is None:
             continue
-        _check_heads(name, dst, T, D, q)
+        _view(name, dst, T, D, q)
         if dst.shape != src.shape:
             raise ValueError(f"{name} must be shaped like its input")
         if _self_overlap(dst):
@@ -261,37 +262,38 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     tokens of no sequence have no influence."""
     dtype = _check_first("q", q)
     T, hq, D = q.shape
-    _check_heads("q", q, T, D, q)
-    _check_heads("k", k, T, D, q)
-    _check_heads("v", v, T, D, q)
-    if v.shape != k.shape:
+    qp, qt, qh, _ = _view("q", q, T, D, q)
+    kp, kt, kh, hk = _view("k", k, T, D, q)
+    vp, vt, vh, hv = _view("v", v, T, D, q)
+    if hv != hk:
         raise ValueError("k and v must have the same heads")
     refuse_grad("attention", q, k, v, bias)
-    if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1
-            or cu_seqlens.device != q.device or not cu_seqlens.is_contiguous()):
+    if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.device != q.device
+            or not cu_seqlens.is_contiguous() or cu_seqlens.shape[0] < 1):
         raise ValueError("cu_seqlens must be a contiguous int32 [S + 1] tensor on q's device")
-    S = cu_seqlens.numel() - 1
-    b = None
+    S = cu_seqlens.shape[0] - 1
+    b = (0, 0, 0, 0, 0)
     if bias is not None:
-        if (bias.dim() != 4 or bias.shape[0] not in (1, S) or bias.shape[1] != hq or bias.shape[2] != bias.shape[3]
-                or bias.dtype != q.dtype or bias.device != q.device):
+        shape = bias.shape
+        if (len(shape) != 4 or shape[0] not in (1, S) or shape[1] != hq or shape[2] != shape[3]
+                or bias.dtype is not q.dtype or bias.device != q.device):
             raise ValueError(f"bias must be [1 or {S}, {hq}, n, n] of q's type on its device")
-        n = bias.shape[2]
-        if n > 1 and bias.stride(3) != 1:
+        n, stride = shape[2], bias.stride()
+        if n > 1 and stride[3] != 1:
             raise ValueError("the last axis of bias must be contiguous")
-        b = _lib.TmuAttnBias(bias.data_ptr(), bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1),
-                             bias.stride(2), n)
+        b = (bias.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1], stride[2], n)
     if out is None:
-        out = q.new_empty(q.shape)
+        out = q.new_empty((T, hq, D))
     else:
-        _check_heads("out", out, T, D, q)
         if out.shape != q.shape:
             raise ValueError("out must be shaped like q")
         if _self_overlap(out) or any(_heads_overlap(out, t) for t in (q, k, v)):
             raise ValueError("out must not overlap itself, q, k or v")
         if bias is not None and spans_overlap(out, bias):
             raise ValueError("out must not overlap bias")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    launch(q.device, "tmu_attention", _heads(q), _heads(k), _heads(v), _heads(out), cu_seqlens.data_ptr(), b, S, T, hq,
-           k.shape[1], D, dtype, 1 if causal else 0, scale, pointer(status))
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    args = _lib.ATTENTION_ARGS.pack(qp, qt, qh, kp, kt, kh, vp, vt, vh, *_view("out", out, T, D, q)[:3],
+                                    cu_seqlens.data_ptr(), *b, S, T, hq, hk, D, dtype, 1 if causal else 0, scale,
+                                    pointer(status))
+    launch(q.device, "tmu_attention", args)
     return out

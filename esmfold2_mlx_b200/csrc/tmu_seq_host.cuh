@@ -216,10 +216,12 @@ int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8
 
 extern "C" {
 
-int tmu_qk_norm_rope(const tmu_heads* q, const tmu_heads* k, const tmu_heads* q_out, const tmu_heads* k_out,
-                     const tmu_qk_norm* norm, const tmu_rotary* rot, int T, int Hq, int Hkv, int D, int dtype,
-                     void* stream) {
-  if (!q || !k || !q_out || !k_out || !norm || !rot) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+int tmu_qk_norm_rope(const tmu_qk_norm_rope_args* args, void* stream) {
+  if (!args) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+  const tmu_heads *q = &args->q, *k = &args->k, *q_out = &args->q_out, *k_out = &args->k_out;
+  const tmu_qk_norm* norm = &args->norm;
+  const tmu_rotary* rot = &args->rotary;
+  const int T = args->T, Hq = args->Hq, Hkv = args->Hkv, D = args->D, dtype = args->dtype;
   int st = check_packed(T, Hq, Hkv, D);
   if (st) return st;
   if (D % 16 || D > 256) return fail(TMU_ERR_UNSUPPORTED, "D must be a multiple of 16, at most 256");
@@ -277,10 +279,15 @@ int tmu_qk_norm_rope(const tmu_heads* q, const tmu_heads* k, const tmu_heads* q_
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch qk_rope_kernel");
 }
 
-int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, const tmu_heads* out,
-                  const int* cu_seqlens, const tmu_attn_bias* bias, int S, int T, int Hq, int Hkv, int D, int dtype,
-                  int causal, float scale, void* status, void* stream) {
-  if (!q || !k || !v || !out) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+int tmu_attention(const tmu_attention_args* args, void* stream) {
+  if (!args) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+  const tmu_heads *q = &args->q, *k = &args->k, *v = &args->v, *out = &args->out;
+  const int* cu_seqlens = args->cu_seqlens;
+  const tmu_attn_bias* bias = &args->bias;
+  const int S = args->S, T = args->T, Hq = args->Hq, Hkv = args->Hkv, D = args->D, dtype = args->dtype;
+  const int causal = args->causal;
+  const float scale = args->scale;
+  void* status = args->status;
   int st = check_packed(T, Hq, Hkv, D);
   if (st) return st;
   if (S < 0) return fail(TMU_ERR_INVALID_ARGUMENT, "S must not be negative");
@@ -293,13 +300,13 @@ int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, co
   static const char* const names[4] = {"q", "k", "v", "out"};
   for (int i = 0; i < 4; ++i)
     if ((st = check_heads(views[i]->data, views[i]->stride_token, views[i]->stride_head, names[i]))) return st;
-  if (bias && (bias->n < 0 || (bias->n > 0 && !bias->data))) return fail(TMU_ERR_INVALID_ARGUMENT, "bias");
+  if (bias->n < 0 || (bias->n > 0 && !bias->data)) return fail(TMU_ERR_INVALID_ARGUMENT, "bias");
   // a tensor map cannot step by 0
   const int heads[3] = {Hq, Hkv, Hkv};
   for (int i = 0; i < 3; ++i)
     if ((T > 1 && views[i]->stride_token == 0) || (heads[i] > 1 && views[i]->stride_head == 0))
       return fail(TMU_ERR_UNSUPPORTED, "q, k and v must not be broadcast views");
-  const bool bf16 = dtype == TMU_BF16, biased = bias && bias->n > 0;
+  const bool bf16 = dtype == TMU_BF16, biased = bias->n > 0;
   k7::Params p;
   memset(&p, 0, sizeof(p));
   CUtensorMap* maps[3] = {&p.tm_q, &p.tm_k, &p.tm_v};

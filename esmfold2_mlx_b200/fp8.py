@@ -120,46 +120,51 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
 
     ``bias`` is fp32 [N].  The output is ``out_dtype`` (fp16, bf16 or fp32; x's type by default, fp16 for
     e4m3 x) or ``out`` [..., N], which must not overlap an input."""
-    if not x.is_cuda or x.dtype not in _IN:
+    code = _IN.get(x.dtype)
+    if code is None or not x.is_cuda:
         raise TypeError("x must be a CUDA fp16, bf16 or float8_e4m3fn tensor")
-    n, k = weight.shape
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"x must be [..., {k}], got {tuple(x.shape)}")
-    if weight.w8.device != x.device:
+    w8, scales, shape = weight.w8, weight.scales, x.shape
+    n, k = w8.shape
+    if len(shape) < 1 or shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(shape)}")
+    if w8.device != x.device:
         raise ValueError("the weight must be on x's device")
     refuse_grad("fp8.linear", x, bias)
-    lead = x.shape[:-1]
     rows = _rows("x", x)
-    m = rows.shape[0]
-    xs = None
-    if x.dtype == torch.float8_e4m3fn:
-        if (x_scales is None or x_scales.dtype != torch.float32 or x_scales.shape != (*lead, _blocks(k))
+    m, ld = rows.shape[0], _ld(rows)
+    xs = 0
+    if code == _lib.TMU_E4M3:
+        want = (*shape[:-1], _blocks(k))
+        if (x_scales is None or x_scales.dtype is not torch.float32 or x_scales.shape != want
                 or x_scales.device != x.device or not x_scales.is_contiguous()):
-            raise ValueError(f"e4m3 x needs contiguous fp32 x_scales {[*lead, _blocks(k)]} on its device")
+            raise ValueError(f"e4m3 x needs contiguous fp32 x_scales {list(want)} on its device")
         if not x.is_contiguous():
             raise ValueError("e4m3 x must be contiguous")
-        xs = x_scales
+        xs = x_scales.data_ptr()
     elif x_scales is not None:
         raise ValueError("x_scales go with e4m3 x")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != x.device
-                             or not bias.is_contiguous()):
+    if bias is not None and (bias.dtype is not torch.float32 or bias.dim() != 1 or bias.shape[0] != n
+                             or bias.device != x.device or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous fp32 [{n}] tensor on x's device")
     if out is None:
-        dt = out_dtype or (torch.float16 if x.dtype == torch.float8_e4m3fn else x.dtype)
-        if dt not in _OUT:
+        dt = out_dtype or (torch.float16 if code == _lib.TMU_E4M3 else x.dtype)
+        out_code = _OUT.get(dt)
+        if out_code is None:
             raise TypeError("out_dtype must be fp16, bf16 or fp32")
-        out = x.new_empty((*lead, n), dtype=dt)
+        out = x.new_empty((*shape[:-1], n), dtype=dt)
+        to, ldo = out.data_ptr(), n
     else:
-        if out.shape != (*lead, n) or out.device != x.device or out.dtype not in _OUT:
-            raise ValueError(f"out must be an fp16, bf16 or fp32 {[*lead, n]} tensor on x's device")
+        out_code = _OUT.get(out.dtype)
+        if out_code is None or out.shape != (*shape[:-1], n) or out.device != x.device:
+            raise ValueError(f"out must be an fp16, bf16 or fp32 {[*shape[:-1], n]} tensor on x's device")
         if out_dtype not in (None, out.dtype):
             raise ValueError("out_dtype differs from out's type")
-        if any(t is not None and spans_overlap(out, t) for t in (x, weight.w8, weight.scales, bias, xs)):
+        if any(t is not None and spans_overlap(out, t) for t in (x, w8, scales, bias, x_scales)):
             raise ValueError("out must not overlap an input")
-    orow = _rows("out", out)
-    need = int(_lib.load().tmu_linear_fp8_workspace_bytes(m, n, k))
-    ws = x.new_empty(need, dtype=torch.uint8) if need else None
-    launch(x.device, "tmu_linear_fp8", rows.data_ptr(), _IN[x.dtype], _ld(rows), pointer(xs), weight.w8.data_ptr(),
-           weight.scales.data_ptr(), pointer(bias), orow.data_ptr(), _OUT[out.dtype], _ld(orow), m, n, k, pointer(ws), need,
-           pointer(status))
+        orow = _rows("out", out)
+        to, ldo = orow.data_ptr(), _ld(orow)
+    need = (_lib._lib or _lib.load()).tmu_linear_fp8_workspace_bytes(m, n, k)
+    ws = x.new_empty((need,), dtype=torch.uint8).data_ptr() if need else 0
+    launch(x.device, "tmu_linear_fp8", rows.data_ptr(), code, ld, xs, w8.data_ptr(), scales.data_ptr(), pointer(bias), to,
+           out_code, ldo, m, n, k, ws, need, pointer(status))
     return out

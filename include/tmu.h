@@ -372,13 +372,18 @@ typedef struct tmu_rotary {
 /* K8: norm of every head of q [T, Hq, D] and k [T, Hkv, D] over its D values, then the rotation of
  * its first `rot` values, fp32 inside and rounded once.  D a multiple of 16, at most 256; fp16 or
  * bf16 in and out.  An output may be its own input; otherwise the four must not overlap. */
-int tmu_qk_norm_rope(const tmu_heads* q, const tmu_heads* k, const tmu_heads* q_out, const tmu_heads* k_out,
-                     const tmu_qk_norm* norm, const tmu_rotary* rot, int T, int Hq, int Hkv, int D, int dtype,
-                     void* stream);
+typedef struct tmu_qk_norm_rope_args {
+  tmu_heads q, k, q_out, k_out;
+  tmu_qk_norm norm;
+  tmu_rotary rotary;
+  int T, Hq, Hkv, D, dtype;
+} tmu_qk_norm_rope_args;
+
+int tmu_qk_norm_rope(const tmu_qk_norm_rope_args* args, void* stream);
 
 /* Additive bias of the scores, of q's type: element (i, j) of sequence s and query head h at
  * s * stride_seq + h * stride_head + i * stride_row + j (a stride of 0 shares it).  Positions at or
- * past n have none. */
+ * past n have none; n = 0 for no bias. */
 typedef struct tmu_attn_bias {
   const void* data;
   long long stride_seq, stride_head, stride_row;
@@ -392,9 +397,16 @@ typedef struct tmu_attn_bias {
  * weights are rounded to q's type for their product with v.  A row whose scores are all -inf is 0,
  * and tokens of no sequence keep what `out` holds.  `out` must not overlap q, k or v.  status may be
  * NULL. */
-int tmu_attention(const tmu_heads* q, const tmu_heads* k, const tmu_heads* v, const tmu_heads* out,
-                  const int* cu_seqlens, const tmu_attn_bias* bias, int S, int T, int Hq, int Hkv, int D, int dtype,
-                  int causal, float scale, void* status, void* stream);
+typedef struct tmu_attention_args {
+  tmu_heads q, k, v, out;
+  const int* cu_seqlens; /* [S + 1] */
+  tmu_attn_bias bias;
+  int S, T, Hq, Hkv, D, dtype, causal;
+  float scale;
+  void* status;
+} tmu_attention_args;
+
+int tmu_attention(const tmu_attention_args* args, void* stream);
 
 /* K9, operands: x [M, K] fp16 or bf16 (rows ld elements apart, a multiple of 8) to e4m3 x8 [M, K]
  * and fp32 scales [M, ceil(K / 128)]: scale = max(amax / 448, 2^-126) over 128 values of a row,

@@ -27,7 +27,9 @@ def heads(data=P, st=64, sh=64):
 
 def attention(lib, q=None, k=None, v=None, o=None, cu=P, bias=None, S=1, T=4, hq=2, hkv=1, d=64, dtype=0):
     h = heads()
-    return lib.tmu_attention(q or h, k or h, v or h, o or h, cu, bias, S, T, hq, hkv, d, dtype, 0, 0.125, None, None)
+    a = _lib.TmuAttentionArgs(q or h, k or h, v or h, o or h, cu, bias or _lib.TmuAttnBias(), S, T, hq, hkv, d, dtype, 0,
+                              0.125, None)
+    return lib.tmu_attention(ctypes.byref(a), None)
 
 
 def test_attention_refusals(lib):
@@ -47,7 +49,23 @@ def test_attention_refusals(lib):
         assert attention(lib, **{name: heads(st=-64)}) == INVALID
     assert attention(lib, bias=_lib.TmuAttnBias(None, 0, 0, 0, 5)) == INVALID
     assert attention(lib, bias=_lib.TmuAttnBias(P, 0, 0, 0, -1)) == INVALID
-    assert lib.tmu_attention(None, None, None, None, P, None, 1, 4, 2, 1, 64, 0, 0, 1.0, None, None) == INVALID
+    assert lib.tmu_attention(None, None) == INVALID
+
+
+def test_packed_arguments_have_the_structures_layout():
+    """struct.pack's formats against the ctypes mirrors, field by field."""
+    for fmt, cls in ((_lib.ATTENTION_ARGS, _lib.TmuAttentionArgs), (_lib.QK_NORM_ROPE_ARGS, _lib.TmuQkNormRopeArgs)):
+        assert fmt.size == ctypes.sizeof(cls)
+    a = _lib.TmuAttentionArgs.from_buffer_copy(_lib.ATTENTION_ARGS.pack(*range(1, 19), 19, 20, 21, 22, 23, 24, 25, 0.5, 26))
+    assert (a.q.data, a.k.stride_head, a.out.stride_token, a.cu_seqlens, a.bias.data, a.bias.stride_row, a.bias.n, a.S) == (
+        1, 6, 11, 13, 14, 17, 18, 19)
+    assert (a.T, a.dtype, a.causal, a.scale, a.status) == (20, 24, 25, 0.5, 26)
+    r = _lib.TmuQkNormRopeArgs.from_buffer_copy(
+        _lib.QK_NORM_ROPE_ARGS.pack(*range(1, 13), 13, 0.5, 14, 15, 16, 17, 18, 8, 19, 2.0, 20, 1, 21, 22, 23, 24, 25))
+    assert (r.k_out.stride_head, r.norm.kind, r.norm.eps, r.norm.k_bias, r.rotary.positions, r.rotary.position_bytes) == (
+        12, 13, 0.5, 17, 18, 8)
+    assert (r.rotary.turns, r.rotary.gain, r.rotary.rot, r.rotary.interleaved, r.T, r.Hq, r.Hkv, r.D, r.dtype) == (
+        19, 2.0, 20, 1, 21, 22, 23, 24, 25)
 
 
 def test_empty_calls_do_nothing(lib):
@@ -63,7 +81,7 @@ def rope(lib, d=64, T=4, dtype=0, kind=1, rot=64, pos=P, turns=P, nbytes=4, q=No
     h = heads()
     nrm = _lib.TmuQkNorm(kind, 1e-5, w, None, None, None)
     r = _lib.TmuRotary(pos, nbytes, turns, 1.0, rot, 0)
-    return lib.tmu_qk_norm_rope(q or h, h, h, h, nrm, r, T, hq, 1, d, dtype, None)
+    return lib.tmu_qk_norm_rope(ctypes.byref(_lib.TmuQkNormRopeArgs(q or h, h, h, h, nrm, r, T, hq, 1, d, dtype)), None)
 
 
 def test_qk_norm_rope_refusals(lib):
