@@ -659,13 +659,15 @@ __global__ void __launch_bounds__(kThreads, 2) linear8_kernel(const __grid_const
 // operands of the tiles that run together stay in L2.
 //
 // A step's products are needed apart from the next step's, and TMEM holds two steps (512
-// columns), so the rate hangs on how soon a slot is free again.  Sixteen warps take the products
-// out, 64 columns each, and touch no mbarrier on the way: an mbarrier operation waits behind the
-// MMAs' reads of shared memory (100 to 270 cycles each were seen), so one warp polls for the MMAs'
-// commits and one hands the slots back, and both meet the sixteen at named barriers.
+// columns), so the rate hangs on how soon a slot is free again.  A step is made as two halves of 128
+// columns with slots of their own, so that one is taken out while the other is made.  Eight warps a
+// half take the products out, 64 columns each, and touch no mbarrier on the way: an mbarrier
+// operation waits behind the MMAs' reads of shared memory (100 to 270 cycles each were seen), so a
+// warp of each half polls for the MMAs' commits and hands the slots back, and meets the eight at
+// named barriers.
 //   warp 0      TMA of this CTA's halves, counted on the even CTA's barrier (.cta_group::2)
-//   warp 1      TMEM and, in the even CTA, the MMAs (M = N = 256, four of K = 32 a step)
-//   warp 2      waits for a step's products       warp 3   hands its slot back to the even CTA
+//   warp 1      TMEM and, in the even CTA, the MMAs (M = 256, N = 128, four of K = 32 a half)
+//   warps 2-3   half 0's and 1's barriers
 //   warps 4-19  sums: half h of the columns = warps 4 + 8 h .., two warps a TMEM lane quadrant
 // ------------------------------------------------------------------------------------------
 namespace pair {
@@ -674,8 +676,8 @@ constexpr int kStages = 5;
 constexpr int kThreads = 640;
 constexpr int kTileMN = 256;
 constexpr int kGroup = 8;
-constexpr int kSumThreads = 512;
-constexpr int kBarFull = 1, kBarRead = 3;  // named barriers of the two slots: products there, products read
+constexpr int kSumThreads = 256;           // of a half
+constexpr int kBarFull = 1, kBarRead = 5;  // named barriers of the four slots: products there, products read
 constexpr int kSumRegs = 104, kOtherRegs = 64;  // 512 * 104 + 128 * 64 = 640 * 96
 constexpr int OFF_A = 0;
 constexpr int OFF_B = kStages * kOperand;
@@ -738,9 +740,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
   uint64_t* full = bars;              // [kStages] even CTA: both CTAs' halves have landed
   uint64_t* empty = bars + kStages;   // [kStages] the paired MMAs have read the stage (both CTAs)
-  uint64_t* sfull = bars + 2 * kStages;  // [2] a step's products are in the slot (both CTAs)
-  uint64_t* sempty = sfull + 2;          // [2] even CTA: both CTAs' readers have them
-  uint64_t& drain_bar = sempty[2];
+  uint64_t* sfull = bars + 2 * kStages;  // [2 steps][2 halves] the products are in the slot (both CTAs)
+  uint64_t* sempty = sfull + 4;          // [2 steps][2 halves] even CTA: both CTAs' readers have them
+  uint64_t& drain_bar = sempty[4];
   uint32_t& tmem_base_sh = *reinterpret_cast<uint32_t*>(&drain_bar + 1);
   volatile int& abort_sh = *reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(&drain_bar + 1) + 4);
   const WaitCtx ctx{status, &abort_sh, p.timeout_ns};
@@ -754,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&sfull[s], 1);
       mbar_init(&sempty[s], 2);
     }
@@ -786,13 +788,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         int m0, n0;
         decode(p, t, m0, n0);
         m0 += static_cast<int>(rank) * kTile;
-        n0 += static_cast<int>(rank) * kTile;
+        n0 += static_cast<int>(rank) * (kTile / 2);
         for (int b = 0; b < p.kb; ++b, ++i) {
           if (!(ok = warp_poll(&empty[s], ph ^ 1, ctx, kSiteProd))) break;
           if (leader) {
             if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
             tma_load_2d_pair(smem + OFF_A + s * kOperand, &p.tm_x, bar0 + s * sizeof(uint64_t), b * 128, m0);
+            // of each half's 128 rows of w8 the CTA brings 64
             tma_load_2d_pair(smem + OFF_B + s * kOperand, &p.tm_w, bar0 + s * sizeof(uint64_t), b * 128, n0);
+            tma_load_2d_pair(smem + OFF_B + s * kOperand + kOperand / 2, &p.tm_w, bar0 + s * sizeof(uint64_t), b * 128, n0 + kTile);
           }
           __syncwarp();
           if (++s == kStages) {
@@ -810,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
     } else if (warp == 1 && rank == 0) {
       // The whole warp walks the steps and one lane issues: what the MMAs take from uniform registers
       // (descriptors, addresses) is then computed there, and not moved there value by value.
-      const uint32_t idesc = idesc_e4m3_f32(kTileMN, kTileMN);
+      const uint32_t idesc = idesc_e4m3_f32(kTileMN, kTile);
       const uint64_t ad = sdesc_sw128(smem_u32(smem + OFF_A), 16, 1024), bd = sdesc_sw128(smem_u32(smem + OFF_B), 16, 1024);
       const bool leader = elect_one();
       uint32_t s = 0, ph = 0, i = 0;
@@ -819,19 +823,22 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         for (int b = 0; b < p.kb; ++b, ++i) {
           const uint32_t c = i & 1;
           warp_poll(&full[s], ph, ctx, kSiteMma);
-          warp_poll(&sempty[c], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot);
-          tc_fence_after();
-          const uint64_t as = sdesc_add(ad, s * kOperand), bs = sdesc_add(bd, s * kOperand);
-          const uint32_t d = tmem + c * 256;
-          if (leader) {
-            umma_f8_pair(d, as, bs, idesc, 0u);
-            umma_f8_pair(d, sdesc_add(as, 32), sdesc_add(bs, 32), idesc, 1u);
-            umma_f8_pair(d, sdesc_add(as, 64), sdesc_add(bs, 64), idesc, 1u);
-            umma_f8_pair(d, sdesc_add(as, 96), sdesc_add(bs, 96), idesc, 1u);
-            umma_commit_pair(&sfull[c], 0x3);
-            umma_commit_pair(&empty[s], 0x3);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            warp_poll(&sempty[2 * c + h], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot);
+            tc_fence_after();
+            const uint64_t as = sdesc_add(ad, s * kOperand), bs = sdesc_add(bd, s * kOperand + h * (kOperand / 2));
+            const uint32_t d = tmem + c * 256 + h * kTile;
+            if (leader) {
+              umma_f8_pair(d, as, bs, idesc, 0u);
+              umma_f8_pair(d, sdesc_add(as, 32), sdesc_add(bs, 32), idesc, 1u);
+              umma_f8_pair(d, sdesc_add(as, 64), sdesc_add(bs, 64), idesc, 1u);
+              umma_f8_pair(d, sdesc_add(as, 96), sdesc_add(bs, 96), idesc, 1u);
+              umma_commit_pair(&sfull[2 * c + h], 0x3);
+              if (h == 1) umma_commit_pair(&empty[s], 0x3);
+            }
+            __syncwarp();
           }
-          __syncwarp();
           if (++s == kStages) {
             s = 0;
             ph ^= 1;
@@ -842,25 +849,23 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         mbar_drain(&drain_bar, 0, 200000000ull);
       }
       __syncwarp();
-    } else if (warp == 2) {
+    } else if (warp >= 2) {
+      const int h = warp - 2;
+      const uint32_t slots = cluster_addr(&sempty[h], 0);
       uint32_t i = 0;
       for (int t = first; t < tiles; t += step)
         for (int b = 0; b < p.kb; ++b, ++i) {
-          warp_poll(&sfull[i & 1], (i >> 1) & 1, ctx, kSiteSum);
-          named_bar_arrive(kBarFull + (i & 1), kSumThreads + 32);
-        }
-    } else if (warp == 3) {
-      const uint32_t slots = cluster_addr(&sempty[0], 0);
-      uint32_t i = 0;
-      for (int t = first; t < tiles; t += step)
-        for (int b = 0; b < p.kb; ++b, ++i) {
-          named_bar_sync(kBarRead + (i & 1), kSumThreads + 32);
+          const uint32_t c = i & 1;
+          warp_poll(&sfull[2 * c + h], (i >> 1) & 1, ctx, kSiteSum);
+          named_bar_arrive(kBarFull + 2 * c + h, kSumThreads + 32);
+          named_bar_sync(kBarRead + 2 * c + h, kSumThreads + 32);
           tc_fence_after();
           tc_fence_before();
           if (lane == 0) {
-            if (rank == 0) mbar_arrive(&sempty[i & 1]);
-            else arrive_slot(slots + (i & 1) * sizeof(uint64_t));
+            if (rank == 0) mbar_arrive(&sempty[2 * c + h]);
+            else arrive_slot(slots + 2 * c * sizeof(uint64_t));
           }
+          __syncwarp();
         }
     }
   } else {
@@ -890,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         }
         const float sc = __shfl_sync(0xffffffffu, w0, b & 31) * ring.get(b);
         ring.fetch(b + kScaleAhead, b);
-        named_bar_sync(kBarFull + c, kSumThreads + 32);
+        named_bar_sync(kBarFull + 2 * c + half, kSumThreads + 32);
         tc_fence_after();
         const float2 s2 = make_float2(sc, sc);
 #pragma unroll
@@ -901,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
           tmem_wait_ld16x2(r, r1);
           if (h == 1) {
             tc_fence_before();
-            named_bar_arrive(kBarRead + c, kSumThreads + 32);
+            named_bar_arrive(kBarRead + 2 * c + half, kSumThreads + 32);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {

@@ -97,12 +97,12 @@ int launch_k9_rows(const void* x, int x_dtype, long long ldx, const float* xs, c
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch linear8_rows_kernel");
 }
 
-// A [rows, K] e4m3 matrix, read as bytes in boxes of 128 x 128.
-int encode_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t K) {
+// A [rows, K] e4m3 matrix, read as bytes in boxes of box_rows rows of 128 bytes.
+int encode_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows) {
   int st = get_encoder();
   if (st) return st;
   const cuuint64_t dims[2] = {K, rows}, strides[1] = {K};
-  const cuuint32_t box[2] = {128, k9::kTile}, es[2] = {1, 1};
+  const cuuint32_t box[2] = {128, box_rows}, es[2] = {1, 1};
   CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -124,7 +124,8 @@ int launch_k9(const void* x8, const float* xst, int ld_xs, const void* w8, const
   memset(&p, 0, sizeof(p));
   const long long pair_m = (M + 255) / 256, pair_tiles = pair_m * ((N + 255) / 256);
   const bool pairs_of_ctas = pair_tiles >= dev.sms && pair_tiles <= 0x7fffffffll;
-  if ((st = encode_bytes(&p.tm_x, x8, M, K)) || (st = encode_bytes(&p.tm_w, w8, N, K)))
+  if ((st = encode_bytes(&p.tm_x, x8, M, K, k9::kTile)) ||
+      (st = encode_bytes(&p.tm_w, w8, N, K, pairs_of_ctas ? k9::kTile / 2 : k9::kTile)))
     return st;
   p.xst = xst;
   p.ld_xs = ld_xs;
