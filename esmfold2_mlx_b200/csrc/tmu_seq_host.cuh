@@ -30,6 +30,7 @@ int check_heads(const void* p, long long st, long long sh, const char* what) {
 
 int check_packed(int T, int hq, int hkv, int D) {
   if (T < 0 || hq < 1 || hkv < 1 || D < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "T, heads and D must be positive");
+  if (T > 1 << 30) return fail(TMU_ERR_UNSUPPORTED, "T > 2^30");
   return TMU_OK;
 }
 
@@ -292,6 +293,7 @@ int tmu_attention(const tmu_attention_args* args, void* stream) {
   int st = check_packed(T, Hq, Hkv, D);
   if (st) return st;
   if (S < 0) return fail(TMU_ERR_INVALID_ARGUMENT, "S must not be negative");
+  if (!std::isfinite(scale)) return fail(TMU_ERR_INVALID_ARGUMENT, "scale must be finite");
   if (Hq % Hkv) return fail(TMU_ERR_INVALID_ARGUMENT, "Hq must be a multiple of Hkv");
   if (D % 8 || D > 128) return fail(TMU_ERR_UNSUPPORTED, "D must be a multiple of 8, at most 128");
   if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");

@@ -164,7 +164,7 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
         orow = _rows("out", out)
         to, ldo = orow.data_ptr(), _ld(orow)
     need = (_lib._lib or _lib.load()).tmu_linear_fp8_workspace_bytes(m, n, k)
-    ws = x.new_empty((need,), dtype=torch.uint8).data_ptr() if need else 0
+    ws = x.new_empty((need,), dtype=torch.uint8) if need else None  # held until the launch is in the stream
     launch(x.device, "tmu_linear_fp8", rows.data_ptr(), code, ld, xs, w8.data_ptr(), scales.data_ptr(), pointer(bias), to,
-           out_code, ldo, m, n, k, ws, need, pointer(status))
+           out_code, ldo, m, n, k, pointer(ws), need, pointer(status))
     return out

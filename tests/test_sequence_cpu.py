@@ -25,10 +25,10 @@ def heads(data=P, st=64, sh=64):
     return _lib.TmuHeads(data, st, sh)
 
 
-def attention(lib, q=None, k=None, v=None, o=None, cu=P, bias=None, S=1, T=4, hq=2, hkv=1, d=64, dtype=0):
+def attention(lib, q=None, k=None, v=None, o=None, cu=P, bias=None, S=1, T=4, hq=2, hkv=1, d=64, dtype=0, scale=0.125):
     h = heads()
     a = _lib.TmuAttentionArgs(q or h, k or h, v or h, o or h, cu, bias or _lib.TmuAttnBias(), S, T, hq, hkv, d, dtype, 0,
-                              0.125, None)
+                              scale, None)
     return lib.tmu_attention(ctypes.byref(a), None)
 
 
@@ -41,6 +41,10 @@ def test_attention_refusals(lib):
     assert attention(lib, d=136) == UNSUPPORTED
     assert attention(lib, dtype=_lib.TMU_F32) == UNSUPPORTED
     assert attention(lib, cu=None) == INVALID
+    assert attention(lib, scale=math.nan) == INVALID and attention(lib, scale=math.inf) == INVALID
+    assert attention(lib, T=(1 << 30) + 1) == UNSUPPORTED
+    assert attention(lib, q=heads(st=0)) == UNSUPPORTED and attention(lib, k=heads(st=0)) == UNSUPPORTED
+    assert attention(lib, hq=4, hkv=2, v=heads(sh=0)) == UNSUPPORTED
     for name in "qkvo":
         assert attention(lib, **{name: heads(None)}) == INVALID
         assert attention(lib, **{name: heads(P + 2)}) == MISALIGNED

@@ -153,14 +153,15 @@ def test_attention_bias_is_what_pair_cond_makes():
         assert_within(got, ref, tol)
 
 
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
-def test_attention_ignores_other_tokens(causal):
+def test_attention_ignores_other_tokens(causal, d):
     """NaN and infinities in other sequences and behind the last one reach nothing; rows of no
     sequence stay as they were."""
     for dtype in (FP16, BF16):
         lens = [130, 70, 200, 19]
-        q, k, v, cu = make_qkv(lens, 4, 2, 64, dtype, 8, extra=141)
-        ref, tol = attention_ref(q, k, v, lens, causal, 0.125)
+        q, k, v, cu = make_qkv(lens, 4, 2, d, dtype, 8, extra=141)
+        ref, tol = attention_ref(q, k, v, lens, causal, 1 / math.sqrt(d))
         for t in (q, k, v):
             t[419:] = float("nan")
             t[450:500] = float("inf")
@@ -175,18 +176,65 @@ def test_attention_ignores_other_tokens(causal):
         assert_within(out[200:419], ref[200:419], tol[200:419])
 
 
-def test_attention_causal_future_scores_do_not_count():
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_causal_future_scores_do_not_count(d):
     """Infinite and NaN keys and biases behind a causal row do not reach it."""
-    lens, d = [300], 64
+    lens = [300]
     q, k, v, cu = make_qkv(lens, 2, 2, d, FP16, 9)
     b = torch.randn(1, 2, 300, 300, generator=gen(10), device="cuda").half()
-    ref, tol = attention_ref(q, k, v, lens, True, 0.125, b)
+    ref, tol = attention_ref(q, k, v, lens, True, 1 / math.sqrt(d), b)
     b[:, :, :200, 200:] = float("nan")
     b[:, :, 100:150, 150:200] = float("inf")
     k[200:] = float("nan")
     got = att.attention(q, k, v, cu, causal=True, bias=b)
     assert_within(got[:150], ref[:150], tol[:150])
     assert got[200:].isnan().all()
+
+
+@pytest.mark.parametrize("d", [48, 64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_one_bad_score_spoils_its_row_only(bad, d):
+    """A single NaN or +inf score, at every place of a step and in its first and a later one, makes its
+    row NaN, as a softmax is, and no other."""
+    n = 280
+    q, k, v, cu = make_qkv([n], 1, 1, d, FP16, 51)
+    b = torch.zeros(1, 1, n, n, device="cuda", dtype=FP16)
+    rows = torch.arange(n, device="cuda")
+    hit = rows[::3]
+    b[0, 0, hit, (hit * 7 + 5) % n] = bad
+    got = att.attention(q, k, v, cu, bias=b)
+    assert got[hit].isnan().all()
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[hit] = False
+    ref, tol = attention_ref(q, k, v, [n], False, 1 / math.sqrt(d))
+    assert_within(got[keep], ref[keep], tol[keep])
+    q2 = q.clone()
+    q2[hit] = bad  # the same without a bias: a row whose scores are NaN or infinite
+    got = att.attention(q2, k, v, cu)
+    assert got[hit].isnan().all()
+    assert_within(got[keep], ref[keep], tol[keep])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-20, 3.0])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_scales(scale, d):
+    lens = [200, 131]
+    q, k, v, cu = make_qkv(lens, 2, 2, d, BF16, 52)
+    b = torch.randn(2, 2, 200, 200, generator=gen(53), device="cuda").to(BF16)
+    b[:, :, :, 7] = -math.inf
+    for bias in (None, b):
+        for causal in (False, True):
+            got = att.attention(q, k, v, cu, scale=scale, bias=bias, causal=causal)
+            assert_within(got, *attention_ref(q, k, v, lens, causal, scale, bias))
+
+
+def test_attention_many_short_and_empty_sequences():
+    """More sequences than one search step holds, empty ones among them."""
+    g = torch.Generator().manual_seed(54)
+    lens = [int(x) for x in torch.randint(0, 40, (1500,), generator=g)]
+    q, k, v, cu = make_qkv(lens, 2, 1, 64, FP16, 55)
+    for causal in (False, True):
+        assert_within(att.attention(q, k, v, cu, causal=causal), *attention_ref(q, k, v, lens, causal, 0.125))
 
 
 @pytest.mark.parametrize("dtype", [FP16, BF16])
