@@ -88,6 +88,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// 1 / sqrt(x) for normal x by the hardware's approximation (off by about 2^-22.9); x of 0 gives
+// infinity, and with eps = 0 a head of zeros a NaN, as the division does.
+__device__ __forceinline__ float rsqrt_near(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <int LPH>
 __device__ __forceinline__ float head_sum(float x) {
 #pragma unroll
@@ -114,11 +122,11 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
   griddep_wait();
 
   // cos, sin of the lane's four pairs
-  float cs[4], sn[4];
+  float cs[4], sn[4], ns[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     cs[e] = 1.f;
-    sn[e] = 0.f;
+    sn[e] = ns[e] = 0.f;
   }
   if (turned) {
     const long long pos = p.pos64 ? static_cast<const long long*>(p.pos)[t] : static_cast<const int*>(p.pos)[t];
@@ -128,6 +136,7 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
       sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 0x1p-31f, &sn[e], &cs[e]);
       cs[e] *= p.gain;
       sn[e] *= p.gain;
+      ns[e] = -sn[e];
     }
   }
 
@@ -143,23 +152,28 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
         bb[v] = b != nullptr && act ? __ldg(reinterpret_cast<const float2*>(b + at)) : make_float2(0.f, 0.f);
       }
     }
-    const T* src = static_cast<const T*>(in.p) + t * in.st;
-    T* dst = static_cast<T*>(out.p) + t * out.st;
-    for (int k0 = begin; k0 < end; k0 += kBatch) {
+    // the lane's first value of head begin * HPW + sub; a turn further is `ahead` bytes on
+    const int d01 = (d1 - d0) * 2;
+    const int h0 = begin * HPW + sub;
+    const char* src = reinterpret_cast<const char*>(static_cast<const T*>(in.p) + t * in.st + h0 * in.sh + d0);
+    char* dst = reinterpret_cast<char*>(static_cast<T*>(out.p) + t * out.st + h0 * out.sh + d0);
+    const long long src_ahead = 2ll * HPW * in.sh, dst_ahead = 2ll * HPW * out.sh;
+    // turns in which this lane has a head
+    const int mine = act ? min(end - begin, (heads - h0 + HPW - 1) / HPW) : 0;
+    for (int k0 = 0; k0 < end - begin; k0 += kBatch) {
       uint2 raw[kBatch][2];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int h = (k0 + i) * HPW + sub;
         raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
-        if (act && k0 + i < end && h < heads) {
-          raw[i][0] = *reinterpret_cast<const uint2*>(src + h * in.sh + d0);
-          raw[i][1] = *reinterpret_cast<const uint2*>(src + h * in.sh + d1);
+        if (k0 + i < mine) {
+          raw[i][0] = *reinterpret_cast<const uint2*>(src);
+          raw[i][1] = *reinterpret_cast<const uint2*>(src + d01);
         }
+        src += src_ahead;
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (k0 + i >= end) break;
-        const int h = (k0 + i) * HPW + sub;
+        if (k0 + i >= end - begin) break;
         float2 y[4] = {unpack2(raw[i][0].x, T()), unpack2(raw[i][0].y, T()), unpack2(raw[i][1].x, T()),
                        unpack2(raw[i][1].y, T())};
         if (NORM == kLayer) {
@@ -173,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
           float2 s2 = __fmul2_rn(y[0], y[0]);
 #pragma unroll
           for (int v = 1; v < 4; ++v) s2 = __ffma2_rn(y[v], y[v], s2);
-          const float r = rsqrtf(fmaf(head_sum<LPH>(s2.x + s2.y), p.inv_d, p.eps));
+          const float r = rsqrt_near(fmaf(head_sum<LPH>(s2.x + s2.y), p.inv_d, p.eps));
 #pragma unroll
           for (int v = 0; v < 4; ++v) y[v] = __ffma2_rn(__fmul2_rn(y[v], make_float2(r, r)), ww[v], bb[v]);
         }
@@ -187,16 +201,16 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
             for (int v = 0; v < 2; ++v) {
               const float2 cc = make_float2(cs[2 * v], cs[2 * v + 1]), ss = make_float2(sn[2 * v], sn[2 * v + 1]);
               const float2 a = y[v], o = y[v + 2];
-              y[v] = __ffma2_rn(a, cc, __fmul2_rn(o, make_float2(-ss.x, -ss.y)));
+              y[v] = __ffma2_rn(a, cc, __fmul2_rn(o, make_float2(ns[2 * v], ns[2 * v + 1])));
               y[v + 2] = __ffma2_rn(o, cc, __fmul2_rn(a, ss));
             }
           }
         }
-        if (act && h < heads) {
-          T* to = dst + h * out.sh;
-          *reinterpret_cast<uint2*>(to + d0) = make_uint2(pack2(y[0].x, y[0].y, T()), pack2(y[1].x, y[1].y, T()));
-          *reinterpret_cast<uint2*>(to + d1) = make_uint2(pack2(y[2].x, y[2].y, T()), pack2(y[3].x, y[3].y, T()));
+        if (k0 + i < mine) {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(y[0].x, y[0].y, T()), pack2(y[1].x, y[1].y, T()));
+          *reinterpret_cast<uint2*>(dst + d01) = make_uint2(pack2(y[2].x, y[2].y, T()), pack2(y[3].x, y[3].y, T()));
         }
+        dst += dst_ahead;
       }
     }
   };
