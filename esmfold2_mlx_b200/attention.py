@@ -188,8 +188,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
                1 if rotary.layout == "interleaved" else 0)
     if q_out is not None or k_out is not None:
         _check_rope_outputs(q, k, q_out, k_out)
-    q_out = q.new_empty((T, hq, D)) if q_out is None else q_out
-    k_out = q.new_empty((T, hk, D)) if k_out is None else k_out
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
     args = _lib.QK_NORM_ROPE_ARGS.pack(qp, qt, qh, kp, kt, kh, *_view("q_out", q_out, T, D, q)[:3],
                                        *_view("k_out", k_out, T, D, q)[:3], kind, eps, pointer(q_weight), pointer(q_bias),
                                        pointer(k_weight), pointer(k_bias), *rot, T, hq, hk, D, dtype)
@@ -283,7 +283,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
             raise ValueError("the last axis of bias must be contiguous")
         b = (bias.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1], stride[2], n)
     if out is None:
-        out = q.new_empty((T, hq, D))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         if out.shape != q.shape:
             raise ValueError("out must be shaped like q")

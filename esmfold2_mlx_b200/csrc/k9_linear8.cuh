@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
     }
   }
   // linear8_rows_kernel reads w8 before its dependency wait, so nothing that could be a weight may
-  // be announced before it is visible
+  // be announced before it is visible.  (Announced at the start, the products' blocks come while
+  // these still run, two on some SMs and none on others: 13.4 -> 16 us at 1283 x 1000 x 1360.)
   if (p.chained) griddep_trigger();
 }
 
