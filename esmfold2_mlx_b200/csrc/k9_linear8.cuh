@@ -18,7 +18,7 @@
 namespace tmu {
 namespace k9 {
 
-constexpr int kQuantThreads = 256, kQuantUnroll = 4;
+constexpr int kQuantThreads = 256, kQuantRows = kQuantThreads / 8;
 
 struct QuantParams {
   const void* x;
@@ -53,17 +53,19 @@ __device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b, __nv_bfloat1
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// 8 values a lane, 16 lanes a block of 128 (all of the warp takes part): the block's scale and the
-// lane's e4m3.  A quotient a / b is rounded correctly from the correctly rounded r = 1 / b: q = a r, then
+// C runs of 8 values a lane, 16 / C lanes a block of 128 (all of the warp takes part): the block's
+// scale and the lane's e4m3.  A quotient a / b is rounded correctly from the correctly rounded r = 1 / b: q = a r, then
 // q + (a - q b) r with fused multiply-adds (Markstein 1990; right but for divisors whose significand
 // is all ones: 448 = 7 * 2^6 is none, nor is an 8 or 11-bit number over it, whose 24 bits repeat
 // with the period 3 of sevenths).  The remainder must not underflow, which the scale's lower limit
 // sees to for itself (a quotient below 2^-126 is replaced) and a power of two for the values.
-template <typename T>
-__device__ __forceinline__ void quantize8(const uint32_t (&u)[4], float& s, uint2& o) {
-  uint32_t m = absmax2(absmax2(u[0], u[1], T()), absmax2(u[2], u[3], T()), T());
+template <typename T, int C>
+__device__ __forceinline__ void quantize(const uint4 (&raw)[C], float& s, uint2 (&o)[C]) {
+  uint32_t m = 0u;
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, d), T());
+  for (int i = 0; i < C; ++i) m = absmax2(m, absmax2(absmax2(raw[i].x, raw[i].y, T()), absmax2(raw[i].z, raw[i].w, T()), T()), T());
+#pragma unroll
+  for (int d = 8 / C; d > 0; d >>= 1) m = absmax2(m, __shfl_xor_sync(0xffffffffu, m, d), T());
   const float2 pair = k8::unpack2(m, T());
   const float amax = max_nan(pair.x, pair.y);
   constexpr float r448 = 1.f / 448.f;
@@ -72,47 +74,54 @@ __device__ __forceinline__ void quantize8(const uint32_t (&u)[4], float& s, uint
   const float up = s < 0x1p-60f ? 0x1p66f : 1.f;
   const float t = s * up, r = __frcp_rn(t);
   const float2 r2 = make_float2(r, r), nt2 = make_float2(-t, -t);
-  uint32_t w[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float2 a = k8::unpack2(u[e], T());
-    if (up != 1.f) a = make_float2(a.x * up, a.y * up);
-    const float2 q = __fmul2_rn(a, r2);
-    const float2 v = __ffma2_rn(__ffma2_rn(q, nt2, a), r2, q);
-    w[e] = e4m3x2(v.x, v.y);
+  for (int i = 0; i < C; ++i) {
+    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float2 a = k8::unpack2(u[e], T());
+      if (up != 1.f) a = make_float2(a.x * up, a.y * up);
+      const float2 q = __fmul2_rn(a, r2);
+      const float2 v = __ffma2_rn(__ffma2_rn(q, nt2, a), r2, q);
+      w[e] = e4m3x2(v.x, v.y);
+    }
+    o[i] = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
   }
-  o = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
 }
 
-// Half a warp takes U blocks of 128 of one row (8 values, 16 bytes, a lane and block), all loaded
-// before the first is worked on, and a block of threads sixteen rows, so that the scales of a
-// block of 128, transposed for the tensor-core kernels, are written 64 bytes at a time.
-// Bound: HBM (2 bytes read and 1 written a value).
+// Eight lanes take U blocks of 128 of one row (16 values a lane and block), all loaded before the
+// first is worked on, and a block of threads 32 rows, so that the scales of a block of 128, transposed
+// for the tensor-core kernels, are written 128 bytes at a time.
+// Bound: HBM, 2 bytes read and 1 written a value: 82 us at 16384 x 10240, 6.2 TB/s.  (With 16 lanes a
+// block, and so twice the scales' arithmetic, the instructions bound it: 97 us, 84 % of the issue slots.)
 template <typename T, int U>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantParams p) {
-  const int l = threadIdx.x & 15;
+  const int l = threadIdx.x & 7;
   const int per = (p.kb + U - 1) / U;
   const int rows = blockIdx.x / per;
-  const int m = rows * (kQuantThreads / 16) + (threadIdx.x >> 4), b0 = (blockIdx.x - rows * per) * U;
+  const int m = rows * kQuantRows + (threadIdx.x >> 3), b0 = (blockIdx.x - rows * per) * U;
   griddep_wait();
-  uint4 raw[U];
+  uint4 raw[U][2];
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int k = (b0 + i) * 128 + l * 8;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (m < p.M && k < p.K) raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.ld + k);
-  }
+  for (int i = 0; i < U; ++i)
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    const int k = (b0 + i) * 128 + l * 8;
-    uint2 o;
-    float s;
-    quantize8<T>(u, s, o);
-    if (m < p.M && k < p.K) {
-      *reinterpret_cast<uint2*>(p.x8 + static_cast<long long>(m) * p.K + k) = o;
-      if (l == 0) p.xs[m * p.xs_m + (b0 + i) * p.xs_b] = s;
+    for (int c = 0; c < 2; ++c) {
+      const int k = (b0 + i) * 128 + c * 64 + l * 8;
+      raw[i][c] = make_uint4(0u, 0u, 0u, 0u);
+      if (m < p.M && k < p.K) raw[i][c] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + m * p.ld + k);
     }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    uint2 o[2];
+    float s;
+    quantize<T, 2>(raw[i], s, o);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int k = (b0 + i) * 128 + c * 64 + l * 8;
+      if (m < p.M && k < p.K) *reinterpret_cast<uint2*>(p.x8 + static_cast<long long>(m) * p.K + k) = o[c];
+    }
+    if (m < p.M && b0 + i < p.kb && l == 0) p.xs[m * p.xs_m + (b0 + i) * p.xs_b] = s;
   }
   // linear8_rows_kernel reads w8 before its dependency wait, so nothing that could be a weight may
   // be announced before it is visible.  (Announced at the start, the products' blocks come while
@@ -249,13 +258,13 @@ __global__ void __launch_bounds__(kRowsThreads, PAIRS == 1 ? 4 : PAIRS == 4 ? 3 
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
       if (2 * i >= p.M) break;
-      uint2 o = make_uint2(xcur[i].x, xcur[i].y);
+      uint2 o[1] = {make_uint2(xcur[i].x, xcur[i].y)};
       float s = scur[i];
       if constexpr (sizeof(X) != 1) {
-        const uint32_t u[4] = {xcur[i].x, xcur[i].y, xcur[i].z, xcur[i].w};
-        quantize8<X>(u, s, o);
+        const uint4 raw[1] = {xcur[i]};
+        quantize<X, 1>(raw, s, o);
       }
-      *reinterpret_cast<uint2*>(&xq[warp][2 * i + (lane >> 4)][l * 8]) = o;
+      *reinterpret_cast<uint2*>(&xq[warp][2 * i + (lane >> 4)][l * 8]) = o[0];
       if (l == 0) xsc[warp][2 * i + (lane >> 4)] = s;
     }
     __syncwarp();

@@ -202,14 +202,14 @@ int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8
   p.xs_m = xs_m;
   p.xs_b = xs_b;
   p.chained = chained;
-  // four blocks of 128 a half-warp once that still gives every SM eight blocks of threads
-  const long long groups = (M + 15) / 16;
-  const bool four = groups * ((p.kb + 3) / 4) >= 8ll * dev.sms;
-  const long long grid = groups * (four ? (p.kb + 3) / 4 : p.kb);
+  // two blocks of 128 at a time once that still gives every SM eight blocks of threads
+  const long long groups = (M + k9::kQuantRows - 1) / k9::kQuantRows;
+  const bool two = groups * ((p.kb + 1) / 2) >= 8ll * dev.sms;
+  const long long grid = groups * (two ? (p.kb + 1) / 2 : p.kb);
   if (grid > 0x7fffffffll) return fail(TMU_ERR_UNSUPPORTED, "M and K are too large");
   void (*kern)(k9::QuantParams) =
-      dtype == TMU_F16 ? (four ? k9::quantize_kernel<__half, 4> : k9::quantize_kernel<__half, 1>)
-                       : (four ? k9::quantize_kernel<__nv_bfloat16, 4> : k9::quantize_kernel<__nv_bfloat16, 1>);
+      dtype == TMU_F16 ? (two ? k9::quantize_kernel<__half, 2> : k9::quantize_kernel<__half, 1>)
+                       : (two ? k9::quantize_kernel<__nv_bfloat16, 2> : k9::quantize_kernel<__nv_bfloat16, 1>);
   cudaError_t e = launch_pdl(kern, static_cast<int>(grid), k9::kQuantThreads, 0, stream, p);
   return e == cudaSuccess ? TMU_OK : cuda_fail(e, "launch quantize_kernel");
 }
