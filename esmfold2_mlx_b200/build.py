@@ -3,8 +3,8 @@
     python -m esmfold2_mlx_b200.build [--force]
 
 One translation unit (``csrc/tmu_capi.cu``) includes every kernel header in ``csrc/`` (the tri-mul
-kernels K1-K3 and their c_z = 256 forms, the transition K4, the distogram K5, the GEMM K6 and the
-row LayerNorm pass); the result is a plain C-ABI shared library (``include/tmu.h``) with the CUDA
+kernels K1-K3 and their c_z = 256 forms, the transition K4, the distogram K5, the GEMM K6, the
+row LayerNorm pass, and the sequence operators K7-K9); the result is a plain C-ABI shared library (``include/tmu.h``) with the CUDA
 runtime linked statically.
 """
 
