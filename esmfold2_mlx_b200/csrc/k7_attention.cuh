@@ -19,9 +19,9 @@
 //   D > 64   one block an SM, of two tiles A and B of one sequence that share their keys and values,
 //            which two blocks would not find room for
 // (A row's softmax spread over two threads was no faster at D = 64 and 8 % slower at 128.)
-// Warps of a block: the softmax, a thread a row (warp w: tile w / 4, TMEM lanes 32 (w % 4) ..), then one for TMA (Q, then K and V through rings of kStages tiles), one
-// for TMEM and the MMAs, and two idle ones that complete the warpgroup which gives its registers to
-// the softmax.
+// Warps of a block: the softmax, a thread a row (warp w: tile w / 4, TMEM lanes 32 (w % 4) ..), then one
+// for TMA (Q, then K and V through rings of kStages tiles), one for TMEM and the MMAs, and two idle
+// ones that complete the warpgroup which gives its registers to the softmax.
 // TMEM columns: D <= 64: O 64, S 128, P 64: S has its own columns, so the next S is made while the
 // softmax works on this one.  D > 64: O 2 x 128, S 2 x 128, and P overwrites S; the MMAs of a block
 // execute in issue order, so S of step j + 1 follows the P V that reads them.
@@ -75,7 +75,7 @@ struct Cfg {
   static constexpr int OFF_V = OFF_K + kStages * kTileBytes;
   // A quarter of the exponentials on the FMA units, where two of the special function unit's 16 a
   // cycle and SM are as long as the products (a half as long at D > 64): 108 -> 100 us at 4096 tokens,
-  // 18 heads of 64; 128 heads' values: 629 -> 643 us of the causal prompts.
+  // 18 heads of 64.  At D = 128 it does not pay: the causal prompts took 643 us with it and 629 without.
   static constexpr bool kMixedExp = DP == 64;
   // Bias of a warp's 32 rows: a step's 128 keys, or as many as fit beside the tiles.  The rows' 16-byte
   // accesses of eight rows meet 8 different bank groups by a swizzle (128 keys: no room for more than
@@ -429,6 +429,11 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
         BIAS && p.bias_width == 2 ? (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(bbase + row * p.bias_sr) >> 1) & 1u) * 16u : 0u;
     const bool shifted = BIAS && __any_sync(0xffffffffu, bshift != 0u);
     const float2 c2 = make_float2(flip ? -c : c, flip ? -c : c);
+    // bf16's lowest value times log2 e is past fp32's range: with a bf16 bias the maximum is kept in x's
+    // own units and subtracted before the factor, so a row that is masked by nothing but lowest values
+    // still sees its keys evenly.  (fp16 values are far from it, and take the factor in one operation.)
+    constexpr bool kUnits = BIAS && !__is_same(T, __half);
+    constexpr float kMove = kUnits ? kMoveMax / kLog2e : kMoveMax;
     if (BIAS && nx > 0) fetch_bias(0);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -517,16 +522,16 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
         for (int e = 4; e < kTile; ++e) mx[e & 3] = fmaxf(mx[e & 3], v[e]);
         part = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       }
-      const float top = part * mul;
+      const float top = kUnits ? part : part * mul;
       if (j > 0 && C::kOwnP) {  // P's columns and O belong to P V of the last step (else S's being there says so)
         if (!(ok = warp_poll(&ofull[x], (j - 1) & 1, ctx, kSiteSoftO))) break;
         tc_fence_after();
       }
-      const bool move = top > m + kMoveMax || (m == -INFINITY && top > m);
+      const bool move = top > m + kMove || (m == -INFINITY && top > m);
       if (j == 0) {
         m = fmaxf(m, top);
       } else if (__any_sync(0xffffffffu, move)) {
-        const float f = move ? ex2_approx(m - top) : 1.f;
+        const float f = move ? ex2_approx(kUnits ? (m - top) * kLog2e : m - top) : 1.f;
         if (move) m = top;
         l *= f;
 #pragma unroll 1
@@ -547,8 +552,8 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 t = __ffma2_rn(make_float2(v[b * 32 + 2 * e], v[b * 32 + 2 * e + 1]), make_float2(mul, mul),
-                                      make_float2(neg, neg));
+          const float2 x2 = make_float2(v[b * 32 + 2 * e], v[b * 32 + 2 * e + 1]), n2 = make_float2(neg, neg);
+          const float2 t = kUnits ? __fmul2_rn(__fadd2_rn(x2, n2), make_float2(mul, mul)) : __ffma2_rn(x2, make_float2(mul, mul), n2);
           const float2 q = C::kMixedExp && (e & 3) == 3 ? exp2_fma(t) : make_float2(ex2_approx(t.x), ex2_approx(t.y));
           sum = __fadd2_rn(sum, q);
           w[e] = k8::pack2(q.x, q.y, T());

@@ -131,6 +131,37 @@ def test_attention_bias(lens, h, d, shared, causal, dtype):
         assert (got[5, 0] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("n,d", [(40, 64), (300, 48), (300, 128)])
+def test_attention_masks_of_the_lowest_value(n, d, causal, dtype):
+    """Keys masked by the type's lowest value.  The queries are 0, so a row is the mean of the keys it
+    sees best: those at 0, or, where there are none, those at the lowest value (-inf hides for good).
+
+    The weights are equal before they are rounded to q's type (u) and their exponentials off by 2^-16
+    at most; the sums of v and of the weights add 2 n 2^-24, and the output is rounded once."""
+    _, k, v, cu = make_qkv([n], 1, 1, d, dtype, 60)
+    q = torch.zeros_like(k)
+    low = torch.finfo(dtype).min
+    b = torch.zeros(1, 1, n, n, device="cuda", dtype=dtype)
+    b[0, 0, :, n // 2:] = low          # padding behind
+    b[0, 0, 5:30, :n // 2] = low       # with that, rows of nothing but the lowest value
+    b[0, 0, 20:25, ::3] = -math.inf    # with hidden keys among it
+    b[0, 0, n // 2:, :] = low
+    b[0, 0, n - 9:, n - 20:n - 3] = 0  # a later step's keys beat the first's
+    got = att.attention(q, k, v, cu, causal=causal, bias=b)
+    x = b[0, 0].double()
+    if causal:
+        x = x.masked_fill(torch.ones(n, n, device="cuda", dtype=torch.bool).triu(1), -math.inf)
+    top = x.amax(-1, keepdim=True)
+    p = ((x == top) & (top > -math.inf)).double()
+    p = p / p.sum(-1, keepdim=True).clamp(min=1)
+    vv = v[:, 0].double()
+    ref, a = p @ vv, p @ vv.abs()
+    assert_within(got[:, 0], ref, half_step(dtype) * ref.abs()
+                  + a * (half_step(dtype) + 2.0 ** -15 + (2 * n + 16) * 2.0 ** -24) + least(dtype))
+
+
 def test_attention_bias_views():
     """A bias with odd row pitch, a shorter one than the sequence, and one broadcast over heads."""
     lens, h, d = [150, 90], 4, 64
