@@ -56,6 +56,13 @@ def refuse_grad(where: str, *tensors) -> None:
                 raise ValueError(f"{where} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
+def check_status_block(status: torch.Tensor | None, device: torch.device) -> None:
+    """Raise unless ``status`` is None or a block as ``ops.new_status`` makes it."""
+    if status is not None and (status.dtype is not torch.uint8 or status.numel() < _lib.TMU_STATUS_BYTES
+                               or status.device != device or not status.is_contiguous() or status.data_ptr() % 16):
+        raise ValueError("status must be ops.new_status of the tensors' device")
+
+
 def spans_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the address ranges that two strided tensors reach over meet."""
     if a.numel() == 0 or b.numel() == 0:
@@ -240,7 +247,7 @@ def _heads_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
     step = a.stride(0) * a.element_size()
     wa, wb = token_span(a), token_span(b)
-    if a.shape[0] > 1 and a.stride(0) == b.stride(0) and step >= max(wa, wb):
+    if a.shape[0] > 1 and step == b.stride(0) * b.element_size() and step >= max(wa, wb):
         off = (b.data_ptr() - a.data_ptr()) % step  # b's heads begin `off` bytes behind a's in each period
         return off < wa or off + wb > step
     return True
@@ -257,9 +264,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     scores of each sequence's first n positions (``pair_cond.pair_biases(...)[block]`` with a sequence a
     fold, or with one fold's bias for all of its samples); -inf hides a key, and a row whose keys are
     all hidden comes out as 0.  D is a multiple of 8, at most 128.  Tokens past the last sequence are
-    left as they were in ``out`` (unset in a new one).  A hidden key's value is multiplied by a weight
-    of 0, so an infinity or NaN there still reaches the rows of its own sequence; other sequences and
-    tokens of no sequence have no influence."""
+    left as they were in ``out`` (unset in a new one).  -inf is added to a hidden key's score, and its value
+    is multiplied by a weight of 0, so an infinity or NaN there still reaches the rows of its own
+    sequence; other sequences and tokens of no sequence have no influence."""
     dtype = _check_first("q", q)
     T, hq, D = q.shape
     qp, qt, qh, _ = _view("q", q, T, D, q)
@@ -268,6 +275,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     if hv != hk:
         raise ValueError("k and v must have the same heads")
     refuse_grad("attention", q, k, v, bias)
+    if status is not None:
+        check_status_block(status, q.device)
     if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.device != q.device
             or not cu_seqlens.is_contiguous() or cu_seqlens.shape[0] < 1):
         raise ValueError("cu_seqlens must be a contiguous int32 [S + 1] tensor on q's device")

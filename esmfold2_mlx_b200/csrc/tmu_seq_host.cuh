@@ -115,8 +115,8 @@ size_t k9_scale_bytes(int M, int K) {
   return static_cast<size_t>((M + 255) / 256) * 256 * ((K + 127) / 128) * 4;
 }
 
-int launch_k9(const void* x8, const float* xst, int ld_xs, const void* w8, const float* ws, const float* bias, void* out, int out_dtype,
-              long long ldo, int M, int N, int K, DeviceStatus* status, cudaStream_t stream) {
+int launch_k9(const void* x8, const float* xst, int ld_xs, const void* w8, const float* ws, const float* bias, void* out,
+              int out_dtype, long long ldo, int M, int N, int K, DeviceStatus* status, cudaStream_t stream) {
   Dev dev;
   int st = seq_device(dev, 8, reinterpret_cast<const void*>(&k9::linear8_kernel), k9::SMEM_BYTES);
   if (!st) st = seq_device(dev, 9, reinterpret_cast<const void*>(&k9::pair::linear8_pair_kernel), k9::pair::SMEM_BYTES);
@@ -181,6 +181,7 @@ int launch_k9(const void* x8, const float* xst, int ld_xs, const void* w8, const
 int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, long long xs_m,
                   long long xs_b, bool chained, cudaStream_t stream) {
   if (M < 0 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, K positive");
+  if (M > 1 << 30 || K > 1 << 30) return fail(TMU_ERR_UNSUPPORTED, "M or K > 2^30");
   if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
   if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
   if (M == 0) return TMU_OK;
@@ -354,7 +355,7 @@ int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void
 }
 
 size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
-  if (M <= k9::kRowsMax || N < 1 || K < 1) return 0;
+  if (M <= k9::kRowsMax || M > 1 << 30 || N < 1 || K < 1 || K > 1 << 30) return 0;
   return k9_scale_bytes(M, K) + static_cast<size_t>(M) * K;
 }
 
@@ -362,6 +363,7 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
                    const float* bias, void* out, int out_dtype, long long ldo, int M, int N, int K, void* workspace,
                    size_t workspace_bytes, void* status, void* stream) {
   if (M < 0 || N < 1 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, N and K positive");
+  if (M > 1 << 30 || N > 1 << 30 || K > 1 << 30) return fail(TMU_ERR_UNSUPPORTED, "M, N or K > 2^30");
   if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
   if (x_dtype != TMU_F16 && x_dtype != TMU_BF16 && x_dtype != TMU_E4M3) return fail(TMU_ERR_UNSUPPORTED, "x must be fp16, bf16 or e4m3");
   if (out_dtype != TMU_F16 && out_dtype != TMU_BF16 && out_dtype != TMU_F32) return fail(TMU_ERR_UNSUPPORTED, "out must be fp16, bf16 or fp32");

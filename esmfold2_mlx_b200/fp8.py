@@ -20,11 +20,12 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .attention import launch, pointer, refuse_grad, spans_overlap
+from .attention import _heads_overlap, check_status_block, launch, pointer, refuse_grad, spans_overlap
 
 BLOCK = 128
 F8_MAX = 448.0          # the largest e4m3 value
 SCALE_MIN = 2.0 ** -126  # the least scale: an all-zero block keeps a usable quotient
+ROWS_MAX = 2 ** 30       # rows of x, and of a weight
 
 _IN = {torch.float16: _lib.TMU_F16, torch.bfloat16: _lib.TMU_BF16, torch.float8_e4m3fn: _lib.TMU_E4M3}
 _OUT = {torch.float16: _lib.TMU_F16, torch.bfloat16: _lib.TMU_BF16, torch.float32: _lib.TMU_F32}
@@ -45,8 +46,8 @@ class BlockWeight:
         w, s = self.w8, self.scales
         if w.dtype != torch.float8_e4m3fn or w.dim() != 2 or not w.is_contiguous():
             raise ValueError("w8 must be a contiguous float8_e4m3fn [N, K] tensor")
-        if w.shape[0] < 1 or w.shape[1] < 1 or w.shape[1] % 16:
-            raise ValueError("K must be a positive multiple of 16, N positive")
+        if not 1 <= w.shape[0] <= ROWS_MAX or w.shape[1] < 1 or w.shape[1] % 16:
+            raise ValueError(f"K must be a positive multiple of 16, N positive and at most {ROWS_MAX}")
         shape = (_blocks(w.shape[0]), _blocks(w.shape[1]))
         if s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous() or s.device != w.device:
             raise ValueError(f"scales must be a contiguous fp32 {list(shape)} tensor on w8's device")
@@ -106,6 +107,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     refuse_grad("quantize_rows", x)
     x = _rows("x", x)
     m, k = x.shape
+    if m > ROWS_MAX:
+        raise ValueError(f"x has {m} rows, more than {ROWS_MAX}")
     x8 = torch.empty(m, k, dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty(m, _blocks(k), dtype=torch.float32, device=x.device)
     launch(x.device, "tmu_quantize_rows", x.data_ptr(), _IN[x.dtype], _ld(x), m, k, x8.data_ptr(), scales.data_ptr())
@@ -130,8 +133,12 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
     if w8.device != x.device:
         raise ValueError("the weight must be on x's device")
     refuse_grad("fp8.linear", x, bias)
+    if status is not None:
+        check_status_block(status, x.device)
     rows = _rows("x", x)
     m, ld = rows.shape[0], _ld(rows)
+    if m > ROWS_MAX:
+        raise ValueError(f"x has {m} rows, more than {ROWS_MAX}")
     xs = 0
     if code == _lib.TMU_E4M3:
         want = (*shape[:-1], _blocks(k))
@@ -159,9 +166,11 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
             raise ValueError(f"out must be an fp16, bf16 or fp32 {[*shape[:-1], n]} tensor on x's device")
         if out_dtype not in (None, out.dtype):
             raise ValueError("out_dtype differs from out's type")
-        if any(t is not None and spans_overlap(out, t) for t in (x, w8, scales, bias, x_scales)):
-            raise ValueError("out must not overlap an input")
         orow = _rows("out", out)
+        # (out may be columns beside x's in one buffer)
+        if (_heads_overlap(orow.unsqueeze(1), rows.unsqueeze(1))
+                or any(t is not None and spans_overlap(out, t) for t in (w8, scales, bias, x_scales))):
+            raise ValueError("out must not overlap an input")
         to, ldo = orow.data_ptr(), _ld(orow)
     need = (_lib._lib or _lib.load()).tmu_linear_fp8_workspace_bytes(m, n, k)
     ws = x.new_empty((need,), dtype=torch.uint8) if need else None  # held until the launch is in the stream

@@ -130,6 +130,35 @@ def test_linear_refusals(lib):
     assert lib.tmu_quantize_rows(P, 2, 48, 2, 48, P, P, None) == UNSUPPORTED
 
 
+def test_sizes_past_the_index_range(lib):
+    big = (1 << 30) + 1
+    assert linear(lib, M=big) == UNSUPPORTED and linear(lib, N=big, ldo=1 << 31) == UNSUPPORTED
+    assert linear(lib, K=(1 << 30) + 16, ldx=1 << 31) == UNSUPPORTED
+    assert lib.tmu_quantize_rows(P, 0, 64, big, 64, P, P, None) == UNSUPPORTED
+    assert lib.tmu_linear_fp8_workspace_bytes(big, 8, 64) == 0
+
+
+def test_status_block():
+    dev = torch.device("cpu")
+    att.check_status_block(None, dev)
+    att.check_status_block(torch.zeros(_lib.TMU_STATUS_BYTES, dtype=torch.uint8), dev)
+    for bad in (torch.zeros(_lib.TMU_STATUS_BYTES - 1, dtype=torch.uint8), torch.zeros(_lib.TMU_STATUS_BYTES),
+                torch.zeros(2 * _lib.TMU_STATUS_BYTES, dtype=torch.uint8)[::2],
+                torch.zeros(2 * _lib.TMU_STATUS_BYTES, dtype=torch.uint8)[8:]):
+        with pytest.raises(ValueError):
+            att.check_status_block(bad, dev)
+
+
+def test_rows_beside_one_another():
+    """Columns of one buffer, of one type or two, do not overlap; rows that meet do."""
+    buf = torch.zeros(10, 48, dtype=torch.float32)
+    x, y = buf[:, :16].unsqueeze(1), buf[:, 16:].unsqueeze(1)
+    assert not att._heads_overlap(y, x) and att._heads_overlap(buf[:, 15:].unsqueeze(1), x)
+    half = buf.view(torch.float16)[:, :32].unsqueeze(1)
+    assert not att._heads_overlap(y, half) and att._heads_overlap(x, half)
+    assert att._heads_overlap(buf[:, :17].unsqueeze(1), y)
+
+
 def test_python_refusals():
     x = torch.zeros(4, 2, 64, dtype=torch.float16)
     with pytest.raises(TypeError):

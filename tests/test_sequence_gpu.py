@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from esmfold2_mlx_b200 import attention as att
-from esmfold2_mlx_b200 import fp8
+from esmfold2_mlx_b200 import fp8, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -517,6 +517,20 @@ def test_linear_views_and_shapes():
     assert fp8.linear(x[:0], w).shape == (0, 5, 200)
 
 
+@pytest.mark.parametrize("m", [5, 30])
+def test_linear_beside_its_input(m):
+    """x and out as columns of one buffer."""
+    g = gen(34)
+    w = fp8.quantize_weight(torch.randn(200, 256, generator=g, device="cuda"))
+    buf = torch.randn(m, 456, generator=g, device="cuda").half()
+    x = buf[:, :256].clone()
+    want = fp8.linear(x, w)
+    fp8.linear(buf[:, :256], w, out=buf[:, 256:])
+    assert torch.equal(buf[:, 256:], want) and torch.equal(buf[:, :256], x)
+    with pytest.raises(ValueError):
+        fp8.linear(buf[:, :256], w, out=buf[:, 255:455])
+
+
 def test_linear_non_finite_rows_stay_apart():
     g = gen(33)
     for m in (4, 200):
@@ -608,6 +622,24 @@ def test_layer_captured_and_on_other_streams():
         eager = layer(*st)
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][1], want2) and torch.equal(graphs[1][1], want2) and torch.equal(eager, want2)
+
+
+def test_status_blocks():
+    """A caller's status block stays clean over good calls, and a wrong one is refused."""
+    q, k, v, cu = make_qkv([300, 20], 2, 2, 64, FP16, 61)
+    status = ops.new_status(q.device)
+    o = att.attention(q, k, v, cu, status=status)
+    assert torch.equal(o, att.attention(q, k, v, cu))
+    w = fp8.quantize_weight(torch.randn(4100, 256))
+    for m in (3, 200, 2500):
+        x = torch.randn(m, 256, generator=gen(62), device="cuda").half()
+        assert torch.equal(fp8.linear(x, w, status=status), fp8.linear(x, w))
+    ops.check_status(status, "sequence operators")
+    for bad in (status.cpu(), status[:64], status.float()):
+        with pytest.raises(ValueError):
+            att.attention(q, k, v, cu, status=bad)
+        with pytest.raises(ValueError):
+            fp8.linear(x, w, status=bad)
 
 
 # ---- refusals that need CUDA tensors ----------------------------------------------------------
