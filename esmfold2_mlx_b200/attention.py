@@ -264,9 +264,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     scores of each sequence's first n positions (``pair_cond.pair_biases(...)[block]`` with a sequence a
     fold, or with one fold's bias for all of its samples); -inf hides a key, and a row whose keys are
     all hidden comes out as 0.  D is a multiple of 8, at most 128.  Tokens past the last sequence are
-    left as they were in ``out`` (unset in a new one).  -inf is added to a hidden key's score, and its value
-    is multiplied by a weight of 0, so an infinity or NaN there still reaches the rows of its own
-    sequence; other sequences and tokens of no sequence have no influence."""
+    left as they were in ``out`` (unset in a new one).  What a row does not see, a key that its bias hides, a
+    later one if ``causal``, another sequence, a token of no sequence, does not reach it, be it an infinity or
+    a NaN."""
     dtype = _check_first("q", q)
     T, hq, D = q.shape
     qp, qt, qh, _ = _view("q", q, T, D, q)

@@ -2,7 +2,8 @@
 //
 // Row i of sequence s (tokens cu[s] .. cu[s + 1]) and query head h, key head h / (Hq / Hkv):
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(x_ij - max_j x_ij),   x_ij = scale q_i . k_j + bias_ij
-// over the keys j of the same sequence, j <= i if causal.  A row whose keys are all at -inf is zero.
+// over the keys j of the same sequence, j <= i if causal, that bias_ij = -inf does not hide.  A row
+// that sees no key is zero.
 //
 // One pass over the keys with the running maximum m and sum l of the softmax, in base 2 (x times
 // log2 e).  The accumulator O = sum_j 2^(x_ij - m) v_j stays in tensor memory, so moving m would
@@ -26,6 +27,12 @@
 // softmax works on this one.  D > 64: O 2 x 128, S 2 x 128, and P overwrites S; the MMAs of a block
 // execute in issue order, so S of step j + 1 follows the P V that reads them.
 //
+// A product cannot leave out a hidden key: its weight is 0, and 0 times an infinity or a NaN in its v is a
+// NaN (as is -inf plus a NaN score).  A row with hidden keys that comes out non-finite is therefore made
+// again key by key (exact_row), by its warp; rows that a key they do see makes NaN come out so again.
+// (The check and the two functions' presence cost 0 to 2 %: causal prompts 630 -> 631 us, 2048 tokens 69.1
+// -> 69.6, 4 x 384 tokens with bias 13.9 -> 14.2.)
+//
 // Blocks find their sequence without a prefix sum over the lengths: sequence s owns the slots
 // from floor(cu[s] / R) + s (R rows a block), at least as many as it has blocks, and the slots it does
 // not need return at once.  The heads are the grid's fast axis, and later rows come first when
@@ -46,7 +53,7 @@ constexpr float kMoveMax = 8.f;
 
 struct Params {
   CUtensorMap tm_q, tm_k, tm_v;  // [H, T, D]: box {64, 128, 1}, 128B swizzle, zero past the ends
-  k8::View o;
+  k8::View q, k, v, o;  // (q, k and v again, for exact_row)
   const int* cu;
   const void* bias;  // [S or 1, Hq, n, n] or null, the last axis contiguous
   long long bias_ss, bias_sh, bias_sr;
@@ -177,6 +184,92 @@ __device__ __forceinline__ int find_sequence(const int* cu, int S, int T, int sl
     hi = min(hi, lo + step);
   }
   return lo;
+}
+
+// Row `row` of a sequence by a warp, over the keys that the row sees and no others: 32 keys at a time, a
+// lane a key for the scores and a column (of every 32) for the output.  Weights stay in fp32.  Slow (4096
+// causal tokens, 32 heads of 128, made so throughout: 55 ms instead of 0.16), and reached only as said at
+// the top; it stops where the whole row is NaN.
+template <typename T>
+__device__ __noinline__ void exact_row(const Params& p, int seq, int head, int beg, int len, int row) {
+  const int lane = threadIdx.x & 31, kv = head / p.group, lim = p.causal ? min(len, row + 1) : len;
+  const T* q = static_cast<const T*>(p.q.p) + (beg + row) * p.q.st + head * p.q.sh;
+  const T* k = static_cast<const T*>(p.k.p) + beg * p.k.st + kv * p.k.sh;
+  const T* v = static_cast<const T*>(p.v.p) + beg * p.v.st + kv * p.v.sh;
+  const bool biased = row < p.bias_n;
+  const T* b = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh + row * p.bias_sr;
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < lim; j0 += 32) {
+    const int j = j0 + lane;
+    const float bias = biased && j < min(lim, p.bias_n) ? static_cast<float>(b[j]) : 0.f;
+    const bool seen = j < lim && bias != -INFINITY;
+    float x = -INFINITY;
+    if (seen) {
+      float s = 0.f;
+      for (int c = 0; c < p.d; c += 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(q + c), e = *reinterpret_cast<const uint4*>(k + j * p.k.st + c);
+        const uint32_t au[4] = {a.x, a.y, a.z, a.w}, eu[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = k8::unpack2(au[i], T()), g = k8::unpack2(eu[i], T());
+          s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+        }
+      }
+      x = fmaf(s, p.scale, bias);
+    }
+    float top = x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = fmaxf(m, top);
+    const float at = top == -INFINITY ? 0.f : top;
+    const float f = ex2_approx((m - at) * kLog2e), w = seen ? ex2_approx((x - at) * kLog2e) : 0.f;
+    m = top;
+    float sum = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = fmaf(l, f, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= f;
+    for (unsigned left = __ballot_sync(0xffffffffu, seen); left != 0u; left &= left - 1) {
+      const int s = __ffs(left) - 1;
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const T* vs = v + (j0 + s) * p.v.st;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i * 32 + lane < p.d) acc[i] = fmaf(ws, static_cast<float>(vs[i * 32 + lane]), acc[i]);
+    }
+    bool lost = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lost = lost && (i * 32 + lane >= p.d || acc[i] != acc[i]);
+    if (__all_sync(0xffffffffu, lost)) break;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(p.o.p) + (beg + row) * p.o.st + head * p.o.sh;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i * 32 + lane < p.d) out[i * 32 + lane] = static_cast<T>(acc[i] * inv);
+  __syncwarp();
+}
+
+// The last key in [from, to) whose v is not finite, or -1; for a warp.
+template <typename T>
+__device__ __noinline__ int last_non_finite(const Params& p, int head, int beg, int from, int to) {
+  const T* v = static_cast<const T*>(p.v.p) + beg * p.v.st + head / p.group * p.v.sh;
+  int last = -1;
+  for (int j = from + (threadIdx.x & 31); j < to; j += 32) {
+    float zero = 0.f;
+    for (int c = 0; c < p.d; c += 8) {
+      const uint4 a = *reinterpret_cast<const uint4*>(v + j * p.v.st + c);
+      const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = k8::unpack2(u[i], T());
+        zero = fmaf(f.x, 0.f, fmaf(f.y, 0.f, zero));
+      }
+    }
+    if (zero != 0.f) last = j;
+  }
+  return __reduce_max_sync(0xffffffffu, last);
 }
 
 template <typename T, int DP, bool BIAS>
@@ -431,7 +524,8 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
     const float2 c2 = make_float2(flip ? -c : c, flip ? -c : c);
     // bf16's lowest value times log2 e is past fp32's range: with a bf16 bias the maximum is kept in x's
     // own units and subtracted before the factor, so a row that is masked by nothing but lowest values
-    // still sees its keys evenly.  (fp16 values are far from it, and take the factor in one operation.)
+    // still sees its keys evenly.  (4 x 384 tokens, 16 heads of 48: 13.6 -> 14.2 us.  fp16 values
+    // are far from it, and take the factor in one operation.)
     constexpr bool kUnits = BIAS && !__is_same(T, __half);
     constexpr float kMove = kUnits ? kMoveMax / kLog2e : kMoveMax;
     if (BIAS && nx > 0) fetch_bias(0);
@@ -572,6 +666,7 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.o.p) + static_cast<long long>(beg + row) * p.o.st + head * p.o.sh;
+      float zero = l * 0.f;  // or a NaN, if anything of the row is not finite
 #pragma unroll
       for (int b = 0; b < DP / 32; ++b) {
         const int c0 = b * 32;
@@ -584,10 +679,21 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
           if (c0 + g * 8 >= p.d) break;
           uint32_t u[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            u[e] = k8::pack2(__uint_as_float(o[g * 8 + 2 * e]) * inv, __uint_as_float(o[g * 8 + 2 * e + 1]) * inv, T());
+          for (int e = 0; e < 4; ++e) {
+            const float2 y = make_float2(__uint_as_float(o[g * 8 + 2 * e]), __uint_as_float(o[g * 8 + 2 * e + 1]));
+            zero = fmaf(y.x, 0.f, fmaf(y.y, 0.f, zero));
+            u[e] = k8::pack2(y.x * inv, y.y * inv, T());
+          }
           *reinterpret_cast<uint4*>(out + c0 + g * 8) = make_uint4(u[0], u[1], u[2], u[3]);
         }
+      }
+      __syncwarp();  // (exact_row's stores follow the lanes' own)
+      if (BIAS || p.causal) {
+        unsigned left = __ballot_sync(0xffffffffu, row < len && zero != 0.f);
+        // without a bias, only the last step has keys that some of its rows do not see
+        if (!BIAS && left != 0u)
+          left &= __ballot_sync(0xffffffffu, row < last_non_finite<T>(p, head, beg, tile0, min(len, tile0 + kTile)));
+        for (; left != 0u; left &= left - 1) exact_row<T>(p, seq, head, beg, len, row - lane + __ffs(left) - 1);
       }
     }
   }

@@ -305,6 +305,7 @@ int tmu_attention(const tmu_attention_args* args, void* stream) {
   for (int i = 0; i < 4; ++i)
     if ((st = check_heads(views[i]->data, views[i]->stride_token, views[i]->stride_head, names[i]))) return st;
   if (bias->n < 0 || (bias->n > 0 && !bias->data)) return fail(TMU_ERR_INVALID_ARGUMENT, "bias");
+  if (!aligned16(status)) return fail(TMU_ERR_MISALIGNED, "status not 16-byte aligned");
   // a tensor map cannot step by 0
   const int heads[3] = {Hq, Hkv, Hkv};
   for (int i = 0; i < 3; ++i)
@@ -321,7 +322,8 @@ int tmu_attention(const tmu_attention_args* args, void* stream) {
     const uint32_t box[3] = {64, (uint32_t)k7::kTile, 1};
     if ((st = encode_map(maps[i], views[i]->data, 3, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B))) return st;
   }
-  p.o = k8::View{out->data, out->stride_token, out->stride_head};
+  k8::View* dst[4] = {&p.q, &p.k, &p.v, &p.o};
+  for (int i = 0; i < 4; ++i) *dst[i] = k8::View{views[i]->data, views[i]->stride_token, views[i]->stride_head};
   p.cu = cu_seqlens;
   if (biased) {
     p.bias = bias->data;
@@ -371,6 +373,7 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
   if (!x || !w8 || !w_scales || !out || (x_dtype == TMU_E4M3 && !x_scales)) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL tensor");
   if (ldo < N && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of out overlap: ldo < N");
   if (!aligned16(x) || !aligned16(w8)) return fail(TMU_ERR_MISALIGNED, "x, w8 must be 16-byte aligned");
+  if (!aligned16(status)) return fail(TMU_ERR_MISALIGNED, "status not 16-byte aligned");
   if (x_dtype == TMU_E4M3 && ldx != K) return fail(TMU_ERR_UNSUPPORTED, "e4m3 x must be contiguous");
   if (ldx % 8) return fail(TMU_ERR_MISALIGNED, "ldx must be a multiple of 8");
   if (ldx < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of x overlap: ldx < K");

@@ -382,8 +382,8 @@ typedef struct tmu_qk_norm_rope_args {
 int tmu_qk_norm_rope(const tmu_qk_norm_rope_args* args, void* stream);
 
 /* Additive bias of the scores, of q's type: element (i, j) of sequence s and query head h at
- * s * stride_seq + h * stride_head + i * stride_row + j (a stride of 0 shares it).  Positions at or
- * past n have none; n = 0 for no bias. */
+ * s * stride_seq + h * stride_head + i * stride_row + j (a stride of 0 shares it).  -inf hides key j from
+ * row i.  Positions at or past n have none; n = 0 for no bias. */
 typedef struct tmu_attn_bias {
   const void* data;
   long long stride_seq, stride_head, stride_row;
@@ -394,9 +394,9 @@ typedef struct tmu_attn_bias {
  * cu_seqlens[s] .. cu_seqlens[s + 1] (int32, device, ascending; values outside [0, T] are clamped),
  * Hq a multiple of Hkv, D a multiple of 8, at most 128, fp16 or bf16.  With `causal` a token sees
  * itself and the tokens before it.  Scores, maxima, sums and the output are fp32 inside; the
- * weights are rounded to q's type for their product with v.  A row whose scores are all -inf is 0,
- * and tokens of no sequence keep what `out` holds.  `out` must not overlap q, k or v.  status may be
- * NULL. */
+ * weights are rounded to q's type for their product with v.  A key that a row does not see does not
+ * reach it, whatever its k and v hold; a row that sees none is 0, and tokens of no sequence keep what
+ * `out` holds.  `out` must not overlap q, k or v.  status may be NULL. */
 typedef struct tmu_attention_args {
   tmu_heads q, k, v, out;
   const int* cu_seqlens; /* [S + 1] */

@@ -222,6 +222,41 @@ def test_attention_causal_future_scores_do_not_count(d):
     assert got[200:].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("d", [8, 40, 64, 128])
+def test_attention_hidden_keys_do_not_count_whatever_they_hold(d, dtype):
+    """NaN and infinities in k and v of keys that -inf hides (a padded batch), or that lie behind a
+    causal row, reach no row that does not see them: also in a step of their own, in a row without
+    keys, with shared heads, and beside another sequence."""
+    lens, hq, hkv = [300, 33, 150], 4, 2
+    q, k, v, cu = make_qkv(lens, hq, hkv, d, dtype, 63)
+    b = torch.randn(3, hq, 300, 300, generator=gen(64), device="cuda").to(dtype)
+    pads = [130, 20, 150]  # keys of each sequence that are there
+    for s, n in enumerate(pads):
+        b[s, :, :, n:] = -math.inf
+    b[0, :, 3, :] = -math.inf
+    scale = 1 / math.sqrt(d)
+    for causal in (False, True):
+        ref, tol = attention_ref(q, k, v, lens, causal, scale, b)
+        k2, v2 = k.clone(), v.clone()
+        k2[130:300:2], v2[131:300:2] = float("nan"), float("nan")
+        k2[133:300:5], v2[135:300:7] = float("inf"), -float("inf")
+        v2[320:333, :, ::3] = float("nan")
+        got = att.attention(q, k2, v2, cu, causal=causal, bias=b)
+        assert_within(got, ref, tol)
+        assert (got[3] == 0).all()
+    ref, tol = attention_ref(q, k, v, lens, True, scale)
+    k2, v2 = k.clone(), v.clone()
+    k2[200], v2[200:204] = float("nan"), float("inf")
+    v2[310, 1, d - 1] = float("nan")
+    got = att.attention(q, k2, v2, cu, causal=True)
+    keep = torch.ones(got.shape, dtype=torch.bool, device="cuda")
+    keep[200:300] = False           # these see keys 200 on
+    keep[310:333, 2:, d - 1] = False  # key head 1 is query heads 2 and 3's
+    assert_within(got[keep], ref[keep], tol[keep])
+    assert got[200:300].isnan().all() and got[310:333, 2:, d - 1].isnan().all()
+
+
 @pytest.mark.parametrize("d", [48, 64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_attention_one_bad_score_spoils_its_row_only(bad, d):
