@@ -193,64 +193,77 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
             raise ValueError("the rotary must be on q's device")
         rot = (positions.data_ptr(), positions.element_size(), rotary.turns.data_ptr(), rotary.gain, rotary.rot,
                1 if rotary.layout == "interleaved" else 0)
-    if q_out is not None or k_out is not None:
-        _check_rope_outputs(q, k, q_out, k_out)
-    q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
-    k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
-    args = _lib.QK_NORM_ROPE_ARGS.pack(qp, qt, qh, kp, kt, kh, *_view("q_out", q_out, T, D, q)[:3],
-                                       *_view("k_out", k_out, T, D, q)[:3], kind, eps, pointer(q_weight), pointer(q_bias),
-                                       pointer(k_weight), pointer(k_bias), *rot, T, hq, hk, D, dtype)
+    given = q_out is not None or k_out is not None
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        qo = (q_out.data_ptr(), hq * D, D, hq)
+    else:
+        qo = (qp, qt, qh, hq) if q_out is q else _view("q_out", q_out, T, D, q)
+    if k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        ko = (k_out.data_ptr(), hk * D, D, hk)
+    else:
+        ko = (kp, kt, kh, hk) if k_out is k else _view("k_out", k_out, T, D, q)
+    if given:
+        _check_rope_outputs((qp, qt, qh, hq), (kp, kt, kh, hk), qo, ko, T, D)
+    args = _lib.QK_NORM_ROPE_ARGS.pack(qp, qt, qh, kp, kt, kh, *qo[:3], *ko[:3], kind, eps, pointer(q_weight),
+                                       pointer(q_bias), pointer(k_weight), pointer(k_bias), *rot, T, hq, hk, D, dtype)
     launch(q.device, "tmu_qk_norm_rope", args)
     return q_out, k_out
 
 
-def _check_rope_outputs(q, k, q_out, k_out) -> None:
-    T, _, D = q.shape
+def _check_rope_outputs(q, k, q_out, k_out, T: int, D: int) -> None:
+    """The views (address, token stride, head stride, heads) of 16-bit tensors."""
     for name, src, dst, other in (("q_out", q, q_out, k), ("k_out", k, k_out, q)):
-        if dst is None:
-            continue
-        _view(name, dst, T, D, q)
-        if dst.shape != src.shape:
+        if dst[3] != src[3]:
             raise ValueError(f"{name} must be shaped like its input")
-        if _self_overlap(dst):
+        if _folded(dst, T, D):
             raise ValueError(f"{name} must not overlap itself")
-        in_place = src.data_ptr() == dst.data_ptr() and src.stride() == dst.stride()
-        if _heads_overlap(dst, other) or (_heads_overlap(dst, src) and not in_place):
+        if _meet(dst, other, T, D, T, D) or (dst != src and _meet(dst, src, T, D, T, D)):
             raise ValueError(f"{name} may be its own input, and must not overlap one otherwise")
-    if q_out is not None and k_out is not None and _heads_overlap(q_out, k_out):
+    if _meet(q_out, k_out, T, D, T, D):
         raise ValueError("q_out and k_out must not overlap")
 
 
-def _self_overlap(t: torch.Tensor) -> bool:
+def _folded(view, T: int, D: int) -> bool:
     """Whether two heads of a [T, H, D] view share memory (exact for non-negative strides)."""
-    (T, H, D), (st, sh, _) = t.shape, t.stride()
-    axes = sorted((s, n) for s, n in ((st, T), (sh, H)) if n > 1)
+    _, st, sh, H = view
+    axes = [(s, n) for s, n in ((st, T), (sh, H)) if n > 1]
     span = D
-    for s, n in axes:
+    for s, n in sorted(axes):
         if s < span:
             return True
-        span = s * (n - 1) + span
+        span += s * (n - 1)
     return False
 
 
-def _heads_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two [T, H, D] views share memory.  Views of one projection interleave without
-    sharing: with one token stride, their heads' ranges are compared within a token."""
-    if a.numel() == 0 or b.numel() == 0:
+def _meet(a, b, Ta: int, Da: int, Tb: int, Db: int, size_a: int = 2, size_b: int = 2) -> bool:
+    """Whether two [T, H, D] views of elements of the given sizes share memory.  Views of one
+    projection interleave without sharing: with one token stride, their heads' ranges are compared
+    within a token."""
+    (pa, sta, sha, ha), (pb, stb, shb, hb) = a, b
+    if Ta == 0 or Tb == 0 or ha == 0 or hb == 0:
         return False
-
-    if not spans_overlap(a, b):
+    wa, wb = ((ha - 1) * sha + Da) * size_a, ((hb - 1) * shb + Db) * size_b  # bytes that a token's heads reach over
+    if pa + (Ta - 1) * sta * size_a + wa <= pb or pb + (Tb - 1) * stb * size_b + wb <= pa:
         return False
-
-    def token_span(t):
-        return (sum((t.shape[i] - 1) * t.stride(i) for i in (1, 2)) + 1) * t.element_size()
-
-    step = a.stride(0) * a.element_size()
-    wa, wb = token_span(a), token_span(b)
-    if a.shape[0] > 1 and step == b.stride(0) * b.element_size() and step >= max(wa, wb):
-        off = (b.data_ptr() - a.data_ptr()) % step  # b's heads begin `off` bytes behind a's in each period
+    step = sta * size_a
+    if Ta > 1 and step == stb * size_b and step >= wa and step >= wb:
+        off = (pb - pa) % step  # b's heads begin `off` bytes behind a's in each period
         return off < wa or off + wb > step
     return True
+
+
+def _ints(t: torch.Tensor) -> tuple[int, int, int, int]:
+    return t.data_ptr(), t.stride(0), t.stride(1), t.shape[1]
+
+
+def _self_overlap(t: torch.Tensor) -> bool:
+    return _folded(_ints(t), t.shape[0], t.shape[2])
+
+
+def _heads_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return _meet(_ints(a), _ints(b), a.shape[0], a.shape[2], b.shape[0], b.shape[2], a.element_size(), b.element_size())
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *, causal: bool = False,
@@ -293,15 +306,17 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
         b = (bias.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1], stride[2], n)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        op, ot, oh = out.data_ptr(), hq * D, D
     else:
         if out.shape != q.shape:
             raise ValueError("out must be shaped like q")
-        if _self_overlap(out) or any(_heads_overlap(out, t) for t in (q, k, v)):
+        o = op, ot, oh, _ = _view("out", out, T, D, q)
+        if _folded(o, T, D) or any(_meet(o, t, T, D, T, D) for t in ((qp, qt, qh, hq), (kp, kt, kh, hk), (vp, vt, vh, hk))):
             raise ValueError("out must not overlap itself, q, k or v")
         if bias is not None and spans_overlap(out, bias):
             raise ValueError("out must not overlap bias")
     scale = 1.0 / math.sqrt(D) if scale is None else scale
-    args = _lib.ATTENTION_ARGS.pack(qp, qt, qh, kp, kt, kh, vp, vt, vh, *_view("out", out, T, D, q)[:3],
+    args = _lib.ATTENTION_ARGS.pack(qp, qt, qh, kp, kt, kh, vp, vt, vh, op, ot, oh,
                                     cu_seqlens.data_ptr(), *b, S, T, hq, hk, D, dtype, 1 if causal else 0, scale,
                                     pointer(status))
     launch(q.device, "tmu_attention", args)
