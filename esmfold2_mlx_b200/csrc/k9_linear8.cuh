@@ -27,7 +27,6 @@ struct QuantParams {
   uint8_t* x8;  // [M, K]
   float* xs;    // scale of row m and block b at m * xs_m + b * xs_b
   long long xs_m, xs_b;
-  int chained;  // the outputs are a workspace that only the next kernel of the same call reads
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // keeps a NaN
@@ -123,10 +122,9 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
     }
     if (m < p.M && b0 + i < p.kb && l == 0) p.xs[m * p.xs_m + (b0 + i) * p.xs_b] = s;
   }
-  // linear8_rows_kernel reads w8 before its dependency wait, so nothing that could be a weight may
-  // be announced before it is visible.  (Announced at the start, the products' blocks come while
-  // these still run, two on some SMs and none on others: 13.4 -> 16 us at 1283 x 1000 x 1360.)
-  if (p.chained) griddep_trigger();
+  // (Announced at the start, the products' blocks come while these still run, two on some SMs and none
+  // on others: 13.4 -> 16 us at 1283 x 1000 x 1360.)
+  griddep_trigger();
 }
 
 // Row-major scales [M, kb] to [kb, ld], for the tensor-core kernels.
@@ -240,8 +238,8 @@ __global__ void __launch_bounds__(kRowsThreads, PAIRS == 1 ? 4 : PAIRS == 4 ? 3 
   };
   uint4 cur[2][2], xcur[PAIRS];
   float scur[PAIRS];
-  load_w(warp, cur);  // no kernel that starts its successor early writes a weight, so this need not wait
-  griddep_wait();
+  griddep_wait();  // w8 too may be what the kernel in front of this one writes
+  load_w(warp, cur);
   load_x(warp, xcur, scur);
   float total[G][4];
 #pragma unroll

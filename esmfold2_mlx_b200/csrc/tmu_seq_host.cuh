@@ -179,7 +179,7 @@ int launch_k9(const void* x8, const float* xst, int ld_xs, const void* w8, const
 }
 
 int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, long long xs_m,
-                  long long xs_b, bool chained, cudaStream_t stream) {
+                  long long xs_b, cudaStream_t stream) {
   if (M < 0 || K < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "M must not be negative, K positive");
   if (M > 1 << 30 || K > 1 << 30) return fail(TMU_ERR_UNSUPPORTED, "M or K > 2^30");
   if (K % 16) return fail(TMU_ERR_UNSUPPORTED, "K must be a multiple of 16");
@@ -202,7 +202,6 @@ int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8
   p.xs = scales;
   p.xs_m = xs_m;
   p.xs_b = xs_b;
-  p.chained = chained;
   // two blocks of 128 at a time once that still gives every SM eight blocks of threads
   const long long groups = (M + k9::kQuantRows - 1) / k9::kQuantRows;
   const bool two = groups * ((p.kb + 1) / 2) >= 8ll * dev.sms;
@@ -353,7 +352,7 @@ int tmu_attention(const tmu_attention_args* args, void* stream) {
 }
 
 int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8, float* scales, void* stream) {
-  return quantize_rows(x, dtype, ld, M, K, x8, scales, (K + 127) / 128, 1, false, static_cast<cudaStream_t>(stream));
+  return quantize_rows(x, dtype, ld, M, K, x8, scales, (K + 127) / 128, 1, static_cast<cudaStream_t>(stream));
 }
 
 size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
@@ -387,7 +386,7 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
   const uint8_t* x8 = static_cast<const uint8_t*>(x);
   if (x_dtype != TMU_E4M3) {
     uint8_t* ws = static_cast<uint8_t*>(workspace) + k9_scale_bytes(M, K);
-    int st = quantize_rows(x, x_dtype, ldx, M, K, ws, xst, 1, ld_xs, true, s);
+    int st = quantize_rows(x, x_dtype, ldx, M, K, ws, xst, 1, ld_xs, s);
     if (st) return st;
     x8 = ws;
   } else {

@@ -5,6 +5,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -223,3 +225,39 @@ def test_weight_layout():
     assert ((d - w).abs() <= torch.maximum(w.abs() * 2.0**-4, s * 2.0**-10) * (1 + 1e-6)).all()
     z = fp8.quantize_weight(torch.zeros(8, 16), "cpu")
     assert (z.dequantize() == 0).all() and (z.scales == fp8.SCALE_MIN).all()
+
+
+def kernels(text):
+    """Name and body of every __global__ function in a source file."""
+    for m in re.finditer(r"__global__[^;{]*?(\w+)\(const __grid_constant__[^)]*\)\s*\{", text):
+        depth, end = 1, m.end()
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        yield m.group(1), text[m.end():end]
+
+
+def test_kernels_read_nothing_before_their_dependency_wait():
+    """Whatever a call is given, weights too, may be the output of the kernel in front of it: no load of the
+    sequence kernels stands before griddepcontrol.wait.  (Bodies of lambdas are left out: they run where
+    they are called.)"""
+    found = set()
+    for name in ("k7_attention.cuh", "k8_qk_rope.cuh", "k9_linear8.cuh"):
+        with open(os.path.join(build.CSRC, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for kernel, body in kernels(text):
+            found.add(kernel)
+            head, wait, _ = body.partition("griddep_wait();")
+            assert wait, kernel
+            while True:
+                m = re.search(r"auto \w+ = \[&\]\(.*?\)\s*\{", head)
+                if m is None:
+                    break
+                depth, end = 1, m.end()
+                while depth:
+                    depth += {"{": 1, "}": -1}.get(head[end], 0)
+                    end += 1
+                head = head[:m.start()] + head[end:]
+            assert not re.search(r"\b(load\w*|__ldg|tma_load\w*|run)\(|ld\.global|cp\.async", head), kernel
+    assert found == {"attention_kernel", "qk_rope_kernel", "quantize_kernel", "transpose_scales_kernel",
+                     "linear8_rows_kernel", "linear8_kernel", "linear8_pair_kernel"}

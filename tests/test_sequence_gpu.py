@@ -580,6 +580,55 @@ def test_linear_non_finite_rows_stay_apart():
         assert torch.equal(got[keep], clean[keep]) and got[1].isnan().all() and got[3].isnan().all()
 
 
+@pytest.mark.parametrize("writer", ["copy", "linear"])
+@pytest.mark.parametrize("m", [1, 16])
+def test_linear_weight_of_the_kernel_in_front(m, writer):
+    """Weights that the kernel directly in front writes, by a copy or by a linear layer that starts its
+    successor early, eagerly and in a graph: each call multiplies by the new ones.
+
+    The writing layer picks columns of a matrix of few-bit values, exactly: an fp16 value's two bytes are
+    then an e4m3 value and a 0."""
+    g = gen(35)
+    n, k, deep = 256, 128, 10240
+    values = torch.tensor([0.5, 1.0, 1.5, 2.0, 3.0, -0.5, -1.0, -2.0], device="cuda")
+    table = values[torch.randint(0, 8, (k // 2, deep), generator=g, device="cuda")]
+    picker = fp8.BlockWeight(table.to(torch.float8_e4m3fn), torch.ones(1, deep // 128, device="cuda"))
+    picks = [torch.nn.functional.one_hot(torch.randint(0, deep, (n,), generator=g, device="cuda"), deep).half()
+             for _ in range(2)]
+    new = [fp8.linear(p, picker) for p in picks]
+    for p, y in zip(picks, new):
+        assert torch.equal(y, table.t()[p.argmax(1)].half())
+    buf = torch.zeros(n, k // 2, dtype=FP16, device="cuda")
+    w = fp8.BlockWeight(buf.view(torch.float8_e4m3fn), torch.ones(n // 128, 1, device="cuda"))
+    x = torch.randn(m, k, generator=g, device="cuda").half()
+    want = []
+    for y in new:
+        buf.copy_(y)
+        torch.cuda.synchronize()
+        want.append(fp8.linear(x, w))
+    torch.cuda.synchronize()
+    assert not torch.equal(*want)
+
+    def turns():
+        outs = []
+        for i in range(20):
+            if writer == "copy":
+                torch.add(new[i % 2], 0.0, out=buf)
+            else:
+                fp8.linear(picks[i % 2], picker, out=buf)
+            outs.append(fp8.linear(x, w))
+        return outs
+
+    outs = turns()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(outs))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = turns()
+    for _ in range(5):
+        graph.replay()
+        assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(outs))
+
+
 # ---- together --------------------------------------------------------------------------------
 
 def layer(x, pos, cu, rotary, w_qkv, w_out, gq, gk, hq, hkv, d):
