@@ -16,12 +16,14 @@ device; nothing synchronises.  Inference only: an input that asks for gradients 
 from __future__ import annotations
 
 import math
+from decimal import Context, Decimal, localcontext
 
 import torch
 
 from . import _lib
 
 _DTYPES = {torch.float16: _lib.TMU_F16, torch.bfloat16: _lib.TMU_BF16}
+_PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
 _NORMS = {None: _lib.TMU_NORM_NONE, "rms": _lib.TMU_NORM_RMS, "layer": _lib.TMU_NORM_LAYER}
 
 
@@ -112,8 +114,10 @@ class Rotary:
       below ``beta_slow`` are divided by s, with a linear ramp over the pair index between, and the
       rotated values are multiplied by ``gain``.
 
-    Frequencies are kept as turns a position in 64-bit fixed point, so no position is too far: the
-    angle is exact to 2^-32 of a turn for every 64-bit position, negative ones included."""
+    Frequencies are kept as turns a position in 64-bit fixed point, each the nearest one, and multiplied
+    by the 64-bit position in integers, negative ones too.  So the angle is off by at most
+    ``abs(position) * 2**-65`` of a turn (2^-33 at 2^32 positions, 2^-26 at 2^39) and by its conversion to
+    fp32, 2^-26 of a turn.  ``frequencies`` has them in radians a position, rounded to 64-bit floats."""
 
     def __init__(self, rot: int, base: float = 10000.0, layout: str = "half", scaling: dict | None = None,
                  device="cuda"):
@@ -123,35 +127,40 @@ class Rotary:
             raise ValueError("layout must be 'half' or 'interleaved'")
         self.rot, self.base, self.layout = int(rot), float(base), layout
         self.gain = 1.0
-        self.frequencies = self._frequencies(scaling)  # radians a position
-        fixed = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequencies]
+        with localcontext(Context(prec=60)):  # 64 bits of a turn need more digits than a float's 53
+            exact = self._frequencies(scaling)
+            fixed = [int((f / (2 * _PI) * 2**64).to_integral_value()) % 2**64 for f in exact]
+        self.frequencies = [float(f) for f in exact]
         signed = [f - 2**64 if f >= 2**63 else f for f in fixed]
         self.turns = torch.tensor(signed, dtype=torch.int64).to(device)
 
-    def _frequencies(self, scaling: dict | None) -> list[float]:
-        half, base = self.rot // 2, self.base
+    def _frequencies(self, scaling: dict | None) -> list[Decimal]:
+        """Radians a position, to the digits of the current decimal context."""
+        half, base = self.rot // 2, Decimal(self.base)
         kind = None if scaling is None else scaling.get("type")
         if kind not in (None, "linear", "ntk", "yarn"):
             raise ValueError(f"unknown scaling {kind!r}")
         s = 1.0 if kind is None else float(scaling["factor"])
-        if s <= 0.0 or base <= 1.0:
-            raise ValueError("the factor must be positive and the base above 1")
+        if not (0.0 < s < math.inf and 1.0 < self.base < math.inf):
+            raise ValueError("the factor must be positive and the base above 1, both finite")
+        factor = Decimal(s)
         if kind == "ntk":
-            base *= s ** (self.rot / (self.rot - 2))
-        freq = [base ** (-i / half) for i in range(half)]
+            base *= factor ** (Decimal(self.rot) / (self.rot - 2))
+        freq = [base ** (Decimal(-i) / half) for i in range(half)]
         if kind == "linear":
-            return [f / s for f in freq]
+            return [f / factor for f in freq]
         if kind == "yarn":
             n = float(scaling["original_length"])
 
             def pair_at(turns):  # the pair index that turns `turns` times over n positions
-                return half * math.log(n / (turns * 2.0 * math.pi)) / math.log(base)
+                return half * math.log(n / (turns * 2.0 * math.pi)) / math.log(self.base)
 
             lo = max(math.floor(pair_at(float(scaling.get("beta_fast", 32.0)))), 0)
             hi = min(math.ceil(pair_at(float(scaling.get("beta_slow", 1.0)))), self.rot - 1)
             self.gain = float(scaling.get("gain", 0.1 * math.log(s) + 1.0 if s > 1.0 else 1.0))
-            ramp = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(half)]
-            return [f * (1.0 - r) + f / s * r for f, r in zip(freq, ramp)]
+            width = Decimal(hi - lo) if hi > lo else Decimal("0.001")
+            ramp = [min(Decimal(1), max(Decimal(0), (i - lo) / width)) for i in range(half)]
+            return [f * (1 - r) + f / factor * r for f, r in zip(freq, ramp)]
         return freq
 
 

@@ -9,8 +9,9 @@
 //
 // The angle.  f_i is kept as turns a position in 64-bit fixed point, F_i = round(f_i / 2 pi * 2^64):
 // the product pos * F_i wraps modulo 2^64, which is modulo one turn, so its top 32 bits are the
-// angle's fraction of a turn to 2^-32 (1.5e-9 rad) for every position, however far, and no table
-// of positions has to be kept or bounded.  (An fp32 product pos * f_i is off by up to pos * 2^-24 rad.)
+// angle's fraction of a turn, and no table of positions has to be kept or bounded.  F_i's rounding puts
+// it off by |pos| 2^-65 of a turn (2^-33 at 2^32 positions), its own to fp32 by 2^-26 of a turn (9e-8 rad).
+// (An fp32 product pos * f_i is off by up to pos * 2^-24 rad.)
 //
 // Bound: HBM (each value is read once and written once, 4 bytes moved for about 20 operations).
 // Split: D / 8 lanes (rounded up to a power of two, LPH) a head and 8 values a lane, as two runs of

@@ -363,7 +363,8 @@ typedef struct tmu_qk_norm {
 typedef struct tmu_rotary {
   const void* positions;            /* int32 or int64 [T] */
   int position_bytes;               /* 4 or 8 */
-  const unsigned long long* turns;  /* [rot / 2]: turns a position of each pair, times 2^64 */
+  const unsigned long long* turns;  /* [rot / 2]: turns a position of each pair, times 2^64, to nearest: an
+                                       angle is off by |position| 2^-65 of a turn, plus 2^-26 of fp32 */
   float gain;                       /* factor of the rotated values */
   int rot;                          /* rotated values of a head: a multiple of 16, 0 for none */
   int interleaved;                  /* pairs (2i, 2i + 1); else (i, i + rot / 2) */

@@ -7,6 +7,7 @@ import ctypes
 import math
 import os
 import re
+from fractions import Fraction
 
 import pytest
 import torch
@@ -261,3 +262,53 @@ def test_kernels_read_nothing_before_their_dependency_wait():
             assert not re.search(r"\b(load\w*|__ldg|tma_load\w*|run)\(|ld\.global|cp\.async", head), kernel
     assert found == {"attention_kernel", "qk_rope_kernel", "quantize_kernel", "transpose_scales_kernel",
                      "linear8_rows_kernel", "linear8_kernel", "linear8_pair_kernel"}
+
+
+def pi_bounds():
+    """pi from Machin's formula in integers, to 2^-240 either way."""
+    one = 1 << 256
+
+    def arctan_inverse(x):
+        total, term, k = 0, one // x, 1
+        while term:
+            total += term // k if k % 4 == 1 else -(term // k)
+            term //= x * x
+            k += 2
+        return total
+
+    pi = 4 * (4 * arctan_inverse(5) - arctan_inverse(239))
+    return Fraction(pi - (1 << 16), one), Fraction(pi + (1 << 16), one)
+
+
+@pytest.mark.parametrize("rot,base", [(16, 10000.0), (64, 10000.0), (64, 500000.0), (128, 10000.5)])
+@pytest.mark.parametrize("kind", [None, "linear", "ntk", "yarn"])
+def test_rotary_turns_are_the_nearest(rot, base, kind):
+    """Each 64-bit turn against its definition in rational numbers: with f = 2 pi turns / 2^64, and the
+    factors that the scaling gives it taken off, f^(rot / 2) base^i = 1 lies between half a unit below and
+    above (ntk: f^(h (h - 1)) base^(i (h - 1)) s^(i h) = 1 with h = rot / 2)."""
+    s = Fraction(4) if kind != "yarn" else Fraction(16)
+    scaling = {None: None, "linear": {"type": "linear", "factor": 4.0}, "ntk": {"type": "ntk", "factor": 4.0},
+               "yarn": {"type": "yarn", "factor": 16.0, "original_length": 4096}}[kind]
+    half, b = rot // 2, Fraction(base)
+    lo = max(math.floor(half * math.log(4096 / (32 * 2 * math.pi)) / math.log(base)), 0)
+    hi = min(math.ceil(half * math.log(4096 / (2 * math.pi)) / math.log(base)), rot - 1)
+    pi_lo, pi_hi = pi_bounds()
+    unit = Fraction(1, 1 << 64)
+    near = Fraction(1, 2) + Fraction(1, 1 << 32)
+    for i, t in enumerate(att.Rotary(rot, base, scaling=scaling, device="cpu").turns.tolist()):
+        take = Fraction(1)
+        if kind == "linear":
+            take = s
+        if kind == "yarn":
+            r = min(max(Fraction(i - lo, hi - lo), Fraction(0)), Fraction(1))
+            take = 1 / (1 - r + r / s)
+        low, high = 2 * pi_lo * (t - near) * unit * take, 2 * pi_hi * (t + near) * unit * take
+        if kind == "ntk":
+            rest = b ** (i * (half - 1)) * s ** (i * half)
+            assert low ** (half * (half - 1)) * rest < 1 < high ** (half * (half - 1)) * rest, i
+        else:
+            assert low ** half * b ** i < 1 < high ** half * b ** i, i
+    for bad in ({"base": math.inf}, {"base": math.nan}, {"scaling": {"type": "linear", "factor": math.inf}},
+                {"scaling": {"type": "ntk", "factor": math.nan}}):
+        with pytest.raises(ValueError):
+            att.Rotary(rot, device="cpu", **bad)

@@ -7,6 +7,7 @@ Tolerances count roundings: u = eps / 2 of the stored type, fp32 work at 2^-24 a
 from __future__ import annotations
 
 import math
+from decimal import Decimal, localcontext
 
 import pytest
 import torch
@@ -445,6 +446,38 @@ def test_rotary_far_positions_and_types():
     ref, tol = rope_ref(q, pos, rotary, None, None, None, 0.0)
     assert_within(q64, ref, tol + 2.0 ** -20 * q.double().abs().amax())
     assert torch.equal(q64[0], q[0])
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_positions_past_32_bits(layout):
+    """Angles against 70 digits.  The allowance is the frequency's rounding, 2^-65 of a turn a position,
+    beside the fp32 work of the other tests (whose 2^-20 holds the angle's own rounding, 2^-26 of a turn)."""
+    places = [2 ** 31 + 5, 2 ** 32 + 12345, 2 ** 33 - 1, -(2 ** 36) - 7, 2 ** 40 + 1, 2 ** 45 - 3, -(2 ** 48) + 11]
+    rot, d = 64, 80
+    q = torch.randn(len(places), 3, d, generator=gen(22), device="cuda").half()
+    got, _ = att.qk_norm_rope(q, q.clone(), torch.tensor(places, device="cuda"), att.Rotary(rot, layout=layout))
+    with localcontext() as ctx:
+        ctx.prec = 70
+        # pi by Machin's formula
+        def arctan_inverse(x):
+            total, term, k = Decimal(0), Decimal(1) / x, 1
+            while abs(term) > Decimal(10) ** -75:
+                total, term, k = total + term / k, -term / (x * x), k + 2
+            return total
+        pi = 4 * (4 * arctan_inverse(5) - arctan_inverse(239))
+        turns = [[float(p * Decimal(10000) ** (Decimal(-2 * i) / rot) / (2 * pi) % 1) for i in range(rot // 2)]
+                 for p in places]
+    ang = 2 * math.pi * torch.tensor(turns, dtype=torch.float64, device="cuda")[:, None]
+    i1 = torch.arange(rot // 2, device="cuda")
+    i1, i2 = (i1, i1 + rot // 2) if layout == "half" else (2 * i1, 2 * i1 + 1)
+    x = q.double()
+    ref, size = x.clone(), x.abs()
+    ref[..., i1] = x[..., i1] * ang.cos() - x[..., i2] * ang.sin()
+    ref[..., i2] = x[..., i2] * ang.cos() + x[..., i1] * ang.sin()
+    size[..., i1] = size[..., i2] = x[..., i1].abs() + x[..., i2].abs()
+    far = torch.tensor([2 * math.pi * abs(p) * 2.0 ** -65 for p in places], dtype=torch.float64, device="cuda")
+    tol = half_step(FP16) * ref.abs() + (16 * 2.0 ** -24 + far[:, None, None]) * size + least(FP16)
+    assert_within(got, ref, tol)
 
 
 def test_qk_norm_only_and_constant_rows():
