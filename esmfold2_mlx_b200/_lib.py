@@ -170,6 +170,7 @@ SIGNATURES = {
                            _sz, _vp, _vp]),
     "tmu_parcae_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmu_parcae_step": (_i, [_vp, _vp, _vp, ctypes.POINTER(TmuParcaeWeights), _vp, _i, _i, _i, _vp, _sz, _vp, _vp]),
+    "tmu_sequence_status": (_i, [ctypes.POINTER(_vp)]),
     "tmu_qk_norm_rope": (_i, [_vp, _vp]),
     "tmu_attention": (_i, [_vp, _vp]),
     "tmu_quantize_rows": (_i, [_vp, _i, _ll, _i, _i, _vp, _vp, _vp]),

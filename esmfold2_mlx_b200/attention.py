@@ -11,6 +11,10 @@ model in front of the trunk (``mlx_esmc.py``).  Tokens of all sequences lie behi
 ``q``, ``k`` and ``v`` may be slices of one fused projection: the values of a head are contiguous and
 the other strides are multiples of 8 elements.  Launches go on the current stream of the tensors'
 device; nothing synchronises.  Inference only: an input that asks for gradients is refused.
+
+A kernel's waits are bounded.  One that gives up leaves its output invalid and records it in the call's
+``status`` block (``ops.new_status``, read by ``ops.check_status``), or without one in the device's own
+record, which ``ops.check_sequence_status()`` reads where the program synchronises anyway.
 """
 
 from __future__ import annotations
@@ -288,7 +292,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     all hidden comes out as 0.  D is a multiple of 8, at most 128.  Tokens past the last sequence are
     left as they were in ``out`` (unset in a new one).  What a row does not see, a key that its bias hides, a
     later one if ``causal``, another sequence, a token of no sequence, does not reach it, be it an infinity or
-    a NaN."""
+    a NaN.  Device errors go to ``status``, or to the record that ``ops.check_sequence_status`` reads."""
     dtype = _check_first("q", q)
     T, hq, D = q.shape
     qp, qt, qh, _ = _view("q", q, T, D, q)

@@ -34,7 +34,8 @@ namespace tmu {
 // elected lane issue: the values that TMA and MMA instructions take from uniform registers are then
 // computed there instead of being moved there one by one (the 8-bit pair kernel: 585 -> 521 us).
 
-// Where the sequence kernels' status goes in calls without a status block of their own.
+// Where the sequence kernels' status goes in calls without a status block of their own
+// (tmu_sequence_status gives it to the host).
 __device__ DeviceStatus g_own_status;
 
 // The whole warp waits for a phase of an mbarrier, every lane polling: from a commit to the answering

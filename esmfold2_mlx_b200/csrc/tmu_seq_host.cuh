@@ -218,6 +218,12 @@ int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8
 
 extern "C" {
 
+int tmu_sequence_status(void** status) {
+  if (!status) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
+  cudaError_t e = cudaGetSymbolAddress(status, g_own_status);
+  return e == cudaSuccess ? TMU_OK : cuda_fail(e, "cudaGetSymbolAddress");
+}
+
 int tmu_qk_norm_rope(const tmu_qk_norm_rope_args* args, void* stream) {
   if (!args) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL argument");
   const tmu_heads *q = &args->q, *k = &args->k, *q_out = &args->q_out, *k_out = &args->k_out;

@@ -122,7 +122,8 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
     [..., K] with ``x_scales`` [..., ceil(K / 128)] from :func:`quantize_rows`; returns [..., N].
 
     ``bias`` is fp32 [N].  The output is ``out_dtype`` (fp16, bf16 or fp32; x's type by default, fp16 for
-    e4m3 x) or ``out`` [..., N], which must not overlap an input."""
+    e4m3 x) or ``out`` [..., N], which must not overlap an input.  Device errors go to ``status``, or to the
+    record that ``ops.check_sequence_status`` reads."""
     code = _IN.get(x.dtype)
     if code is None or not x.is_cuda:
         raise TypeError("x must be a CUDA fp16, bf16 or float8_e4m3fn tensor")

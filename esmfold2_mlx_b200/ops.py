@@ -183,6 +183,22 @@ def check_status(status: torch.Tensor, where: str) -> None:
     raise_for_status(*read_status(status), where)
 
 
+def check_sequence_status(device=None) -> None:
+    """Synchronise the current stream of ``device`` (the current one by default) and raise :class:`TmuError`
+    if a sequence operator that was called without a ``status`` block (``attention.attention``,
+    ``fp8.linear``) recorded an error on it since the last check.  The record is cleared."""
+    lib = _lib.load()
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    block, code, site = ctypes.c_void_p(0), ctypes.c_int(0), ctypes.c_int(0)
+    with torch.cuda.device(device):
+        stream = _stream_ptr(torch.device("cuda", torch.cuda.current_device()))
+        _lib.check(lib.tmu_sequence_status(ctypes.byref(block)), "tmu_sequence_status")
+        _lib.check(lib.tmu_read_first_error(block, stream, ctypes.byref(code), ctypes.byref(site)), "tmu_read_first_error")
+        if code.value:
+            _lib.check(lib.tmu_reset_status(block, stream), "tmu_reset_status")
+    raise_for_status(code.value, site.value, "sequence operators")
+
+
 def project_gate(z: torch.Tensor, mask: torch.Tensor | None, w: TrimulWeights, status: torch.Tensor | None = None):
     """K1: returns channel-major (a, b), each [B*c, L, row_pitch(L)] fp16 (pad columns unset)."""
     lib = _lib.load()

@@ -370,6 +370,12 @@ typedef struct tmu_rotary {
   int interleaved;                  /* pairs (2i, 2i + 1); else (i, i + rot / 2) */
 } tmu_rotary;
 
+/* What a call without a status block (status NULL) finds out on the device, a wait that gave up for
+ * instance, whose output is then invalid, is recorded in a block of the current device that the library
+ * owns, for all such calls.  *status is its address: read it with tmu_read_first_error, after which
+ * tmu_reset_status clears it. */
+int tmu_sequence_status(void** status);
+
 /* K8: norm of every head of q [T, Hq, D] and k [T, Hkv, D] over its D values, then the rotation of
  * its first `rot` values, fp32 inside and rounded once.  D a multiple of 16, at most 256; fp16 or
  * bf16 in and out.  An output may be its own input; otherwise the four must not overlap. */
@@ -397,7 +403,7 @@ typedef struct tmu_attn_bias {
  * itself and the tokens before it.  Scores, maxima, sums and the output are fp32 inside; the
  * weights are rounded to q's type for their product with v.  A key that a row does not see does not
  * reach it, whatever its k and v hold; a row that sees none is 0, and tokens of no sequence keep what
- * `out` holds.  `out` must not overlap q, k or v.  status may be NULL. */
+ * `out` holds.  `out` must not overlap q, k or v.  status may be NULL (tmu_sequence_status). */
 typedef struct tmu_attention_args {
   tmu_heads q, k, v, out;
   const int* cu_seqlens; /* [S + 1] */
@@ -420,7 +426,7 @@ int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void
  * workspace; x_scales NULL) or e4m3 with its x_scales (both contiguous),
  * bias fp32 [N] or NULL, out fp16, bf16 or fp32, rows ldo elements apart.  Sums are fp32.
  * Workspace: tmu_linear_fp8_workspace_bytes, 16-byte aligned; it holds nothing between calls.
- * status may be NULL. */
+ * status may be NULL (tmu_sequence_status). */
 size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K);
 int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_scales, const void* w8,
                    const float* w_scales, const float* bias, void* out, int out_dtype, long long ldo, int M, int N,

@@ -141,6 +141,10 @@ def test_sizes_past_the_index_range(lib):
     assert lib.tmu_linear_fp8_workspace_bytes(big, 8, 64) == 0
 
 
+def test_sequence_status_needs_an_address(lib):
+    assert lib.tmu_sequence_status(None) == INVALID
+
+
 def test_status_block(lib):
     assert lib.tmu_linear_fp8(P, 0, 64, None, P, P, None, P, 0, 8, 40, 8, 64, P, 1 << 20, P + 8, None) == MISALIGNED
     dev = torch.device("cpu")

@@ -6,6 +6,7 @@ Tolerances count roundings: u = eps / 2 of the stored type, fp32 work at 2^-24 a
 
 from __future__ import annotations
 
+import ctypes
 import math
 from decimal import Decimal, localcontext
 
@@ -757,6 +758,29 @@ def test_status_blocks():
             att.attention(q, k, v, cu, status=bad)
         with pytest.raises(ValueError):
             fp8.linear(x, w, status=bad)
+
+
+def test_errors_of_calls_without_a_status_block_are_heard():
+    """The device's own record: clean after good calls; an error in it (a bounded wait that runs out, put
+    there by the library's self-test) is raised once, with its code, and cleared."""
+    ops.check_sequence_status()
+    q, k, v, cu = make_qkv([300, 20], 2, 2, 64, FP16, 65)
+    want = att.attention(q, k, v, cu)
+    x, w = torch.randn(200, 256, generator=gen(66), device="cuda").half(), fp8.quantize_weight(torch.randn(64, 256))
+    fp8.linear(x, w)
+    ops.check_sequence_status()
+    lib = att._lib.load()
+    block = ctypes.c_void_p(0)
+    att._lib.check(lib.tmu_sequence_status(ctypes.byref(block)), "tmu_sequence_status")
+    side = torch.cuda.Stream()
+    for where in (torch.cuda.current_stream(), side):
+        att._lib.check(lib.tmu_selftest_wait_timeout(block, 1000000, where.cuda_stream), "tmu_selftest_wait_timeout")
+        with torch.cuda.stream(where), pytest.raises(att._lib.TmuError) as e:
+            ops.check_sequence_status(q.device)
+        assert e.value.name == "TMU_ERR_DEVICE_TIMEOUT"
+        torch.cuda.synchronize()
+        ops.check_sequence_status("cuda")
+    assert torch.equal(att.attention(q, k, v, cu), want)
 
 
 # ---- refusals that need CUDA tensors ----------------------------------------------------------
