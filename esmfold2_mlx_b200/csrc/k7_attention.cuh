@@ -8,8 +8,8 @@
 // One pass over the keys with the running maximum m and sum l of the softmax, in base 2 (x times
 // log2 e).  The accumulator O = sum_j 2^(x_ij - m) v_j stays in tensor memory, so moving m would
 // mean reading and writing all of it: m only moves when a tile's maximum exceeds it by more than
-// 8, so weights reach at most 2^8 (exact in fp32 sums, and a common factor of the 16-bit weights),
-// and the result, O / l, does not depend on when it moved.
+// 8, so weights reach at most 2^8 (exact in fp32 sums, and a common factor of the 16-bit weights;
+// fp16: kLift more), and the result, O / l, does not depend on when it moved.
 //
 // A tile is 128 rows of one head; a step takes 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the
 // softmax of S's rows, P in TMEM in the inputs' type, and O += P V with P as the MMA's A operand out of
@@ -50,6 +50,11 @@ constexpr int kTile = 128;     // query rows of a tile, keys of a step
 constexpr int kAtom = kTile * 128;  // 64 values of 128 rows
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kMoveMax = 8.f;
+// fp16 weights are 2^7 times as large, up to 2^15: those that round to 0 in the product (and stay in the
+// sum) are below 2^-32 of the row's largest, not 2^-25, under which the keys of a long row can add up to
+// a visible share.  bf16 has the range.
+template <typename T>
+constexpr float kLift = __is_same(T, __half) ? 7.f : 0.f;
 
 struct Params {
   CUtensorMap tm_q, tm_k, tm_v;  // [H, T, D]: box {64, 128, 1}, 128B swizzle, zero past the ends
@@ -144,7 +149,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// 2^t of a pair, t <= kMoveMax or so, on the fused multiply-add units: t = n + f with n the nearest
+// 2^t of a pair, t <= kMoveMax + kLift or so, on the fused multiply-add units: t = n + f with n the nearest
 // integer (adding 1.5 * 2^23 leaves it in the low bits) and |f| <= 1/2, 2^f by a polynomial of degree 4
 // with constant term 1 (minimax in the relative error, 2^-18.4, against 2^-9 and 2^-11 of the weights'
 // types), n added to the exponent.  t is held at -127 or above, where the sum of exponents is
@@ -639,7 +644,7 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
           tmem_st16(at, o);
         }
       }
-      const float neg = m == -INFINITY ? 0.f : -m;
+      const float neg = m == -INFINITY ? 0.f : kLift<T> - m;
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int b = 0; b < kTile / 32; ++b) {

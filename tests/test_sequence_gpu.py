@@ -322,6 +322,38 @@ def test_attention_large_scores(dtype):
         assert_within(got, ref, tol)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("bits", [20, 26, 28])
+@pytest.mark.parametrize("heavy", [0, 1000, 2047])
+def test_attention_small_weights_add_up(heavy, bits, with_bias, d):
+    """One key far above 2047 others whose values alone are not 0: the row is the sum of many weights of
+    about 2^-bits.  In fp16 a weight is off by u of itself, or by 2^-25 where it is subnormal, with the row's
+    largest weight at 2^7 or above; the rest as in attention_ref (a bias of its own size has one product)."""
+    n, low = 2048, -bits * math.log(2)
+    q, k, v, cu = make_qkv([n], 1, 1, d, FP16, 67)
+    q.zero_(), k.zero_()
+    v.abs_()
+    v[heavy] = 0.0
+    if with_bias:
+        bias = torch.full((1, 1, n, n), low, dtype=FP16, device="cuda")
+        bias[..., heavy] = 0.0
+        x = bias[0, 0, 0].double()
+    else:
+        bias = None
+        q[:, :, 0] = 8.0
+        k[:, :, 0] = low / 8
+        k[heavy] = 0.0
+        x = 8.0 * k[:, 0, 0].double()
+    got = att.attention(q, k, v, cu, scale=1.0, bias=bias)
+    p = x.exp()
+    ref = (p @ v[:, 0].double() / p.sum())[None, None].expand(n, 1, d)
+    u = half_step(FP16)
+    rel = u + 2 * d * 2.0 ** -24 * x.abs().max() + 2.0 ** -15 + (2 * n + 8) * 2.0 ** -24
+    tol = u * ref + rel * ref + 2.0 ** -32 * v[:, 0].double().sum(0) / p.sum() + least(FP16)
+    assert_within(got, ref, tol)
+
+
 def test_attention_bad_cu_seqlens_stay_in_bounds():
     """Offsets outside the tokens are clamped; the good sequences are right."""
     q, k, v, _ = make_qkv([200], 2, 2, 64, FP16, 12)
