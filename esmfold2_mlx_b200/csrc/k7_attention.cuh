@@ -28,10 +28,11 @@
 // execute in issue order, so S of step j + 1 follows the P V that reads them.
 //
 // A product cannot leave out a hidden key: its weight is 0, and 0 times an infinity or a NaN in its v is a
-// NaN (as is -inf plus a NaN score).  A row with hidden keys that comes out non-finite is therefore made
-// again key by key (exact_row), by its warp; rows that a key they do see makes NaN come out so again.
-// (The check and the two functions' presence cost 0 to 2 %: causal prompts 630 -> 631 us, 2048 tokens 69.1
-// -> 69.6, 4 x 384 tokens with bias 13.9 -> 14.2.)
+// NaN (as is -inf plus a NaN score).  A row that comes out non-finite, and that a key it does not see may
+// have made so (spoiled_rows), is therefore made again key by key (exact_row), by its warp.  (The check
+// and the two functions' presence cost 0 to 2 %: causal prompts 630 -> 631 us, 2048 tokens 69.1 -> 69.6,
+// 4 x 384 tokens with bias 13.9 -> 14.2.  2048 tokens, 16 heads of 64 with a bias, one call alone: 65 us; a NaN
+// that rows see 231, for the search, and 18 ms while every such row was made again; a NaN in hidden v 8 ms.)
 //
 // Blocks find their sequence without a prefix sum over the lengths: sequence s owns the slots
 // from floor(cu[s] / R) + s (R rows a block), at least as many as it has blocks, and the slots it does
@@ -192,9 +193,8 @@ __device__ __forceinline__ int find_sequence(const int* cu, int S, int T, int sl
 }
 
 // Row `row` of a sequence by a warp, over the keys that the row sees and no others: 32 keys at a time, a
-// lane a key for the scores and a column (of every 32) for the output.  Weights stay in fp32.  Slow (4096
-// causal tokens, 32 heads of 128, made so throughout: 55 ms instead of 0.16), and reached only as said at
-// the top; it stops where the whole row is NaN.
+// lane a key for the scores and a column (of every 32) for the output.  Weights stay in fp32.  Slow (0.11 ms
+// a row of 1200 keys of 64), and reached only as said at the top; it stops where the whole row is NaN.
 template <typename T>
 __device__ __noinline__ void exact_row(const Params& p, int seq, int head, int beg, int len, int row) {
   const int lane = threadIdx.x & 31, kv = head / p.group, lim = p.causal ? min(len, row + 1) : len;
@@ -211,6 +211,7 @@ __device__ __noinline__ void exact_row(const Params& p, int seq, int head, int b
     float x = -INFINITY;
     if (seen) {
       float s = 0.f;
+#pragma unroll 4
       for (int c = 0; c < p.d; c += 8) {
         const uint4 a = *reinterpret_cast<const uint4*>(q + c), e = *reinterpret_cast<const uint4*>(k + j * p.k.st + c);
         const uint32_t au[4] = {a.x, a.y, a.z, a.w}, eu[4] = {e.x, e.y, e.z, e.w};
@@ -235,13 +236,23 @@ __device__ __noinline__ void exact_row(const Params& p, int seq, int head, int b
     l = fmaf(l, f, sum);
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= f;
-    for (unsigned left = __ballot_sync(0xffffffffu, seen); left != 0u; left &= left - 1) {
-      const int s = __ffs(left) - 1;
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const T* vs = v + (j0 + s) * p.v.st;
+    // eight keys' loads at a time: one key after the other, a row of 1200 keys took 290 us
+    const unsigned in = __ballot_sync(0xffffffffu, seen);
+#pragma unroll 1
+    for (int s0 = 0; s0 < 32; s0 += 8) {
+      float y[8][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i * 32 + lane < p.d) acc[i] = fmaf(ws, static_cast<float>(vs[i * 32 + lane]), acc[i]);
+      for (int s = 0; s < 8; ++s) {
+        const T* vs = v + min(j0 + s0 + s, lim - 1) * p.v.st;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[s][i] = static_cast<float>(vs[i * 32 + lane < p.d ? i * 32 + lane : 0]);
+      }
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s0 + s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = in >> (s0 + s) & 1u ? fmaf(ws, y[s][i], acc[i]) : acc[i];
+      }
     }
     bool lost = true;
 #pragma unroll
@@ -256,25 +267,45 @@ __device__ __noinline__ void exact_row(const Params& p, int seq, int head, int b
   __syncwarp();
 }
 
-// The last key in [from, to) whose v is not finite, or -1; for a warp.
-template <typename T>
-__device__ __noinline__ int last_non_finite(const Params& p, int head, int beg, int from, int to) {
-  const T* v = static_cast<const T*>(p.v.p) + beg * p.v.st + head / p.group * p.v.sh;
-  int last = -1;
-  for (int j = from + (threadIdx.x & 31); j < to; j += 32) {
-    float zero = 0.f;
+// Which rows of `left` (bit r: row row0 + r) a key that they do not see may have made non-finite; for a
+// warp.  Such a key, in [from, to), has a v that is not finite, or, where its score met a -inf bias, a k
+// that is not or that is past 2^60; a row whose q is past 2^60 counts too (below both, 128 products stay
+// finite in fp32).  A lane a key, then the rows against the keys that were found.
+template <typename T, bool BIAS>
+__device__ __noinline__ unsigned spoiled_rows(const Params& p, int seq, int head, int beg, int from, int to, int row0,
+                                              unsigned left) {
+  const int lane = threadIdx.x & 31, kv = head / p.group;
+  const T* q = static_cast<const T*>(p.q.p) + (beg + row0 + lane) * p.q.st + head * p.q.sh;
+  const T* k = static_cast<const T*>(p.k.p) + beg * p.k.st + kv * p.k.sh;
+  const T* v = static_cast<const T*>(p.v.p) + beg * p.v.st + kv * p.v.sh;
+  const T* b = static_cast<const T*>(p.bias) + seq * p.bias_ss + head * p.bias_sh;
+  auto beyond = [&](const T* x, float limit) {  // is a value of the row not below `limit` (a NaN is not)
+    bool any = false;
+#pragma unroll 4
     for (int c = 0; c < p.d; c += 8) {
-      const uint4 a = *reinterpret_cast<const uint4*>(v + j * p.v.st + c);
+      const uint4 a = *reinterpret_cast<const uint4*>(x + c);
       const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 f = k8::unpack2(u[i], T());
-        zero = fmaf(f.x, 0.f, fmaf(f.y, 0.f, zero));
+        any |= !(fabsf(f.x) < limit) | !(fabsf(f.y) < limit);
       }
     }
-    if (zero != 0.f) last = j;
+    return any;
+  };
+  unsigned found = BIAS ? __ballot_sync(0xffffffffu, (left >> lane & 1u) && beyond(q, 0x1p60f)) : 0u;
+  for (int j0 = from; j0 < to && found != left; j0 += 32) {
+    const int j = j0 + lane;
+    const bool bad = j < to && (beyond(v + j * p.v.st, INFINITY) || (BIAS && beyond(k + j * p.k.st, 0x1p60f)));
+    if (!__any_sync(0xffffffffu, bad)) continue;
+    for (unsigned rest = left & ~found; rest != 0u; rest &= rest - 1) {
+      const int r = __ffs(rest) - 1, row = row0 + r;
+      const bool hidden = (p.causal && j > row) || (BIAS && bad && row < p.bias_n && j < p.bias_n &&
+                                                    static_cast<float>(b[row * p.bias_sr + j]) == -INFINITY);
+      if (__any_sync(0xffffffffu, bad && hidden)) found |= 1u << r;
+    }
   }
-  return __reduce_max_sync(0xffffffffu, last);
+  return found;
 }
 
 template <typename T, int DP, bool BIAS>
@@ -696,8 +727,8 @@ __global__ void __launch_bounds__(Cfg<DP, BIAS>::kThreads, Cfg<DP, BIAS>::kBlock
       if (BIAS || p.causal) {
         unsigned left = __ballot_sync(0xffffffffu, row < len && zero != 0.f);
         // without a bias, only the last step has keys that some of its rows do not see
-        if (!BIAS && left != 0u)
-          left &= __ballot_sync(0xffffffffu, row < last_non_finite<T>(p, head, beg, tile0, min(len, tile0 + kTile)));
+        if (left != 0u)
+          left = spoiled_rows<T, BIAS>(p, seq, head, beg, BIAS ? 0 : tile0, min(len, nx * kTile), row - lane, left);
         for (; left != 0u; left &= left - 1) exact_row<T>(p, seq, head, beg, len, row - lane + __ffs(left) - 1);
       }
     }
