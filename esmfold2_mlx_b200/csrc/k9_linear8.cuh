@@ -721,12 +721,40 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
-// Arrive on the even CTA's barrier to hand a TMEM slot back.  The loads from it have completed and
-// are ordered by tcgen05.fence::before_thread_sync; no memory write is handed over, so the arrive
-// needs no cluster-scope release (with one, and with cluster-scope waits on the MMAs' commits, a step took
-// 20 % longer at 4096 x 4736 x 2560).
-__device__ __forceinline__ void arrive_slot(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+// warp_poll for a barrier that the other CTA of the pair completes, in the cluster's scope: relaxed
+// polls, and once the phase is there an acquire of shared memory alone, the counterpart of
+// mbar_arrive_cluster_smem's release.  All the barriers of a pair are waited for so: the other CTA's loads
+// and readers and the paired MMAs' commits complete them.  (16384 x 10240 -> 2560: 470 us, with acquires of
+// all memory 472; in the CTA's own scope, which orders nothing between two CTAs, 460.)
+__device__ __forceinline__ bool mbar_test_pair(uint64_t* bar, uint32_t parity, uint32_t hint_ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ bool warp_poll_pair(uint64_t* bar, uint32_t parity, const WaitCtx& ctx, unsigned int site) {
+  bool ok = false;
+  for (int i = 0; i < 64 && !ok; ++i) ok = mbar_test_pair(bar, parity, 0);
+  if (!__all_sync(0xffffffffu, ok)) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!ok) {
+      ok = mbar_test_pair(bar, parity, kSuspendHintNs);
+      if (ok || *ctx.abort) break;
+      if (globaltimer_ns() - t0 > ctx.timeout_ns) {
+        raise_abort(ctx, site);
+        break;
+      }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  }
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+  return ok;
 }
 
 // Tile t: row tiles in groups of kGroup, column tiles inside a group, row tiles fastest.
@@ -798,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
         m0 += static_cast<int>(rank) * kTile;
         n0 += static_cast<int>(rank) * (kTile / 2);
         for (int b = 0; b < p.kb; ++b, ++i) {
-          if (!(ok = warp_poll(&empty[s], ph ^ 1, ctx, kSiteProd))) break;
+          if (!(ok = warp_poll_pair(&empty[s], ph ^ 1, ctx, kSiteProd))) break;
           if (leader) {
             if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
             tma_load_2d_pair(smem + OFF_A + s * kOperand, &p.tm_x, bar0 + s * sizeof(uint64_t), b * 128, m0);
@@ -830,10 +858,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       for (int t = first; t < tiles; t += step)
         for (int b = 0; b < p.kb; ++b, ++i) {
           const uint32_t c = i & 1;
-          warp_poll(&full[s], ph, ctx, kSiteMma);
+          warp_poll_pair(&full[s], ph, ctx, kSiteMma);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            warp_poll(&sempty[2 * c + h], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot);
+            warp_poll_pair(&sempty[2 * c + h], ((i >> 1) & 1) ^ 1, ctx, kSiteSlot);
             tc_fence_after();
             const uint64_t as = sdesc_add(ad, s * kOperand), bs = sdesc_add(bd, s * kOperand + h * (kOperand / 2));
             const uint32_t d = tmem + c * 256 + h * kTile;
@@ -864,14 +892,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear8_pair_kernel(const __grid_
       for (int t = first; t < tiles; t += step)
         for (int b = 0; b < p.kb; ++b, ++i) {
           const uint32_t c = i & 1;
-          warp_poll(&sfull[2 * c + h], (i >> 1) & 1, ctx, kSiteSum);
+          warp_poll_pair(&sfull[2 * c + h], (i >> 1) & 1, ctx, kSiteSum);
           named_bar_arrive(kBarFull + 2 * c + h, kSumThreads + 32);
           named_bar_sync(kBarRead + 2 * c + h, kSumThreads + 32);
           tc_fence_after();
           tc_fence_before();
           if (lane == 0) {
             if (rank == 0) mbar_arrive(&sempty[2 * c + h]);
-            else arrive_slot(slots + 2 * c * sizeof(uint64_t));
+            else mbar_arrive_cluster_smem(slots + 2 * c * sizeof(uint64_t));
           }
           __syncwarp();
         }

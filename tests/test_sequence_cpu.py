@@ -316,3 +316,16 @@ def test_rotary_turns_are_the_nearest(rot, base, kind):
                 {"scaling": {"type": "ntk", "factor": math.nan}}):
         with pytest.raises(ValueError):
             att.Rotary(rot, device="cpu", **bad)
+
+
+def test_arrives_on_the_other_cta_have_the_clusters_scope():
+    """An arrive on another CTA's barrier names the cluster's scope (the default is the CTA's), and the pair
+    kernel of the 8-bit product waits in it for every barrier that the pair shares."""
+    for name in sorted(os.listdir(build.CSRC)):
+        with open(os.path.join(build.CSRC, name)) as f:
+            text = f.read()
+        for m in re.finditer(r"mbarrier\.arrive\.[\w.:]*shared::cluster", text):
+            assert re.search(r"\.(release|relaxed)\.cluster\.", m.group(0)), (name, m.group(0))
+        if name == "k9_linear8.cuh":
+            body = dict(kernels(re.sub(r"//[^\n]*", "", text)))["linear8_pair_kernel"]
+            assert body.count("warp_poll_pair(") == 4 and "warp_poll(" not in body
