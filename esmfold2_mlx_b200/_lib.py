@@ -175,6 +175,7 @@ SIGNATURES = {
     "tmu_attention": (_i, [_vp, _vp]),
     "tmu_quantize_rows": (_i, [_vp, _i, _ll, _i, _i, _vp, _vp, _vp]),
     "tmu_linear_fp8_workspace_bytes": (_sz, [_i, _i, _i]),
+    "tmu_linear_fp8_scaled_workspace_bytes": (_sz, [_i, _i, _i]),
     "tmu_linear_fp8": (_i, [_vp, _i, _ll, _vp, _vp, _vp, _vp, _vp, _i, _ll, _i, _i, _i, _vp, _sz, _vp, _vp]),
     "tmu_ipc_export": (_i, [_vp, _vp, ctypes.POINTER(_ull)]),
     "tmu_ipc_import": (_i, [_vp, _ull, ctypes.POINTER(_vp)]),

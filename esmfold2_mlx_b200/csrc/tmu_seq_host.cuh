@@ -110,7 +110,7 @@ int encode_bytes(CUtensorMap* m, const void* base, uint64_t rows, uint64_t K, ui
   return r == CUDA_SUCCESS ? TMU_OK : fail(TMU_ERR_DRIVER, "cuTensorMapEncodeTiled failed for an 8-bit operand");
 }
 
-// The workspace: x's scales [kb, M rounded up to 256], then x8 [M, K].
+// The workspace: x's scales [kb, M rounded up to 256], then x8 [M, K] where x is not e4m3 already.
 size_t k9_scale_bytes(int M, int K) {
   return static_cast<size_t>((M + 255) / 256) * 256 * ((K + 127) / 128) * 4;
 }
@@ -361,9 +361,14 @@ int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void
   return quantize_rows(x, dtype, ld, M, K, x8, scales, (K + 127) / 128, 1, static_cast<cudaStream_t>(stream));
 }
 
-size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
+size_t tmu_linear_fp8_scaled_workspace_bytes(int M, int N, int K) {
   if (M <= k9::kRowsMax || M > 1 << 30 || N < 1 || K < 1 || K > 1 << 30) return 0;
-  return k9_scale_bytes(M, K) + static_cast<size_t>(M) * K;
+  return k9_scale_bytes(M, K);
+}
+
+size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K) {
+  const size_t scales = tmu_linear_fp8_scaled_workspace_bytes(M, N, K);
+  return scales == 0 ? 0 : scales + static_cast<size_t>(M) * K;
 }
 
 int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_scales, const void* w8, const float* w_scales,
@@ -384,7 +389,8 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
   if (ldx < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of x overlap: ldx < K");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (M <= k9::kRowsMax) return launch_k9_rows(x, x_dtype, ldx, x_scales, w8, w_scales, bias, out, out_dtype, ldo, M, N, K, s);
-  if (!workspace || workspace_bytes < tmu_linear_fp8_workspace_bytes(M, N, K))
+  if (!workspace || workspace_bytes < (x_dtype == TMU_E4M3 ? tmu_linear_fp8_scaled_workspace_bytes(M, N, K)
+                                                           : tmu_linear_fp8_workspace_bytes(M, N, K)))
     return fail(TMU_ERR_WORKSPACE_TOO_SMALL, "workspace too small");
   if (!aligned16(workspace)) return fail(TMU_ERR_MISALIGNED, "workspace not 16-byte aligned");
   float* xst = static_cast<float*>(workspace);

@@ -173,7 +173,8 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
                 or any(t is not None and spans_overlap(out, t) for t in (w8, scales, bias, x_scales))):
             raise ValueError("out must not overlap an input")
         to, ldo = orow.data_ptr(), _ld(orow)
-    need = (_lib._lib or _lib.load()).tmu_linear_fp8_workspace_bytes(m, n, k)
+    lib = _lib._lib or _lib.load()
+    need = (lib.tmu_linear_fp8_scaled_workspace_bytes if xs else lib.tmu_linear_fp8_workspace_bytes)(m, n, k)
     ws = x.new_empty((need,), dtype=torch.uint8) if need else None  # held until the launch is in the stream
     launch(x.device, "tmu_linear_fp8", rows.data_ptr(), code, ld, xs, w8.data_ptr(), scales.data_ptr(), pointer(bias), to,
            out_code, ldo, m, n, k, pointer(ws), need, pointer(status))

@@ -425,9 +425,11 @@ int tmu_quantize_rows(const void* x, int dtype, long long ld, int M, int K, void
  * [ceil(N / 128), ceil(K / 128)], x fp16 or bf16 [M, K] (quantised as by tmu_quantize_rows into the
  * workspace; x_scales NULL) or e4m3 with its x_scales (both contiguous),
  * bias fp32 [N] or NULL, out fp16, bf16 or fp32, rows ldo elements apart.  Sums are fp32.
- * Workspace: tmu_linear_fp8_workspace_bytes, 16-byte aligned; it holds nothing between calls.
+ * Workspace: tmu_linear_fp8_workspace_bytes, or for e4m3 x, which needs its scales alone there,
+ * tmu_linear_fp8_scaled_workspace_bytes; 16-byte aligned; it holds nothing between calls.
  * status may be NULL (tmu_sequence_status). */
 size_t tmu_linear_fp8_workspace_bytes(int M, int N, int K);
+size_t tmu_linear_fp8_scaled_workspace_bytes(int M, int N, int K);
 int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_scales, const void* w8,
                    const float* w_scales, const float* bias, void* out, int out_dtype, long long ldo, int M, int N,
                    int K, void* workspace, size_t workspace_bytes, void* status, void* stream);

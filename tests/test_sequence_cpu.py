@@ -133,6 +133,17 @@ def test_linear_refusals(lib):
     assert lib.tmu_quantize_rows(P, 2, 48, 2, 48, P, P, None) == UNSUPPORTED
 
 
+def test_workspace_of_e4m3_rows(lib):
+    """x that is e4m3 already needs room for its scales alone."""
+    e4m3 = {"xd": _lib.TMU_E4M3, "xs": P, "K": 1360, "ldx": 1360, "M": 700}
+    need = lib.tmu_linear_fp8_scaled_workspace_bytes(700, 8, 1360)
+    assert need == 768 * 11 * 4 and lib.tmu_linear_fp8_workspace_bytes(700, 8, 1360) == need + 700 * 1360
+    assert linear(lib, nb=need - 1, **e4m3) == WORKSPACE
+    assert linear(lib, nb=need, work=P + 8, **e4m3) == MISALIGNED  # large enough
+    assert linear(lib, nb=need, work=P + 8, K=1360, ldx=1360, M=700) == WORKSPACE
+    assert lib.tmu_linear_fp8_scaled_workspace_bytes(16, 8, 64) == 0
+
+
 def test_sizes_past_the_index_range(lib):
     big = (1 << 30) + 1
     assert linear(lib, M=big) == UNSUPPORTED and linear(lib, N=big, ldo=1 << 31) == UNSUPPORTED

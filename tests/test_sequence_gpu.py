@@ -661,6 +661,20 @@ def test_linear(m, n, k, dtype):
     assert torch.equal(got, fp8.linear(x, w, out_dtype=F32))  # the same bits by either way, and again
 
 
+def test_linear_of_e4m3_rows_takes_no_second_copy():
+    """The call's workspace for e4m3 x holds the scales (rounded up to 256 rows), not another x."""
+    m, k = 5000, 2048
+    x8, xs = fp8.quantize_rows(torch.randn(m, k, generator=gen(72), device="cuda").half())
+    w = fp8.quantize_weight(torch.randn(64, k, generator=gen(73), device="cuda"))
+    out = torch.empty(m, 64, dtype=FP16, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    fp8.linear(x8, w, x_scales=xs, out=out)
+    assert torch.cuda.max_memory_allocated() - before <= 5120 * 16 * 4 + 512
+    assert_within(out, *linear_ref(x8, xs, w, None, FP16))
+
+
 def test_linear_views_and_shapes():
     g = gen(32)
     w = fp8.quantize_weight(torch.randn(200, 256, generator=g, device="cuda"))
