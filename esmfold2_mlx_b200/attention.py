@@ -10,7 +10,8 @@ model in front of the trunk (``mlx_esmc.py``).  Tokens of all sequences lie behi
 
 ``q``, ``k`` and ``v`` may be slices of one fused projection: the values of a head are contiguous and
 the other strides are multiples of 8 elements.  Launches go on the current stream of the tensors'
-device; nothing synchronises.  Inference only: an input that asks for gradients is refused.
+device; nothing synchronises.  Inference only: an input that asks for gradients, or carries a tangent, is
+refused.
 
 A kernel's waits are bounded.  One that gives up leaves its output invalid and records it in the call's
 ``status`` block (``ops.new_status``, read by ``ops.check_status``), or without one in the device's own
@@ -23,6 +24,7 @@ import math
 from decimal import Context, Decimal, localcontext
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -55,11 +57,15 @@ def pointer(t: torch.Tensor | None) -> int:
 
 
 def refuse_grad(where: str, *tensors) -> None:
-    """Raise if autograd would expect a gradient from an operator that has none."""
+    """Raise if autograd would expect a gradient, or a tangent, from an operator that has none."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{where} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():  # inside forward_ad.dual_level()
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{where} has no forward derivative: unpack its inputs' primals")
 
 
 def check_status_block(status: torch.Tensor | None, device: torch.device) -> None:
@@ -184,7 +190,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
     kind = _NORMS.get(norm)
     if kind is None:
         raise ValueError("norm must be None, 'rms' or 'layer'")
-    refuse_grad("qk_norm_rope", q, k, q_weight, k_weight, q_bias, k_bias)
+    refuse_grad("qk_norm_rope", q, k, q_weight, k_weight, q_bias, k_bias, q_out, k_out)
     if norm is None:
         if not (q_weight is k_weight is q_bias is k_bias is None):
             raise ValueError("weights and biases need a norm")
@@ -300,7 +306,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     vp, vt, vh, hv = _view("v", v, T, D, q)
     if hv != hk:
         raise ValueError("k and v must have the same heads")
-    refuse_grad("attention", q, k, v, bias)
+    refuse_grad("attention", q, k, v, bias, out)
     if status is not None:
         check_status_block(status, q.device)
     if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.device != q.device

@@ -10,7 +10,7 @@ run their 8-bit form and a block's largest value uses the whole range.
     y = fp8.linear(x, w, bias=linear.bias)
 
 Launches go on the current stream of the tensors' device; nothing synchronises.  Inference only: an
-input that asks for gradients is refused.
+input that asks for gradients, or carries a tangent, is refused.
 """
 
 from __future__ import annotations
@@ -133,7 +133,7 @@ def linear(x: torch.Tensor, weight: BlockWeight, bias: torch.Tensor | None = Non
         raise ValueError(f"x must be [..., {k}], got {tuple(shape)}")
     if w8.device != x.device:
         raise ValueError("the weight must be on x's device")
-    refuse_grad("fp8.linear", x, bias)
+    refuse_grad("fp8.linear", x, bias, scales, x_scales, out)
     if status is not None:
         check_status_block(status, x.device)
     rows = _rows("x", x)

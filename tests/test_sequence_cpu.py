@@ -11,6 +11,7 @@ from fractions import Fraction
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from esmfold2_mlx_b200 import _lib, attention as att, build, fp8
 
@@ -196,6 +197,26 @@ def test_python_refusals():
                 lambda: att.Rotary(32, scaling={"type": "linear", "factor": 0.0}, device="cpu")):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_gradients_and_tangents_are_refused():
+    x = torch.zeros(3)
+    y = torch.zeros(3, requires_grad=True)
+    att.refuse_grad("op", None, x)
+    with pytest.raises(ValueError):
+        att.refuse_grad("op", x, y)
+    with torch.no_grad():
+        att.refuse_grad("op", y)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        att.refuse_grad("op", x, forward_ad.unpack_dual(dual).primal)
+        for t in (dual, dual[1:]):
+            with pytest.raises(ValueError):
+                att.refuse_grad("op", None, x, t)
+            with torch.no_grad(), pytest.raises(ValueError):  # tangents are made under it too
+                att.refuse_grad("op", t)
+    with torch.no_grad():
+        att.refuse_grad("op", x)
 
 
 def test_heads_overlap():

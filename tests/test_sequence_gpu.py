@@ -12,6 +12,7 @@ from decimal import Decimal, localcontext
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from esmfold2_mlx_b200 import attention as att
 from esmfold2_mlx_b200 import fp8, ops
@@ -886,6 +887,37 @@ def test_errors_of_calls_without_a_status_block_are_heard():
         torch.cuda.synchronize()
         ops.check_sequence_status("cuda")
     assert torch.equal(att.attention(q, k, v, cu), want)
+
+
+def test_every_input_that_asks_for_a_gradient_is_refused():
+    """Scales and given outputs as much as the values, and tangents as much as gradients."""
+    q, k, v, cu = make_qkv([20], 4, 2, 64, FP16, 74)
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    o = torch.empty_like(q)
+    w = fp8.quantize_weight(torch.randn(32, 64))
+    x = torch.zeros(40, 64, device="cuda", dtype=FP16)
+    x8, xs = fp8.quantize_rows(x)
+    gs = torch.ones(64, device="cuda")
+    y = torch.empty(40, 32, device="cuda", dtype=FP16)
+    calls = [lambda **a: att.attention(**{"q": q, "k": k, "v": v, "out": o, **a}, cu_seqlens=cu),
+             lambda **a: att.qk_norm_rope(**{"q": q, "k": k, "norm": "rms", "q_weight": gs, "q_out": o, **a}),
+             lambda **a: fp8.linear(**{"x": x, "weight": w, "out": y, **a}),
+             lambda **a: fp8.linear(**{"x": x8, "weight": w, "x_scales": xs, "out": y, **a}),
+             lambda **a: fp8.quantize_rows(**{"x": x, **a})]
+    given = [{"q": q, "k": k, "v": v, "out": o}, {"q": q, "k": k, "q_weight": gs, "q_out": o}, {"x": x, "out": y},
+             {"x_scales": xs, "out": y}, {"x": x}]
+    for call, names in zip(calls, given):
+        call()
+        for name, t in names.items():
+            asks = t.detach().clone().requires_grad_()
+            with pytest.raises(ValueError, match="backward"):
+                call(**{name: asks})
+            with torch.no_grad():
+                call(**{name: asks})
+            with forward_ad.dual_level(), pytest.raises(ValueError, match="forward"):
+                call(**{name: forward_ad.make_dual(t, torch.ones_like(t))})
+    with pytest.raises(ValueError, match="backward"):
+        fp8.linear(x, fp8.BlockWeight(w.w8, w.scales.clone().requires_grad_()))
 
 
 # ---- refusals that need CUDA tensors ----------------------------------------------------------
