@@ -28,6 +28,8 @@ int check_heads(const void* p, long long st, long long sh, const char* what) {
   return TMU_OK;
 }
 
+bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 int check_packed(int T, int hq, int hkv, int D) {
   if (T < 0 || hq < 1 || hkv < 1 || D < 1) return fail(TMU_ERR_INVALID_ARGUMENT, "T, heads and D must be positive");
   if (T > 1 << 30) return fail(TMU_ERR_UNSUPPORTED, "T > 2^30");
@@ -188,6 +190,7 @@ int quantize_rows(const void* x, int dtype, long long ld, int M, int K, void* x8
   if (!x || !x8 || !scales) return fail(TMU_ERR_INVALID_ARGUMENT, "NULL tensor");
   if (ld < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows overlap: ld < K");
   if (!aligned16(x) || !aligned16(x8) || ld % 8) return fail(TMU_ERR_MISALIGNED, "x, x8 must be 16-byte aligned, ld a multiple of 8");
+  if (!aligned_to(scales, 4)) return fail(TMU_ERR_MISALIGNED, "scales not aligned to their type");
   Dev dev;
   int st = current_device(dev, 0, nullptr, 0);
   if (st) return st;
@@ -247,6 +250,8 @@ int tmu_qk_norm_rope(const tmu_qk_norm_rope_args* args, void* stream) {
   const float* par[4] = {norm->q_weight, norm->q_bias, norm->k_weight, norm->k_bias};
   for (const float* x : par)
     if (x != nullptr && !aligned16(x)) return fail(TMU_ERR_MISALIGNED, "norm parameter not 16-byte aligned");
+  if (rot->rot > 0 && (!aligned_to(rot->positions, rot->position_bytes) || !aligned_to(rot->turns, 8)))
+    return fail(TMU_ERR_MISALIGNED, "positions or turns not aligned to their type");
   Dev dev;
   if ((st = current_device(dev, 0, nullptr, 0))) return st;
   int lph = 2;
@@ -311,6 +316,8 @@ int tmu_attention(const tmu_attention_args* args, void* stream) {
     if ((st = check_heads(views[i]->data, views[i]->stride_token, views[i]->stride_head, names[i]))) return st;
   if (bias->n < 0 || (bias->n > 0 && !bias->data)) return fail(TMU_ERR_INVALID_ARGUMENT, "bias");
   if (!aligned16(status)) return fail(TMU_ERR_MISALIGNED, "status not 16-byte aligned");
+  if (!aligned_to(cu_seqlens, 4) || (bias->n > 0 && !aligned_to(bias->data, 2)))
+    return fail(TMU_ERR_MISALIGNED, "cu_seqlens or bias not aligned to its type");
   // a tensor map cannot step by 0
   const int heads[3] = {Hq, Hkv, Hkv};
   for (int i = 0; i < 3; ++i)
@@ -384,6 +391,9 @@ int tmu_linear_fp8(const void* x, int x_dtype, long long ldx, const float* x_sca
   if (ldo < N && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of out overlap: ldo < N");
   if (!aligned16(x) || !aligned16(w8)) return fail(TMU_ERR_MISALIGNED, "x, w8 must be 16-byte aligned");
   if (!aligned16(status)) return fail(TMU_ERR_MISALIGNED, "status not 16-byte aligned");
+  if (!aligned_to(out, out_dtype == TMU_F32 ? 4 : 2) || !aligned_to(w_scales, 4) || !aligned_to(bias, 4) ||
+      !aligned_to(x_scales, 4))
+    return fail(TMU_ERR_MISALIGNED, "out, a scale or bias not aligned to its type");
   if (x_dtype == TMU_E4M3 && ldx != K) return fail(TMU_ERR_UNSUPPORTED, "e4m3 x must be contiguous");
   if (ldx % 8) return fail(TMU_ERR_MISALIGNED, "ldx must be a multiple of 8");
   if (ldx < K && M > 1) return fail(TMU_ERR_INVALID_ARGUMENT, "rows of x overlap: ldx < K");

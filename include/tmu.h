@@ -336,7 +336,8 @@ int tmu_copy2d_async(void* dst, size_t dst_pitch, const void* src, size_t src_pi
  * MLX (mx.fast.scaled_dot_product_attention, mx.fast.rope, mx.quantized_matmul).  Inference only.
  *
  * A tensor of heads is [T, H, D]: values of a head contiguous, tokens and heads at element strides
- * that are multiples of 8 (so slices of one fused projection do), the base 16-byte aligned. */
+ * that are multiples of 8 (so slices of one fused projection do), the base 16-byte aligned.  Where no other
+ * alignment is stated, a pointer is aligned to what it points to (else TMU_ERR_MISALIGNED). */
 #define TMU_F16 0
 #define TMU_BF16 1
 #define TMU_F32 2

@@ -145,6 +145,21 @@ def test_workspace_of_e4m3_rows(lib):
     assert lib.tmu_linear_fp8_scaled_workspace_bytes(16, 8, 64) == 0
 
 
+def test_pointers_off_their_types_alignment(lib):
+    """Every pointer that a kernel follows one value at a time, an odd number of bytes off."""
+    assert attention(lib, cu=P + 2) == MISALIGNED
+    assert attention(lib, bias=_lib.TmuAttnBias(P + 1, 0, 0, 8, 4)) == MISALIGNED
+    assert rope(lib, pos=P + 2) == MISALIGNED and rope(lib, pos=P + 4, nbytes=8) == MISALIGNED
+    assert rope(lib, turns=P + 4) == MISALIGNED
+    for m in (1, 40):  # both kernels' ranges of rows
+        assert linear(lib, M=m, out=P + 1) == MISALIGNED
+        assert linear(lib, M=m, out=P + 2, od=_lib.TMU_F32) == MISALIGNED
+        assert linear(lib, M=m, ws=P + 2) == MISALIGNED
+        assert linear(lib, M=m, xd=_lib.TMU_E4M3, xs=P + 2) == MISALIGNED
+        assert lib.tmu_linear_fp8(P, 0, 64, None, P, P, P + 2, P, 0, 8, m, 8, 64, P, 1 << 20, None, None) == MISALIGNED
+    assert lib.tmu_quantize_rows(P, 0, 48, 2, 48, P, P + 2, None) == MISALIGNED
+
+
 def test_sizes_past_the_index_range(lib):
     big = (1 << 30) + 1
     assert linear(lib, M=big) == UNSUPPORTED and linear(lib, N=big, ldo=1 << 31) == UNSUPPORTED
