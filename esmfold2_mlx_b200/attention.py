@@ -180,8 +180,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
     """K8: the norm of every head of ``q`` [T, Hq, D] and ``k`` [T, Hkv, D] over its D values, then the
     rotation by ``positions`` [T] (int32 or int64), in one pass; returns ``(q_out, k_out)``.
 
-    ``norm`` is None, ``"rms"`` or ``"layer"``, with fp32 weights and biases [D] (None: 1 and 0); without
-    ``rotary`` only the norm is applied.  D is a multiple of 16, at most 256.  ``q_out`` may be ``q`` and
+    ``norm`` is None, ``"rms"`` or ``"layer"``, with fp32 weights and biases [D] (None: 1 and 0), ``eps`` 0 or
+    above (the mean square plus eps counts as 0 below 2^-126); without ``rotary`` only the norm is applied.  D is a multiple of 16, at most 256.  ``q_out`` may be ``q`` and
     ``k_out`` may be ``k``; other overlaps are refused."""
     dtype = _check_first("q", q)
     T, hq, D = q.shape

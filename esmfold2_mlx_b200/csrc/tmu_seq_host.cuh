@@ -238,6 +238,8 @@ int tmu_qk_norm_rope(const tmu_qk_norm_rope_args* args, void* stream) {
   if (D % 16 || D > 256) return fail(TMU_ERR_UNSUPPORTED, "D must be a multiple of 16, at most 256");
   if (dtype != TMU_F16 && dtype != TMU_BF16) return fail(TMU_ERR_UNSUPPORTED, "dtype must be fp16 or bf16");
   if (norm->kind < TMU_NORM_NONE || norm->kind > TMU_NORM_LAYER) return fail(TMU_ERR_INVALID_ARGUMENT, "norm kind");
+  if (norm->kind != TMU_NORM_NONE && !(norm->eps >= 0.0f && std::isfinite(norm->eps)))
+    return fail(TMU_ERR_INVALID_ARGUMENT, "eps must not be negative, and finite");
   if (rot->rot < 0 || rot->rot > D || rot->rot % 16)
     return fail(TMU_ERR_UNSUPPORTED, "the rotated part must be a multiple of 16, at most D");
   if (rot->rot > 0 && (!rot->positions || !rot->turns)) return fail(TMU_ERR_INVALID_ARGUMENT, "positions or turns is NULL");

@@ -354,7 +354,7 @@ typedef struct tmu_heads {
 
 typedef struct tmu_qk_norm {
   int kind;
-  float eps;
+  float eps; /* 0 or above; the mean square plus eps counts as 0 below 2^-126 */
   const float* q_weight; /* fp32 [D], 16-byte aligned, each may be NULL (1 and 0) */
   const float* q_bias;
   const float* k_weight;

@@ -109,6 +109,15 @@ def test_qk_norm_rope_refusals(lib):
     assert rope(lib, T=0) == OK
 
 
+@pytest.mark.parametrize("eps", [-1e-5, math.nan, math.inf])
+def test_norm_eps_refusals(lib, eps):
+    h = heads()
+    for kind, want in ((1, INVALID), (2, INVALID), (0, OK)):  # (T = 0: nothing is launched)
+        args = _lib.TmuQkNormRopeArgs(h, h, h, h, _lib.TmuQkNorm(kind, eps, None, None, None, None),
+                                      _lib.TmuRotary(None, 4, None, 1.0, 0, 0), 0, 1, 1, 64, 0)
+        assert lib.tmu_qk_norm_rope(ctypes.byref(args), None) == want
+
+
 def linear(lib, x=P, xd=0, ldx=64, xs=None, w=P, ws=P, out=P, od=0, ldo=8, M=40, N=8, K=64, work=P, nb=1 << 20):
     return lib.tmu_linear_fp8(x, xd, ldx, xs, w, ws, None, out, od, ldo, M, N, K, work, nb, None, None)
 
