@@ -181,7 +181,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor | Non
                  *, norm: str | None = None, q_weight=None, k_weight=None, q_bias=None, k_bias=None,
                  eps: float = 1e-5, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None):
     """K8: the norm of every head of ``q`` [T, Hq, D] and ``k`` [T, Hkv, D] over its D values, then the
-    rotation by ``positions`` [T] (int32 or int64), in one pass; returns ``(q_out, k_out)``.
+    rotation by ``positions`` [T] (int32 or int64), in one pass; returns ``(q_out, k_out)``.  (A norm over
+    all heads of a token together, as some models have before they split the heads, is another one: apply
+    it first and rotate with ``norm=None``.)
 
     ``norm`` is None, ``"rms"`` or ``"layer"``, with fp32 weights and biases [D] (None: 1 and 0), ``eps`` 0 or
     above (the mean square plus eps counts as 0 below 2^-126); without ``rotary`` only the norm is applied.  D is a multiple of 16, at most 256.  ``q_out`` may be ``q`` and

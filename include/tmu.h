@@ -25,6 +25,10 @@
  *     current call's first error (tmu_read_status; cleared by the first kernel of tmu_trimul and
  *     tmu_pair_block) and the first error since the block was last zeroed by tmu_reset_status
  *     (tmu_read_first_error; no kernel clears it, so one read covers a whole sequence of calls).
+ *   - The pair kernels with weights of their own (tmu_project_gate, tmu_emit_residual, tmu_disto and the
+ *     calls made of them) read those while the kernel in front of them in the stream may still run:
+ *     a weight is complete before that kernel starts, it is not that kernel's output.  The sequence
+ *     operators read nothing of theirs ahead.
  *   - Widths: c_z == c, 128 or 256 (the released ESMFold2 trunk's width, mlx_trunk.py:4);
  *     1 <= L <= 8192, B*c <= 65535.  Other sizes return TMU_ERR_UNSUPPORTED.  At c_z = 256,
  *     z_out must not overlap z (two CTAs share each tile's z): TMU_ERR_INVALID_ARGUMENT.
