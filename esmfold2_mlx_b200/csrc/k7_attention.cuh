@@ -6,10 +6,11 @@
 // that sees no key is zero.
 //
 // One pass over the keys with the running maximum m and sum l of the softmax (Milakov and Gimelshein
-// 2018), in base 2 (x times log2 e).  The accumulator O = sum_j 2^(x_ij - m) v_j stays in tensor memory, so moving m would
-// mean reading and writing all of it: m only moves (a published refinement of that pass) when a tile's maximum exceeds it by more than
-// 8, so weights reach at most 2^8 (exact in fp32 sums, and a common factor of the 16-bit weights;
-// fp16: kLift more), and the result, O / l, does not depend on when it moved.
+// 2018), in base 2 (x times log2 e).  The accumulator O = sum_j 2^(x_ij - m) v_j stays in tensor memory,
+// so moving m would mean reading and writing all of it: m only moves when a tile's maximum exceeds it by
+// more than 8 (a published refinement of that pass), so weights reach at most 2^8 (exact in fp32 sums, and
+// a common factor of the 16-bit weights; fp16: kLift more), and the result, O / l, does not depend on when
+// it moved.
 //
 // A tile is 128 rows of one head; a step takes 128 keys: S = Q K^T (128 x 128, fp32 in TMEM), the
 // softmax of S's rows, P in TMEM in the inputs' type, and O += P V with P as the MMA's A operand out of
@@ -152,10 +153,10 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 
 // 2^t of a pair, t <= kMoveMax + kLift or so, on the fused multiply-add units, by the reduction and
 // polynomial of Cody and Waite 1980 (sharing a softmax's exponentials between the two units is published
-// too): t = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits) and |f| <= 1/2, 2^f by a polynomial of degree 4
-// with constant term 1 (minimax in the relative error, 2^-18.4, against 2^-9 and 2^-11 of the weights'
-// types), n added to the exponent.  t is held at -127 or above, where the sum of exponents is
-// exactly 0: -inf gives +0.  A NaN is lost.
+// too): t = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits) and |f| <= 1/2,
+// 2^f by a polynomial of degree 4 with constant term 1 (minimax in the relative error, 2^-18.4, against 2^-9
+// and 2^-11 of the weights' types), n added to the exponent.  t is held at -127 or above, where the sum of
+// exponents is exactly 0: -inf gives +0.  A NaN is lost.
 __device__ __forceinline__ float2 exp2_fma(float2 t) {
   t = make_float2(fmaxf(t.x, -127.f), fmaxf(t.y, -127.f));
   const float2 r = __fadd2_rn(t, make_float2(12582912.f, 12582912.f));
